@@ -191,6 +191,122 @@ TL_API tl_status tl_quantize_i8(int8_t* q, float* scales, const float* x, size_t
                                 size_t group, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Serving step over a paged KV cache.  No counterpart in the reference,     */
+/* whose InferenceState (inference_state.h:8-72) holds one sequence in one   */
+/* contiguous cache.  A step runs tl_paged_plan once, tl_qk_norm_rope and    */
+/* tl_paged_attention once per layer, and tl_sample_rows once.  All lengths, */
+/* tables and parameters of requests are device arrays (int32 / fp32), so a  */
+/* step can be captured in a CUDA graph and replayed with new contents.      */
+/* They are not read on the host: an entry out of range never makes a        */
+/* kernel access memory outside the arrays given; what it means is said      */
+/* below.  Rows that belong to no sequence are left as they were.            */
+/* ------------------------------------------------------------------------ */
+
+typedef enum tl_dtype { TL_F32 = 0, TL_F16 = 1, TL_BF16 = 2 } tl_dtype;
+
+/* One layer's pages.  k and v (device): page b, kv head g, row t of the page
+ * is the head_dim contiguous elements at
+ *   b * block_stride + (g * block_size + t) * head_dim.
+ * block_stride (elements) >= n_kv_heads * block_size * head_dim, so K and V
+ * pages may be interleaved or belong to a larger array.  block_size is a power
+ * of two from 8 to 256, head_dim 64 or 128; k, v and block_stride are aligned
+ * to 16 bytes.  n_blocks * block_size must stay below 2^31. */
+typedef struct tl_paged_cache {
+    void* k;
+    void* v;
+    size_t n_blocks, n_kv_heads, block_size, head_dim;
+    size_t block_stride;
+    tl_dtype dtype;
+} tl_paged_cache;
+
+/* Block tables and slot maps of one step.  Request b of n_req has cached[b]
+ * tokens in its pages and brings new_tokens[b] (negative counts as 0).  The
+ * tokens of all requests lie one after the other in n_tokens rows:
+ *   q_start[n_req + 1]  first row of each request (the running sum, cut at n_tokens)
+ *   seq_lens[n_req]     cached + the new tokens that have rows
+ *   block_table[n_req][max_blocks], in place: a request's first
+ *       ceil(cached / block_size) entries stay, the entries that its new tokens
+ *       need get the next ids of free_blocks[n_free] (in request order), -1
+ *       once the list is used up; entries past max_blocks do not exist
+ *   positions[n_tokens] position of each row's token in its sequence
+ *   slots[n_tokens]     page id * block_size + offset in the page; -1 for a
+ *       token without a page
+ *   counts[2]           ids taken from free_blocks; ids missing
+ * Rows behind the last request get position and slot -1.  n_req = 0 or
+ * n_tokens = 0 are allowed.  n_req * max_blocks and n_tokens must stay below 2^31. */
+TL_API tl_status tl_paged_plan(int32_t* block_table, int32_t* q_start, int32_t* seq_lens, int32_t* positions,
+                               int32_t* slots, int32_t* counts, const int32_t* cached, const int32_t* new_tokens,
+                               const int32_t* free_blocks, size_t n_free, size_t n_req, size_t max_blocks,
+                               size_t block_size, size_t n_tokens, void* stream);
+
+/* RMSNorm of every q and k head (modules.cpp:31-46 over head_dim; skipped for
+ * the side whose weight is NULL), rotation of the first rot_dim dims (pairs
+ * (i, i + rot_dim / 2) by cos_ / sin_[positions[t]][i], kernels.cpp:78-95; the
+ * rest stays) and the write of k and v into their pages, in one pass.
+ *   qkv      rows of [q heads | k heads | v heads] x head_dim in `dtype`,
+ *            row_stride elements apart (>= (n_heads + 2 n_kv_heads) head_dim)
+ *   q_out    [n_tokens][n_heads][head_dim] in the cache's dtype
+ *   cos_, sin_  fp32 [n_pos][rot_dim / 2]; q_weight, k_weight fp32 [head_dim]
+ *   slots    as tl_paged_plan gives them
+ * A row whose position is not in [0, n_pos) belongs to no sequence: nothing is
+ * written for it.  A row whose slot names no page of the cache gets its q, and
+ * no cache write.  Two rows with one slot leave either's k and v there.
+ * Arithmetic is fp32, rounded once.  rot_dim is a multiple of 16 up to
+ * head_dim; pointers and row_stride are aligned to 16 bytes; q_out does not
+ * overlap qkv. */
+TL_API tl_status tl_qk_norm_rope(void* q_out, const tl_paged_cache* cache, const void* qkv, tl_dtype dtype,
+                                 size_t row_stride, const int32_t* positions, const int32_t* slots,
+                                 const float* cos_, const float* sin_, size_t n_pos, size_t rot_dim,
+                                 const float* q_weight, const float* k_weight, float eps, size_t n_tokens,
+                                 size_t n_heads, void* stream);
+
+/* Causal GQA attention of new tokens over the pages (modules.cpp:65-88 for
+ * many sequences; q head h reads kv head h / (n_heads / n_kv_heads)).
+ * Sequence b has the query rows q_start[b] .. q_start[b + 1) and seq_lens[b]
+ * cached tokens, the queries' own among them: its i-th query of n stands at
+ * position p = seq_lens[b] - n + i and attends to the positions
+ * max(0, p - window + 1) .. p (window 0: all of 0 .. p) whose table entry
+ * names a page of the cache.  What is not attended (other sequences' pages,
+ * rows of a page behind the sequence, entries out of range) does not reach the
+ * result, not even as NaN or infinity.  A query that attends to nothing gets
+ * zeros.  A single query per sequence is a decode step.
+ *   q    rows of n_heads x head_dim, q_stride elements apart; out [n_tokens]
+ *        [n_heads][head_dim], both in the cache's dtype, not overlapping
+ *   block_table [n_seq][max_blocks]; q_start [n_seq + 1], not decreasing
+ * Rows outside q_start[0] .. q_start[n_seq] stay as they were.  Scores and sums
+ * are fp32; with fp16 / bf16 caches the weights of the values are rounded to
+ * that type for the tensor cores.  `workspace` holds the partial results
+ * of split sequences: tl_paged_attention_workspace bytes, 16-byte aligned, its
+ * contents need no preparation; calls that may overlap in time need one each.
+ * A captured call keeps using the workspace it was captured with. */
+TL_API tl_status tl_paged_attention_workspace(const tl_paged_cache* cache, size_t n_tokens, size_t n_heads,
+                                              size_t n_seq, size_t max_blocks, size_t* bytes);
+TL_API tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl_paged_cache* cache,
+                                    const int32_t* block_table, size_t max_blocks, const int32_t* q_start,
+                                    const int32_t* seq_lens, size_t n_seq, size_t n_tokens, size_t n_heads,
+                                    float scale, size_t window, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
+/* tl_sample_multinomial for n_rows rows at once, each with its own settings
+ * (device arrays of n_rows; top_k, top_p and min_p may be NULL: off):
+ *   w_i = exp((x_i - max) / temperature); order: w descending, equal logits by
+ *   lowest index;
+ *   top_k  keeps the first k of the order        (k <= 0 or >= n: off)
+ *   top_p  keeps its shortest prefix whose sum reaches top_p x the sum of what
+ *          top_k left (at least one)             (>= 1 or NaN: off)
+ *   min_p  keeps those with w >= min_p (max has w = 1)  (<= 0 or NaN: off)
+ * out[row] = the first kept index, in index order, whose running sum of kept w
+ * reaches r x (sum of all kept w); r in [0, 1).  temperature <= 0 or NaN:
+ * sample_max (main.cpp:10-21).  A row with a NaN or +inf logit, or with -inf
+ * alone, gives n - 1 at a temperature > 0, as tl_sample_multinomial does.
+ * Weights are fp64 rounded to multiples of 2^-40 and summed exactly, so the
+ * result does not depend on the order of the sums.  logits: n values per row
+ * in `dtype`, row_stride elements apart; n < 2^22.  No allocation. */
+TL_API tl_status tl_sample_rows(uint32_t* out, const void* logits, tl_dtype dtype, size_t row_stride, size_t n_rows,
+                                size_t n, const float* r, const float* temperature, const int32_t* top_k,
+                                const float* top_p, const float* min_p, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Model level: Parameters + InferenceState + Model<T> on one device.        */
 /* ------------------------------------------------------------------------ */
 

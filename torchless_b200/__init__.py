@@ -7,7 +7,9 @@ interfaces for the path:
 * ``ops``            - src/common/kernels.h (matmul, row_matmul, softmax, rope,
                        silu, sum, add, mul, pow, sqrt) plus rmsnorm, rotary,
                        argmax (sample_max), the fused gate/up and the quantiser,
-                       on CUDA tensors;
+                       and the operators of a serving step over a paged cache
+                       (paged_plan, qk_norm_rope, paged_attention,
+                       sample_rows), on CUDA tensors;
 * ``Model``          - Parameters::load_parameters + InferenceState +
                        Model<int8_t>::forward (src/loader, src/model/mistral),
                        device resident;
@@ -55,6 +57,12 @@ class tl_model_options(ctypes.Structure):
                 ("sliding_window", ctypes.c_int), ("weights_f16", ctypes.c_int)]
 
 
+class tl_paged_cache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_blocks", ctypes.c_size_t),
+                ("n_kv_heads", ctypes.c_size_t), ("block_size", ctypes.c_size_t), ("head_dim", ctypes.c_size_t),
+                ("block_stride", ctypes.c_size_t), ("dtype", ctypes.c_int)]
+
+
 TP_HANDLE_BYTES = 64
 
 
@@ -94,6 +102,13 @@ SIGNATURES = {
     "tl_model_set_sampling": [_P, _F, ctypes.c_uint64],
     "tl_mlp_gate_up": [_P, _P, _P, _P, _P, _P, _S, _S, _P],
     "tl_quantize_i8": [_P, _P, _P, _S, _S, _P],
+    "tl_paged_plan": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _S, _S, _S, _S, _P],
+    "tl_qk_norm_rope": [_P, ctypes.POINTER(tl_paged_cache), _P, _I, _S, _P, _P, _P, _P, _S, _S, _P, _P, _F, _S, _S,
+                        _P],
+    "tl_paged_attention_workspace": [ctypes.POINTER(tl_paged_cache), _S, _S, _S, _S, ctypes.POINTER(_S)],
+    "tl_paged_attention": [_P, _P, _S, ctypes.POINTER(tl_paged_cache), _P, _S, _P, _P, _S, _S, _S, _F, _S, _P, _S,
+                           _P],
+    "tl_sample_rows": [_P, _P, _I, _S, _S, _S, _P, _P, _P, _P, _P, _P],
     "tl_gemm_f16": [_P, _P, _P, _S, _S, _S, _S, _I, _P],
     "tl_gemm_q8": [_P, _P, _P, _P, _P, _P, _S, _S, _S, _S, _I, _P],
     "tl_model_load": [ctypes.c_char_p, ctypes.POINTER(tl_model_options), ctypes.POINTER(_P)],

@@ -153,3 +153,197 @@ def quantize_i8(x, group: int = 64):
     s = torch.empty(xc.numel() // group, dtype=torch.float32, device=x.device)
     check(lib().tl_quantize_i8(_ptr(q), _f32(s), _f32(xc), xc.numel(), group, _stream()))
     return q, s
+
+
+# ---- serving step over a paged KV cache (no reference counterpart: its
+# InferenceState, inference_state.h:8-72, holds one sequence) ----
+#
+# The pages of a layer are two tensors k_cache, v_cache
+# [n_blocks, n_kv_heads, block_size, head_dim] (float32, float16 or bfloat16),
+# contiguous but for the stride between pages.  Lengths, tables and settings
+# of requests are int32 / float32 tensors on the device, never read by the
+# host, so a step can be captured in a CUDA graph.
+
+
+class _On:
+    """Makes a tensor's device current for a call where it is not."""
+
+    def __init__(self, device):
+        import torch
+        self.torch, self.device, self.before = torch, device, -1
+
+    def __enter__(self):
+        cur = self.torch.cuda.current_device()
+        if cur != self.device.index:
+            self.before = cur
+            self.torch.cuda.set_device(self.device)
+        return ctypes.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.before >= 0:
+            self.torch.cuda.set_device(self.before)
+
+
+_DTYPES = None
+
+
+def _dtype(t) -> int:
+    global _DTYPES
+    if _DTYPES is None:
+        import torch
+        _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}") from None
+
+
+def _arg(t, dtype, device, n=None, name="argument"):
+    """A contiguous tensor of `dtype` on `device` with n elements: its address."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if n is not None and t.numel() != n:
+        raise ValueError(f"{name} has {t.numel()} elements, not {n}")
+    return t.data_ptr()
+
+
+def _cache(k_cache, v_cache):
+    from . import tl_paged_cache
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise ValueError("k_cache and v_cache must be [n_blocks, n_kv_heads, block_size, head_dim] of one layout")
+    if k_cache.dtype != v_cache.dtype or k_cache.device != v_cache.device or not k_cache.is_cuda:
+        raise ValueError("k_cache and v_cache must be CUDA tensors of one type and device")
+    n, kv, bs, hd = k_cache.shape
+    st = k_cache.stride()
+    if st[1:] != (bs * hd, hd, 1):
+        raise ValueError("the pages of a cache must be contiguous")
+    return tl_paged_cache(k=k_cache.data_ptr(), v=v_cache.data_ptr(), n_blocks=n, n_kv_heads=kv, block_size=bs,
+                          head_dim=hd, block_stride=max(st[0], kv * bs * hd) if n == 1 else st[0],
+                          dtype=_dtype(k_cache))
+
+
+def paged_plan(block_table, cached, new_tokens, free_blocks, block_size: int, n_tokens: int):
+    """Block tables and slot maps of a step from the request lengths.
+
+    ``block_table`` [n_req, max_blocks] is extended in place by the pages that
+    the new tokens need, taken from ``free_blocks`` in order (-1 once it is used
+    up).  ``cached`` and ``new_tokens`` [n_req] are each request's tokens
+    before and in this step; the new tokens lie one after the other in
+    ``n_tokens`` rows.  Returns int32 tensors
+    ``(q_start [n_req + 1], seq_lens [n_req], positions [n_tokens],
+    slots [n_tokens], counts [2])``; position and slot are -1 in rows behind
+    the last token, the slot of a token without a page is -1, and counts are
+    the pages taken and the pages missing."""
+    import torch
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [n_req, max_blocks]")
+    n_req, width = block_table.shape
+    dev, i32 = block_table.device, torch.int32
+    if not block_table.is_cuda:
+        raise ValueError("ops take CUDA tensors")
+    if n_tokens < 0 or block_size < 0:
+        raise ValueError("n_tokens and block_size must not be negative")
+    t, c, f = (_arg(block_table, i32, dev, name="block_table"), _arg(cached, i32, dev, n_req, "cached"),
+               _arg(new_tokens, i32, dev, n_req, "new_tokens"))
+    fr = _arg(free_blocks, i32, dev, name="free_blocks")
+    out = torch.empty(2 * n_req + 1 + 2 * n_tokens + 2, dtype=i32, device=dev)
+    q_start, seq_lens, positions, slots, counts = parts = out.split([n_req + 1, n_req, n_tokens, n_tokens, 2])
+    with _On(dev) as s:
+        check(lib().tl_paged_plan(t, q_start.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+                                  counts.data_ptr(), c, f, fr, free_blocks.numel(), n_req, width, block_size, n_tokens, s))
+    return parts
+
+
+def qk_norm_rope(q_out, k_cache, v_cache, qkv, positions, slots, cos, sin, q_weight=None, k_weight=None,
+                 eps: float = 1e-5) -> None:
+    """RMSNorm of each q and k head (where its weight is given), rotation and
+    the write of k and v into their pages, in one pass.
+
+    ``qkv`` [n_tokens, (n_heads + 2 n_kv_heads) * head_dim] (rows may be
+    strided), ``q_out`` [n_tokens, n_heads, head_dim] in the cache's type,
+    ``positions`` / ``slots`` as paged_plan gives them, ``cos`` / ``sin``
+    float32 [n_pos, rot_dim / 2].  Rows with a position outside the tables are
+    left alone; rows without a page get their q only."""
+    import torch
+    c = _cache(k_cache, v_cache)
+    dev, f32 = k_cache.device, torch.float32
+    if q_out.dim() != 3 or q_out.shape[2] != c.head_dim or q_out.dtype != k_cache.dtype:
+        raise ValueError("q_out must be [n_tokens, n_heads, head_dim] in the cache's type")
+    n, heads, hd = q_out.shape
+    if qkv.dim() != 2 or qkv.shape != (n, (heads + 2 * c.n_kv_heads) * hd) or (n and qkv.stride(1) != 1):
+        raise ValueError("qkv must be [n_tokens, (n_heads + 2 n_kv_heads) * head_dim]")
+    if qkv.device != dev:
+        raise ValueError(f"qkv is on {qkv.device}, not {dev}")
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError("cos and sin must be [n_pos, rot_dim / 2]")
+    stride = qkv.stride(0) if n > 1 else qkv.shape[1]
+    with _On(dev) as s:
+        check(lib().tl_qk_norm_rope(
+            _arg(q_out, q_out.dtype, dev, name="q_out"), ctypes.byref(c), qkv.data_ptr(), _dtype(qkv), stride,
+            _arg(positions, torch.int32, dev, n, "positions"), _arg(slots, torch.int32, dev, n, "slots"),
+            _arg(cos, f32, dev, name="cos"), _arg(sin, f32, dev, name="sin"), cos.shape[0], 2 * cos.shape[1],
+            None if q_weight is None else _arg(q_weight, f32, dev, hd, "q_weight"),
+            None if k_weight is None else _arg(k_weight, f32, dev, hd, "k_weight"), float(eps), n, heads, s))
+
+
+def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, scale=None, window: int = 0) -> None:
+    """Causal GQA attention of each sequence's new tokens over its pages.
+
+    ``q`` and ``out`` [n_tokens, n_heads, head_dim] in the cache's type (``q``
+    may be strided between tokens); sequence b has the rows q_start[b] ..
+    q_start[b + 1), which are the last of its seq_lens[b] tokens.  ``scale``
+    defaults to 1 / sqrt(head_dim); ``window`` > 0 attends to that many last
+    positions.  A query that attends to nothing gets zeros; rows of no sequence
+    are left as they were."""
+    import torch
+    c = _cache(k_cache, v_cache)
+    dev, i32 = k_cache.device, torch.int32
+    if q.dim() != 3 or q.shape[2] != c.head_dim or q.dtype != k_cache.dtype or q.shape != out.shape \
+            or out.dtype != q.dtype:
+        raise ValueError("q and out must be [n_tokens, n_heads, head_dim] in the cache's type")
+    n, heads, hd = q.shape
+    if n and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != hd)):
+        raise ValueError("the heads of a token must be contiguous in q")
+    if q.device != dev:
+        raise ValueError(f"q is on {q.device}, not {dev}")
+    if block_table.dim() != 2 or window < 0:
+        raise ValueError("block_table must be [n_seq, max_blocks] and window not negative")
+    n_seq, width = block_table.shape
+    args = (_arg(block_table, i32, dev, name="block_table"), width, _arg(q_start, i32, dev, n_seq + 1, "q_start"),
+            _arg(seq_lens, i32, dev, n_seq, "seq_lens"), n_seq, n, heads)
+    need = ctypes.c_size_t()
+    L = lib()
+    check(L.tl_paged_attention_workspace(ctypes.byref(c), n, heads, n_seq, width, ctypes.byref(need)))
+    with _On(dev) as s:
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        check(L.tl_paged_attention(
+            _arg(out, out.dtype, dev, name="out"), q.data_ptr(), q.stride(0) if n > 1 else heads * hd, ctypes.byref(c),
+            *args, hd ** -0.5 if scale is None else float(scale), int(window), ws.data_ptr(), need.value, s))
+
+
+def sample_rows(logits, r, temperature, top_k=None, top_p=None, min_p=None):
+    """sample_multinomial for each row of ``logits`` [n_rows, n] (float32,
+    float16 or bfloat16; rows may be strided) with the row's own uniform draw
+    ``r`` in [0, 1), ``temperature`` (<= 0: sample_max), and optionally
+    ``top_k`` (int32; <= 0: off), ``top_p`` (>= 1: off) and ``min_p`` (<= 0:
+    off), applied in that order.  Returns the indexes, an int32 tensor [n_rows]."""
+    import torch
+    if logits.dim() != 2 or (logits.shape[0] and logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [n_rows, n] with contiguous rows")
+    if not logits.is_cuda:
+        raise ValueError("ops take CUDA tensors")
+    rows, n = logits.shape
+    dev, f32 = logits.device, torch.float32
+    ptrs = (_arg(r, f32, dev, rows, "r"), _arg(temperature, f32, dev, rows, "temperature"),
+            None if top_k is None else _arg(top_k, torch.int32, dev, rows, "top_k"),
+            None if top_p is None else _arg(top_p, f32, dev, rows, "top_p"),
+            None if min_p is None else _arg(min_p, f32, dev, rows, "min_p"))
+    with _On(dev) as s:
+        out = torch.empty(rows, dtype=torch.int32, device=dev)
+        check(lib().tl_sample_rows(out.data_ptr(), logits.data_ptr(), _dtype(logits),
+                                   logits.stride(0) if rows > 1 else n, rows, n, *ptrs, s))
+    return out
