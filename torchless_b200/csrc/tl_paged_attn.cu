@@ -1,36 +1,816 @@
-// tl_paged_attn.cu -- tl_paged_attention: causal GQA attention of new tokens
-// over a paged KV cache.
+// tl_paged_attn.cu -- tl_paged_attention: entry points, and the kernel for few
+// query rows per sequence (decode steps).
+//
+// Every key is read once for all query rows that share its kv head, and with so
+// few rows the reading is what takes the time: 2 * size * hd bytes a key and kv
+// head against at most 16 rows of arithmetic.  So the kernel is built to keep
+// HBM busy whatever the lengths are:
+//   - The work of the whole call, counted in steps of 16 keys (8 for fp32), is
+//     cut into one equal share per SM, across sequences, kv heads and the middle
+//     of a sequence.  Each block finds its share by a scan over the lengths on
+//     the device: no length is known to the host, and a batch of unlike lengths
+//     is as balanced as one of equal ones.
+//   - In a block, 8 warps take the steps of a tile in turn.  Each has its own
+//     ring of stages that lane 0 fills by TMA (a page's rows, both panels, one
+//     instruction for K and one for V), running ahead into the next tiles; no
+//     barrier is shared in the loop.
+//   - fp16 / bf16: scores and values on mma.sync m16n8k16 (16 rows fill the
+//     instruction's height; tcgen05's 128 would be nearly empty, and its rate is
+//     not what bounds).  The weights enter as a sum of two 16-bit numbers, so
+//     that only the result's own rounding remains.  fp32: FMA.
+//   - At a tile's end the warps join (max, sum, accumulator) in shared memory;
+//     a tile that continues in another block leaves its part in the workspace,
+//     and a second small kernel joins the parts in order.
 #include <math.h>
 
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "tl_paged_attn.cuh"
 
 namespace tl {
 namespace paged {
-namespace {
 
-// Warp = one (token, head): lanes hold HD / 32 dims, one online softmax over
-// the attended keys.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) k_attend_rows(AttendArgs a) {
-    const int lane = threadIdx.x & 31;
-    const long long u = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    if (u >= static_cast<long long>(a.n_tokens) * a.H) return;
-    const int t = static_cast<int>(u / a.H), h = static_cast<int>(u % a.H);
-    const int b = sequence_of(a, t);
-    if (b < 0) return;
-    attend_row<T, HD>(a, b, t, h, lane);
+using namespace tc;
+
+tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache* c, int rows) {
+    auto fn = encode_fn();
+    if (!fn) return set_error(TL_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const bool wide = c->dtype == TL_F32;
+    const size_t es = dtype_size(c->dtype);
+    const cuuint32_t cols = wide ? static_cast<cuuint32_t>(c->head_dim) : 64u;
+    const cuuint32_t panels = static_cast<cuuint32_t>(c->head_dim) / cols;
+    const cuuint64_t dims[4] = {cols, c->n_kv_heads * c->block_size, panels, c->n_blocks};
+    const cuuint64_t strides[3] = {c->head_dim * es, cols * es, c->block_stride * es};
+    const cuuint32_t box[4] = {cols, static_cast<cuuint32_t>(rows), panels, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map,
+                          wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                               : c->dtype == TL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          wide ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(TL_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return TL_OK;
 }
 
+namespace {
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int row, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4}], [%5];" ::
+            "r"(su32(dst)), "l"(map), "r"(0), "r"(row), "r"(page), "r"(su32(bar))
+        : "memory");
+}
+
+// Keys per step, stages per warp, and the bytes of one side of a stage.
+template <typename T, int HD>
+struct Shape {
+    static constexpr int KS = std::is_same<T, float>::value ? 8 : 16;
+    static constexpr int SIDE = KS * HD * static_cast<int>(sizeof(T));
+    static constexpr int NST = SIDE >= 4096 ? 3 : 5;
+    static constexpr int JOIN = 8 * (HD + 4);  // floats of one warp's 8 rows: {max, sum, flag, -, values}
+    static constexpr size_t SMEM = 1024 + static_cast<size_t>(kWarps) * NST * 2 * SIDE + kWarps * JOIN * 4 + 512;
+};
+
+// What one block leaves behind of a tile that it begins and others end.
+struct Head {
+    int parts, slot, b, rt, g;
+};
+
+// Units (steps) of one tile; a tile without keys counts one, so that its zeros get written.
+template <int KS>
+__device__ __forceinline__ int steps_of(const Tile& t) {
+    if (t.hi <= t.lo) return 1;
+    return (t.hi - 1) / KS - t.lo / KS + 1;
+}
+
+// Place in the call's work: tile (b, rt, g) and the steps [s, end) of it that belong to this block.
+struct Cursor {
+    int b, rt, g;
+    int s, end, steps;
+    long long left;  // units of the block from this tile's step s on
+    Tile t;
+};
+
+template <int R, int KS>
+__device__ __forceinline__ void enter(const AttendArgs& a, Cursor& c) {
+    c.t = tile_of(a, c.b, c.rt, R);
+    c.steps = steps_of<KS>(c.t);
+    c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
+}
+// To the next tile that has rows; false when the block's share is done.
+template <int R, int KS>
+__device__ __forceinline__ bool next_tile(const AttendArgs& a, Cursor& c) {
+    c.left -= c.end - c.s;
+    if (c.left <= 0) return false;
+    c.s = 0;
+    if (++c.g == a.KV) {
+        c.g = 0;
+        c.rt++;
+        while (c.rt * R >= c.t.n * a.group) {  // sequences without rows have no units
+            if (++c.b >= a.n_seq) return false;
+            c.rt = 0;
+            rows_of(a, c.b, c.t.first, c.t.n);
+        }
+    }
+    enter<R, KS>(a, c);
+    return true;
+}
+
+// ---- arithmetic of one warp -------------------------------------------------
+
+// One step's bounds: keys [key0, key0 + KS), page halves that exist (bit 0: first 8 keys, bit 1: the rest).
+struct StepInfo {
+    int key0;
+    uint32_t valid;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
 template <typename T>
-void launch_rows(const AttendArgs& a, int hd, cudaStream_t s) {
-    const unsigned grid = static_cast<unsigned>((static_cast<long long>(a.n_tokens) * a.H + 3) / 4);
-    if (hd == 128) k_attend_rows<T, 128><<<grid, 128, 0, s>>>(a);
-    else k_attend_rows<T, 64><<<grid, 128, 0, s>>>(a);
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two floats as 16-bit halves of a word, and what the rounding left of them.
+__device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo, __half*) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo, __nv_bfloat16*) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 16 rows on the matrix instruction: lane l holds rows l / 4 and l / 4 + 8.
+template <typename T, int HD, int R>
+struct Core {
+    static_assert(R == 16, "the instruction's height");
+    static constexpr int NO = HD / 8;
+    uint32_t q[HD / 16][4];
+    float o[NO][4];
+    float m[2], l[2];
+    int lo[2], hi[2];  // this lane's rows' attended positions
+    int hs, ps;        // bytes between the 8-key halves and between the panels of a side
+
+    __device__ void begin(const AttendArgs& a, const Cursor& c, int lane) {
+        const T* qb = static_cast<const T*>(a.q);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = lane / 4 + 8 * i;
+            const bool in = r < c.t.nrows;
+            const int fr = c.t.r0 + (in ? r : 0);
+            const int tok = fr / a.group, h = c.g * a.group + fr % a.group;
+            attended(a, c.t.p0 + tok, lo[i], hi[i]);
+            if (!in) hi[i] = 0;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(
+                qb + static_cast<size_t>(c.t.first + tok) * a.q_stride + static_cast<size_t>(h) * HD) + (lane & 3);
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++) {
+                q[k][i] = in ? src[8 * k] : 0u;
+                q[k][2 + i] = in ? src[8 * k + 4] : 0u;
+            }
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < NO; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        hs = 1024;
+        ps = 2048;
+        if (a.shift == 3) {
+            hs = 1024 * (HD / 64);
+            ps = 1024;
+        }
+    }
+
+    __device__ __forceinline__ uint32_t at(int key, int chunk) const {  // byte offset of 8 dims of a key
+        return static_cast<uint32_t>((key >> 3) * hs + (chunk >> 3) * ps + (key & 7) * 128 +
+                                     (((chunk & 7) ^ (key & 7)) << 4));
+    }
+
+    __device__ void step(const AttendArgs& a, const Cursor& c, StepInfo si, const uint8_t* sk, const uint8_t* sv,
+                         int lane) {
+        float s[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        const uint32_t kb = su32(sk), vb = su32(sv);
+        {
+            const int key = (lane >> 4) * 8 + (lane & 7), c0 = (lane >> 3) & 1;
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++) {
+                uint32_t r[4];
+                ldsm4(r, kb + at(key, 2 * k + c0));
+                mma16<T>(s[0], q[k], r[0], r[1]);
+                mma16<T>(s[1], q[k], r[2], r[3]);
+            }
+        }
+        const float sl = a.scale * 1.4426950408889634f;  // log2 units
+        // every row attends to every key of an inner step
+        const bool edge = si.valid != 3u || si.key0 < c.t.lo_last || si.key0 > c.t.hi_first - 16;
+        const int kc = si.key0 + 2 * (lane & 3);
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[n][e] *= sl;
+                if (edge) {
+                    const int key = kc + 8 * n + (e & 1), i = e >> 1;
+                    if (!(key >= lo[i] && key < hi[i] && ((si.valid >> n) & 1))) s[n][e] = -INFINITY;
+                }
+            }
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float mx = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
+            const float mn = fmaxf(m[i], mx);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            f[i] = ex2(m[i] - base);
+            m[i] = mn;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) s[n][2 * i + e] = ex2(s[n][2 * i + e] - base);
+            l[i] = l[i] * f[i] + ((s[0][2 * i] + s[0][2 * i + 1]) + (s[1][2 * i] + s[1][2 * i + 1]));
+        }
+        if (__any_sync(FULL, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+            for (int n = 0; n < NO; n++) {
+                o[n][0] *= f[0];
+                o[n][1] *= f[0];
+                o[n][2] *= f[1];
+                o[n][3] *= f[1];
+            }
+        }
+        uint32_t ph[4], pl[4];
+        ph[0] = split2(s[0][0], s[0][1], pl[0], static_cast<T*>(nullptr));
+        ph[1] = split2(s[0][2], s[0][3], pl[1], static_cast<T*>(nullptr));
+        ph[2] = split2(s[1][0], s[1][1], pl[2], static_cast<T*>(nullptr));
+        ph[3] = split2(s[1][2], s[1][3], pl[3], static_cast<T*>(nullptr));
+        // keys that no row attends to must not reach the products (0 x NaN)
+        uint32_t keep[2] = {~0u, ~0u};
+        if (edge) {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int key = kc + 8 * n + e;
+                    if (!(key >= c.t.lo && key < c.t.hi && ((si.valid >> n) & 1))) keep[n] &= e ? 0xffffu : 0xffff0000u;
+                }
+        }
+        const int vkey = ((lane >> 3) & 1) * 8 + (lane & 7), vc = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < HD / 16; j++) {
+            uint32_t r[4];
+            ldsm4t(r, vb + at(vkey, 2 * j + vc));
+            if (edge) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) r[u] &= keep[u & 1];
+            }
+            mma16<T>(o[2 * j], ph, r[0], r[1]);
+            mma16<T>(o[2 * j + 1], ph, r[2], r[3]);
+            mma16<T>(o[2 * j], pl, r[0], r[1]);
+            mma16<T>(o[2 * j + 1], pl, r[2], r[3]);
+        }
+    }
+
+    // Sums over the lanes; whether a result of this lane is not finite.
+    __device__ bool finish(int nrows, int lane) {
+        float z = 0.f;  // NaN once a value is not finite
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            l[i] += __shfl_xor_sync(FULL, l[i], 1);
+            l[i] += __shfl_xor_sync(FULL, l[i], 2);
+            if (lane / 4 + 8 * i < nrows) {
+                z = fmaf(l[i], 0.f, z);
+#pragma unroll
+                for (int n = 0; n < NO; n++) z = fmaf(o[n][2 * i], 0.f, fmaf(o[n][2 * i + 1], 0.f, z));
+            }
+        }
+        return z != z;
+    }
+    // rows 8 * pass .. of this warp into its part of the join buffer
+    __device__ void dump(float* j, int pass, int lane) const {
+        float* row = j + (lane >> 2) * (HD + 4);
+        if ((lane & 3) == 0) {
+            row[0] = pass ? m[1] : m[0];
+            row[1] = pass ? l[1] : l[0];
+        }
+#pragma unroll
+        for (int n = 0; n < NO; n++)
+            *reinterpret_cast<float2*>(row + 4 + 8 * n + 2 * (lane & 3)) =
+                pass ? make_float2(o[n][2], o[n][3]) : make_float2(o[n][0], o[n][1]);
+    }
+};
+
+// fp32: lane l holds dims l * HD / 32 ... of R rows; the R x 8 partial dot
+// products of a step are reduced together (transposed reduction), after which
+// lane l has the score of row 4 * rg + l / 8 and key l % 8.
+template <int HD, int R>
+struct Core<float, HD, R> {
+    static constexpr int D = HD / 32, RG = R / 4;
+    float q[R][D], o[R][D], m[R];
+    float l[RG];
+    int lo[RG], hi[RG];
+
+    __device__ __forceinline__ static void load(float (&v)[D], const float* p) {
+        if constexpr (D == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+            const float2 f = *reinterpret_cast<const float2*>(p);
+            v[0] = f.x; v[1] = f.y;
+        }
+    }
+
+    __device__ void begin(const AttendArgs& a, const Cursor& c, int lane) {
+        const float* qb = static_cast<const float*>(a.q);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const bool in = r < c.t.nrows;
+            const int fr = c.t.r0 + (in ? r : 0);
+            const int tok = fr / a.group, h = c.g * a.group + fr % a.group;
+            load(q[r], qb + static_cast<size_t>(c.t.first + tok) * a.q_stride + static_cast<size_t>(h) * HD + lane * D);
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                if (!in) q[r][d] = 0.f;
+                o[r][d] = 0.f;
+            }
+            m[r] = -INFINITY;
+        }
+#pragma unroll
+        for (int g = 0; g < RG; g++) {
+            const int r = 4 * g + lane / 8;
+            attended(a, c.t.p0 + (c.t.r0 + r) / a.group, lo[g], hi[g]);
+            if (r >= c.t.nrows) hi[g] = 0;
+            l[g] = 0.f;
+        }
+    }
+
+    __device__ void step(const AttendArgs& a, const Cursor& c, StepInfo si, const uint8_t* sk, const uint8_t* sv,
+                         int lane) {
+        const float* K = reinterpret_cast<const float*>(sk) + lane * D;
+        const float* V = reinterpret_cast<const float*>(sv) + lane * D;
+        const float sl = a.scale * 1.4426950408889634f;
+        const int key = si.key0 + (lane & 7);
+        float p[RG];
+        float k[8][D];
+#pragma unroll
+        for (int f = 0; f < 8; f++) load(k[f], K + f * HD);
+#pragma unroll
+        for (int g = 0; g < RG; g++) {
+            float v[32];
+#pragma unroll
+            for (int h = 0; h < 4; h++)
+#pragma unroll
+                for (int f = 0; f < 8; f++) {
+                    float t = q[4 * g + h][0] * k[f][0];
+#pragma unroll
+                    for (int d = 1; d < D; d++) t = fmaf(q[4 * g + h][d], k[f][d], t);
+                    v[8 * h + f] = t;
+                }
+            warp_reduce_multi<32>(v);
+            const bool in = key >= lo[g] && key < hi[g] && (si.valid & 1);
+            const float s = in ? v[0] * sl : -INFINITY;
+            float mx = s;
+            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
+            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 4));
+            float mine = 0.f, fm = 1.f;  // base and factor of this lane's row
+#pragma unroll
+            for (int h = 0; h < 4; h++) {
+                const int r = 4 * g + h;
+                const float mn = fmaxf(m[r], __shfl_sync(FULL, mx, 8 * h));
+                const float base = mn == -INFINITY ? 0.f : mn;
+                const float f = ex2(m[r] - base);
+                m[r] = mn;
+#pragma unroll
+                for (int d = 0; d < D; d++) o[r][d] *= f;
+                if ((lane >> 3) == h) {
+                    mine = base;
+                    fm = f;
+                }
+            }
+            p[g] = ex2(s - mine);
+            l[g] = l[g] * fm + p[g];
+        }
+#pragma unroll
+        for (int f = 0; f < 8; f++) {
+            float v[D];
+            load(v, V + f * HD);
+            const int kf = si.key0 + f;
+            if (!(kf >= c.t.lo && kf < c.t.hi && (si.valid & 1))) {  // keys that no row attends to: no 0 x NaN
+#pragma unroll
+                for (int d = 0; d < D; d++) v[d] = 0.f;
+            }
+#pragma unroll
+            for (int g = 0; g < RG; g++)
+#pragma unroll
+                for (int h = 0; h < 4; h++) {
+                    const float w = __shfl_sync(FULL, p[g], 8 * h + f);
+#pragma unroll
+                    for (int d = 0; d < D; d++) o[4 * g + h][d] = fmaf(w, v[d], o[4 * g + h][d]);
+                }
+        }
+    }
+
+    __device__ bool finish(int nrows, int lane) {
+        float z = 0.f;
+#pragma unroll
+        for (int g = 0; g < RG; g++) {
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) l[g] += __shfl_xor_sync(FULL, l[g], x);
+            if (4 * g + lane / 8 < nrows) z = fmaf(l[g], 0.f, z);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (r < nrows) {
+#pragma unroll
+                for (int d = 0; d < D; d++) z = fmaf(o[r][d], 0.f, z);
+            }
+        return z != z;
+    }
+    __device__ void dump(float* j, int pass, int lane) const {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (r / 8 != pass) continue;
+            float* row = j + (r & 7) * (HD + 4);
+            const float lr = __shfl_sync(FULL, l[r / 4], 8 * (r & 3));
+            if (lane == 0) {
+                row[0] = m[r];
+                row[1] = lr;
+            }
+#pragma unroll
+            for (int d = 0; d < D; d++) row[4 + lane * D + d] = o[r][d];
+        }
+    }
+};
+
+// Exclusive running sum over the block's threads; `total` gets the sum.
+__device__ __forceinline__ long long scan_block(long long v, long long* ws, long long& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(FULL, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) ws[warp] = x;
+    __syncthreads();
+    long long before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; w++) {
+        if (w < warp) before += ws[w];
+        sum += ws[w];
+    }
+    total = sum;
+    return x - v + before;
+}
+
+template <int R, int KS>
+__device__ __forceinline__ long long units_of(const AttendArgs& a, int b) {
+    if (b >= a.n_seq) return 0;
+    int first, n;
+    rows_of(a, b, first, n);
+    long long u = 0;
+    for (int rt = 0; rt * R < n * a.group; rt++) u += steps_of<KS>(tile_of(a, b, rt, R));
+    return u * a.KV;
+}
+
+template <typename T, int HD, int R>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attend_split(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, AttendArgs a,
+                   Head* heads, float* parts) {
+    using S = Shape<T, HD>;
+    constexpr int KS = S::KS, NST = S::NST;
+    extern __shared__ uint8_t raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* ring = base + static_cast<size_t>(warp) * NST * 2 * S::SIDE;
+    float* join = reinterpret_cast<float*>(base + static_cast<size_t>(kWarps) * NST * 2 * S::SIDE);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(join + kWarps * S::JOIN) + warp * NST;
+    long long* ws = reinterpret_cast<long long*>(join + kWarps * S::JOIN) + kWarps * NST;  // [kWarps]
+    int* found = reinterpret_cast<int*>(ws + kWarps);                                       // [4]: b, -, unit in b
+
+    if (lane == 0) {
+        for (int i = 0; i < NST; i++) bar_init(&bars[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x == 0) heads[blockIdx.x].parts = 0;
+
+    // this block's share [u0, u0 + left) of the call's units
+    long long total = 0, at0 = 0;
+    const long long mine = units_of<R, KS>(a, threadIdx.x);
+    at0 = scan_block(mine, ws, total);
+    const long long chunk0 = total;
+    if (a.n_seq > kThreads) {  // the rest of the sequences: their sum first
+        long long rest = 0, sum;
+        for (int b = kThreads + threadIdx.x; b < a.n_seq; b += kThreads) rest += units_of<R, KS>(a, b);
+        scan_block(rest, ws, sum);
+        total += sum;
+    }
+    // at least one step a warp, so that a small call is not cut into crumbs
+    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kWarps));
+    const long long u0 = per * blockIdx.x;
+    if (u0 >= total) return;
+    if (threadIdx.x == 0) found[0] = -1;
+    __syncthreads();
+    auto place = [&](int b, long long at, long long n) {
+        if (u0 >= at && u0 < at + n) {
+            found[0] = b;
+            ws[0] = u0 - at;
+        }
+    };
+    if (u0 < chunk0) {
+        place(threadIdx.x, at0, mine);
+    } else {
+        long long before = chunk0;
+        for (int b0 = kThreads; b0 < a.n_seq; b0 += kThreads) {
+            const long long n = units_of<R, KS>(a, b0 + threadIdx.x);
+            long long sum;
+            const long long at = before + scan_block(n, ws, sum);
+            __syncthreads();
+            if (u0 < before + sum) {
+                place(b0 + threadIdx.x, at, n);
+                break;
+            }
+            before += sum;
+        }
+    }
+    __syncthreads();
+    if (found[0] < 0) return;  // (the lengths changed under the call)
+    Cursor c;
+    c.b = found[0];
+    c.rt = 0;
+    c.left = min(per, total - u0);
+    {
+        long long u = ws[0];
+        for (;; c.rt++) {
+            c.t = tile_of(a, c.b, c.rt, R);
+            c.steps = steps_of<KS>(c.t);
+            if (u < static_cast<long long>(c.steps) * a.KV) break;
+            u -= static_cast<long long>(c.steps) * a.KV;
+        }
+        c.g = static_cast<int>(u / c.steps);
+        c.s = static_cast<int>(u % c.steps);
+        c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
+    }
+
+    // producer: a second cursor that runs up to NST steps ahead; ids of this warp's next 32 steps in the lanes
+    Cursor pc = c;
+    int ps = pc.s + warp, pid_at = 0, pid0 = -1, pid1 = -1;
+    bool more = true, fresh = true;
+    int put = 0, got = 0;
+    uint32_t valid_bits = 0;  // 2 bits for each stage
+    int stage_key[NST];
+    auto produce = [&]() {
+        while (more && ps >= pc.end) {
+            more = next_tile<R, KS>(a, pc);
+            ps = pc.s + warp;
+            fresh = true;
+        }
+        if (!more) return;
+        if (fresh || pid_at == 32) {
+            const long long key = (static_cast<long long>(pc.t.lo / KS) + ps + static_cast<long long>(kWarps) * lane) * KS;
+            const int k32 = key < 0x7fffff00ll ? static_cast<int>(key) : -1;
+            pid0 = page_of(a, pc.b, k32);
+            pid1 = (KS == 16 && a.shift == 3) ? page_of(a, pc.b, k32 < 0 ? -1 : k32 + 8) : pid0;
+            pid_at = 0;
+            fresh = false;
+        }
+        const int id0 = __shfl_sync(FULL, pid0, pid_at), id1 = __shfl_sync(FULL, pid1, pid_at);
+        pid_at++;
+        const int st = put % NST;
+        const int key0 = (pc.t.lo / KS + ps) * KS;
+        const uint32_t v = (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u);
+        valid_bits = (valid_bits & ~(3u << (2 * st))) | (v << (2 * st));
+#pragma unroll
+        for (int i = 0; i < NST; i++)
+            if (i == st) stage_key[i] = key0;
+        if (lane == 0) {
+            uint8_t* k = ring + st * 2 * S::SIDE;
+            uint8_t* vv = k + S::SIDE;
+            const int row = (pc.g << a.shift) + (key0 & ((1 << a.shift) - 1));
+            bar_expect_tx(&bars[st], 2 * S::SIDE);
+            tma_page(k, &map_k, row, id0, &bars[st]);
+            tma_page(vv, &map_v, row, id0, &bars[st]);
+            if (KS == 16 && a.shift == 3) {
+                tma_page(k + S::SIDE / 2, &map_k, pc.g << 3, id1, &bars[st]);
+                tma_page(vv + S::SIDE / 2, &map_v, pc.g << 3, id1, &bars[st]);
+            }
+        }
+        put++;
+        ps += kWarps;
+    };
+    __syncwarp();
+    for (int i = 0; i < NST; i++) produce();
+
+    Core<T, HD, R> core;
+    bool first_tile = true, dead = false;
+    for (bool go = true; go; go = next_tile<R, KS>(a, c), first_tile = false) {
+        core.begin(a, c, lane);
+        for (int s = c.s + warp; s < c.end; s += kWarps) {
+            const int st = got % NST;
+            dead |= !bar_wait(&bars[st], (got / NST) & 1);
+            StepInfo si;
+            si.valid = (valid_bits >> (2 * st)) & 3u;
+            si.key0 = 0;
+#pragma unroll
+            for (int i = 0; i < NST; i++)
+                if (i == st) si.key0 = stage_key[i];
+            const uint8_t* k = ring + st * 2 * S::SIDE;
+            core.step(a, c, si, k, k + S::SIDE, lane);
+            got++;
+            __syncwarp();  // every lane has read the stage
+            produce();
+        }
+        // A result that is not finite: a value that one row must not see may have met it as 0 x infinity,
+        // or an infinite value the split weights.  Such a tile is done over row by row, which gives the
+        // formula's result to each.  (Every finite input stays far from this.)
+        const bool redo = core.finish(c.t.nrows, lane) && !dead;
+        const bool whole = c.s == 0 && c.end == c.steps;
+        float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * R * (HD + 4);
+        const int any_redo = __syncthreads_or(redo);
+        for (int pass = 0; pass * 8 < c.t.nrows; pass++) {
+            if (pass) __syncthreads();
+            core.dump(join + warp * S::JOIN, pass, lane);
+            if (dead && lane < 8) join[warp * S::JOIN + lane * (HD + 4) + 1] = NAN;  // a copy never came: no answer
+            __syncthreads();
+            const int row = 8 * pass + warp;  // one warp a row
+            if (row < c.t.nrows) {
+                const float* j = join + warp * (HD + 4);
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) M = fmaxf(M, j[w * S::JOIN]);
+                float L = 0.f, acc[HD / 32];
+#pragma unroll
+                for (int d = 0; d < HD / 32; d++) acc[d] = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) {
+                    const float mw = j[w * S::JOIN];
+                    const float f = M == -INFINITY ? 1.f : ex2(mw - M);  // (all empty: sums are 0 or NaN)
+                    L += j[w * S::JOIN + 1] * f;
+#pragma unroll
+                    for (int d = 0; d < HD / 32; d++) acc[d] += j[w * S::JOIN + 4 + lane + 32 * d] * f;
+                }
+                const int fr = c.t.r0 + row, tok = c.t.first + fr / a.group, h = c.g * a.group + fr % a.group;
+                if (whole) {
+                    if (any_redo) {
+                        attend_row<T, HD>(a, c.b, tok, h, lane);
+                    } else {
+                        T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + h) * HD;
+#pragma unroll
+                        for (int d = 0; d < HD / 32; d++) out[lane + 32 * d] = from_f32<T>(L != 0.f ? acc[d] / L : 0.f);
+                    }
+                } else {
+                    float* pr = part + row * (HD + 4);
+                    if (lane == 0) {
+                        pr[0] = M;
+                        pr[1] = L;
+                        pr[2] = any_redo ? 1.f : 0.f;
+                    }
+#pragma unroll
+                    for (int d = 0; d < HD / 32; d++) pr[4 + lane + 32 * d] = acc[d];
+                }
+            }
+        }
+        if (!whole && c.s == 0 && threadIdx.x == 0) {  // this block begins the tile: it says who has the rest
+            Head h;
+            h.parts = 1 + static_cast<int>((c.steps - c.end + per - 1) / per);
+            h.slot = first_tile ? 0 : 1;
+            h.b = c.b;
+            h.rt = c.rt;
+            h.g = c.g;
+            heads[blockIdx.x] = h;
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the parts of the tile that block blockIdx.x began: part i > 0 is the first tile of block blockIdx.x + i.
+template <typename T, int HD, int R>
+__global__ void __launch_bounds__(kThreads) k_attend_join(AttendArgs a, const Head* heads, const float* parts) {
+    pdl_wait();
+    const Head h = heads[blockIdx.x];
+    if (h.parts == 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Tile t = tile_of(a, h.b, h.rt, R);
+    constexpr size_t rec = static_cast<size_t>(R) * (HD + 4);
+    const float* p0 = parts + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
+    const float* p1 = parts + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;  // parts 1 .. are 2 * rec apart
+    for (int row = warp; row < t.nrows; row += kWarps) {
+        float M = -INFINITY, bad = 0.f;
+        for (int i = lane; i < h.parts; i += 32) {
+            const float* p = (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4);
+            M = fmaxf(M, p[0]);
+            bad = fmaxf(bad, p[2]);
+        }
+        M = warp_max(M);
+        bad = warp_max(bad);
+        const int fr = t.r0 + row, tok = t.first + fr / a.group, hh = h.g * a.group + fr % a.group;
+        if (bad > 0.f) {
+            attend_row<T, HD>(a, h.b, tok, hh, lane);
+            continue;
+        }
+        float L = 0.f, acc[HD / 32];
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) acc[d] = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < h.parts; i++) {
+            const float* p = (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4);
+            const float f = M == -INFINITY ? 1.f : ex2(p[0] - M);
+            L += p[1] * f;
+#pragma unroll
+            for (int d = 0; d < HD / 32; d++) acc[d] += p[4 + lane + 32 * d] * f;
+        }
+        T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++) out[lane + 32 * d] = from_f32<T>(L != 0.f ? acc[d] / L : 0.f);
+    }
+}
+
+constexpr size_t kHeadBytes = 16384;  // of up to 512 blocks
+
+template <typename T, int HD, int R>
+tl_status run_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
+    using S = Shape<T, HD>;
+    static_assert(S::SMEM <= 232448, "shared memory of a block");
+    CUtensorMap mk, mv;
+    const int rows = std::min(S::KS, 1 << a.shift);
+    TL_TRY(encode_pages(&mk, c->k, c, rows));
+    TL_TRY(encode_pages(&mv, c->v, c, rows));
+    TL_CUDA_TRY(cudaFuncSetAttribute(k_attend_split<T, HD, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(S::SMEM)));
+    const int grid = std::min(sm_count(), 512);
+    Head* heads = static_cast<Head*>(workspace);
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeadBytes);
+    k_attend_split<T, HD, R><<<grid, kThreads, S::SMEM, s>>>(mk, mv, a, heads, parts);
+    TL_TRY(check_launch("paged_attention"));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_attend_join<T, HD, R>, a, static_cast<const Head*>(heads),
+                                   static_cast<const float*>(parts)));
+    return TL_OK;
+}
+
+template <int HD>
+tl_status run_split_hd(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
+    if (c->dtype == TL_F16) return run_split<__half, HD, 16>(a, c, workspace, s);
+    if (c->dtype == TL_BF16) return run_split<__nv_bfloat16, HD, 16>(a, c, workspace, s);
+    // fp32: rows are paid for one by one, so no more of them than a decode step has
+    const long long rows = static_cast<long long>(a.n_tokens) * a.group;
+    if (a.group <= 4 && rows <= 4ll * a.n_seq) return run_split<float, HD, 4>(a, c, workspace, s);
+    if (a.group <= 8 && rows <= 8ll * a.n_seq) return run_split<float, HD, 8>(a, c, workspace, s);
+    return run_split<float, HD, 16>(a, c, workspace, s);
 }
 
 }  // namespace
+
+size_t split_workspace(int hd) {
+    return kHeadBytes + static_cast<size_t>(std::min(sm_count(), 512)) * 2 * 16 * (hd + 4) * 4;
+}
+
+tl_status attend_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
+    return c->head_dim == 128 ? run_split_hd<128>(a, c, workspace, s) : run_split_hd<64>(a, c, workspace, s);
+}
+
 }  // namespace paged
 }  // namespace tl
 
@@ -47,7 +827,7 @@ tl_status tl_paged_attention_workspace(const tl_paged_cache* cache, size_t n_tok
     TL_REQUIRE(n_heads > 0 && n_heads % cache->n_kv_heads == 0, "tl_paged_attention_workspace: %zu heads, %zu kv heads",
                n_heads, cache->n_kv_heads);
     (void)n_tokens; (void)n_seq; (void)max_blocks;
-    *bytes = 16;
+    *bytes = split_workspace(static_cast<int>(cache->head_dim));
     return TL_OK;
 }
 
@@ -69,7 +849,10 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     TL_REQUIRE(aligned16(out) && aligned16(q) && q_stride * dtype_size(cache->dtype) % 16 == 0,
                "tl_paged_attention: out, q and q_stride must be 16-byte aligned");
     TL_REQUIRE(scale == scale && fabsf(scale) <= 3.0e38f, "tl_paged_attention: scale %g", static_cast<double>(scale));
-    (void)workspace; (void)workspace_bytes;
+    size_t need = 0;
+    TL_TRY(tl_paged_attention_workspace(cache, n_tokens, n_heads, n_seq, max_blocks, &need));
+    TL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need,
+               "tl_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     AttendArgs a{};
     a.out = out;
     a.q = q;
@@ -90,12 +873,7 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.shift = __builtin_ctzll(cache->block_size);
     a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
     a.scale = scale;
-    const cudaStream_t s = as_stream(stream);
-    const int hd = static_cast<int>(cache->head_dim);
-    if (cache->dtype == TL_F32) launch_rows<float>(a, hd, s);
-    else if (cache->dtype == TL_F16) launch_rows<__half>(a, hd, s);
-    else launch_rows<__nv_bfloat16>(a, hd, s);
-    return check_launch("paged_attention");
+    return attend_split(a, cache, workspace, as_stream(stream));
 }
 
 }  // extern "C"

@@ -5,6 +5,7 @@
 #include <math.h>
 
 #include "tl_paged.cuh"
+#include "tl_tc.cuh"
 
 namespace tl {
 namespace paged {
@@ -23,35 +24,59 @@ struct AttendArgs {
     float scale;
 };
 
+// 2^x (hardware approximation, 2 ulp; 2^-inf = +0)
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // The query rows of sequence b, cut to the rows that exist.
 __device__ __forceinline__ void rows_of(const AttendArgs& a, int b, int& first, int& n) {
     first = min(max(a.q_start[b], 0), a.n_tokens);
     n = max(0, min(a.q_start[b + 1], a.n_tokens) - first);
 }
 
-// The sequence that row t belongs to, -1 if none.
-__device__ __forceinline__ int sequence_of(const AttendArgs& a, int t) {
-    int lo = 0, hi = a.n_seq;  // largest b with q_start[b] <= t
-    if (t < a.q_start[0]) return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_start[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    return t < a.q_start[lo + 1] ? lo : -1;
-}
-
-// Positions [lo, hi) that the query at position p of sequence b may attend to
+// Positions [lo, hi) that the query at position p of a sequence may attend to
 // (pages that do not exist are left out later, key by key).
 __device__ __forceinline__ void attended(const AttendArgs& a, long long p, int& lo, int& hi) {
     hi = static_cast<int>(min(p + 1, static_cast<long long>(a.max_blocks) << a.shift));
     lo = a.window > 0 ? static_cast<int>(max(0ll, p + 1 - a.window)) : 0;
 }
 
+// The page of position key of sequence b; -1 if there is none.
+__device__ __forceinline__ int page_of(const AttendArgs& a, int b, int key) {
+    const int j = key >> a.shift;
+    if (key < 0 || j >= a.max_blocks) return -1;
+    const int id = a.table[static_cast<size_t>(b) * a.max_blocks + j];
+    return id >= 0 && id < a.n_blocks ? id : -1;
+}
+
+// A tile of `rows` query rows of one kv head: row r of sequence b is its token
+// r / group, q head g * group + r % group, so that all heads that share a kv
+// head lie in one tile with their tokens, whatever the group.
+struct Tile {
+    int first, n;        // the sequence's token rows
+    int r0, nrows;       // rows of the tile
+    long long p0;        // position of the sequence's first token row
+    int lo, lo_last;     // first attended position of the tile's first and last token
+    int hi, hi_first;    // end of the attended positions of the last and first token
+};
+__device__ __forceinline__ Tile tile_of(const AttendArgs& a, int b, int rt, int rows) {
+    Tile t;
+    rows_of(a, b, t.first, t.n);
+    t.r0 = rt * rows;
+    t.nrows = min(rows, t.n * a.group - t.r0);
+    t.p0 = static_cast<long long>(a.seq_lens[b]) - t.n;
+    attended(a, t.p0 + t.r0 / a.group, t.lo, t.hi_first);
+    attended(a, t.p0 + (t.r0 + t.nrows - 1) / a.group, t.lo_last, t.hi);
+    return t;
+}
+
 // One (token, head) by one warp, straight from the pages in fp32: lane l holds
 // dims l * HD / 32 ...  Reads the attended keys only.
 template <typename T, int HD>
-__device__ void attend_row(const AttendArgs& a, int b, int t, int h, int lane) {
+__device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h, int lane) {
     constexpr int D = HD / 32;
     int first, n;
     rows_of(a, b, first, n);
@@ -68,8 +93,8 @@ __device__ void attend_row(const AttendArgs& a, int b, int t, int h, int lane) {
     }
     float m = -INFINITY, l = 0.f;
     for (int j = lo; j < hi; j++) {
-        const int id = a.table[static_cast<size_t>(b) * a.max_blocks + (j >> a.shift)];
-        if (id < 0 || id >= a.n_blocks) continue;
+        const int id = page_of(a, b, j);
+        if (id < 0) continue;
         const size_t at = static_cast<size_t>(id) * a.block_stride +
                           ((static_cast<size_t>(g) << a.shift) + (j & ((1 << a.shift) - 1))) * HD + lane * D;
         const T* kp = static_cast<const T*>(a.k) + at;
@@ -90,6 +115,15 @@ __device__ void attend_row(const AttendArgs& a, int b, int t, int h, int lane) {
 #pragma unroll
     for (int d = 0; d < D; d++) op[d] = from_f32<T>(l != 0.f ? acc[d] / l : 0.f);
 }
+
+// Map of one side (K or V) of the pages: {64 or hd columns, rows of all kv heads, column
+// panels, pages}; a box is `rows` rows of every panel of one page, zero where the page does not exist.
+// 16-bit types: panels of 64 columns, SWIZZLE_128B; fp32: one panel, no swizzle.
+tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache* c, int rows);
+
+// Work of few query rows per sequence (tl_paged_attn.cu) and of many (tl_paged_attn_tc.cu).
+size_t split_workspace(int hd);
+tl_status attend_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace tl
