@@ -34,7 +34,7 @@ namespace paged {
 
 using namespace tc;
 
-tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache* c, int rows) {
+tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache* c, int rows, int box_panels) {
     auto fn = encode_fn();
     if (!fn) return set_error(TL_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     const bool wide = c->dtype == TL_F32;
@@ -43,7 +43,7 @@ tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache*
     const cuuint32_t panels = static_cast<cuuint32_t>(c->head_dim) / cols;
     const cuuint64_t dims[4] = {cols, c->n_kv_heads * c->block_size, panels, c->n_blocks};
     const cuuint64_t strides[3] = {c->head_dim * es, cols * es, c->block_stride * es};
-    const cuuint32_t box[4] = {cols, static_cast<cuuint32_t>(rows), panels, 1};
+    const cuuint32_t box[4] = {cols, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(box_panels), 1};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r = fn(map,
                           wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -76,50 +76,14 @@ struct Shape {
     static constexpr size_t SMEM = 1024 + static_cast<size_t>(kWarps) * NST * 2 * SIDE + kWarps * JOIN * 4 + 512;
 };
 
-// What one block leaves behind of a tile that it begins and others end.
-struct Head {
-    int parts, slot, b, rt, g;
-};
-
-// Units (steps) of one tile; a tile without keys counts one, so that its zeros get written.
-template <int KS>
-__device__ __forceinline__ int steps_of(const Tile& t) {
-    if (t.hi <= t.lo) return 1;
-    return (t.hi - 1) / KS - t.lo / KS + 1;
-}
-
-// Place in the call's work: tile (b, rt, g) and the steps [s, end) of it that belong to this block.
-struct Cursor {
-    int b, rt, g;
-    int s, end, steps;
-    long long left;  // units of the block from this tile's step s on
-    Tile t;
-};
-
-template <int R, int KS>
-__device__ __forceinline__ void enter(const AttendArgs& a, Cursor& c) {
-    c.t = tile_of(a, c.b, c.rt, R);
-    c.steps = steps_of<KS>(c.t);
-    c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
-}
-// To the next tile that has rows; false when the block's share is done.
-template <int R, int KS>
-__device__ __forceinline__ bool next_tile(const AttendArgs& a, Cursor& c) {
-    c.left -= c.end - c.s;
-    if (c.left <= 0) return false;
-    c.s = 0;
-    if (++c.g == a.KV) {
-        c.g = 0;
-        c.rt++;
-        while (c.rt * R >= c.t.n * a.group) {  // sequences without rows have no units
-            if (++c.b >= a.n_seq) return false;
-            c.rt = 0;
-            rows_of(a, c.b, c.t.first, c.t.n);
-        }
+// Steps of KS keys, tiles of R rows.  A tile without keys counts one step, so that its zeros get written.
+template <int R_, int KS>
+struct SplitPlan {
+    static constexpr int R = R_;
+    static __device__ __forceinline__ int steps(const Tile& t) {
+        return t.hi <= t.lo ? 1 : (t.hi - 1) / KS - t.lo / KS + 1;
     }
-    enter<R, KS>(a, c);
-    return true;
-}
+};
 
 // ---- arithmetic of one warp -------------------------------------------------
 
@@ -475,38 +439,6 @@ struct Core<float, HD, R> {
     }
 };
 
-// Exclusive running sum over the block's threads; `total` gets the sum.
-__device__ __forceinline__ long long scan_block(long long v, long long* ws, long long& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(FULL, x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) ws[warp] = x;
-    __syncthreads();
-    long long before = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-        if (w < warp) before += ws[w];
-        sum += ws[w];
-    }
-    total = sum;
-    return x - v + before;
-}
-
-template <int R, int KS>
-__device__ __forceinline__ long long units_of(const AttendArgs& a, int b) {
-    if (b >= a.n_seq) return 0;
-    int first, n;
-    rows_of(a, b, first, n);
-    long long u = 0;
-    for (int rt = 0; rt * R < n * a.group; rt++) u += steps_of<KS>(tile_of(a, b, rt, R));
-    return u * a.KV;
-}
-
 template <typename T, int HD, int R>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attend_split(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, AttendArgs a,
@@ -520,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* join = reinterpret_cast<float*>(base + static_cast<size_t>(kWarps) * NST * 2 * S::SIDE);
     uint64_t* bars = reinterpret_cast<uint64_t*>(join + kWarps * S::JOIN) + warp * NST;
     long long* ws = reinterpret_cast<long long*>(join + kWarps * S::JOIN) + kWarps * NST;  // [kWarps]
-    int* found = reinterpret_cast<int*>(ws + kWarps);                                       // [4]: b, -, unit in b
+    int* found = reinterpret_cast<int*>(ws + kWarps);
 
     if (lane == 0) {
         for (int i = 0; i < NST; i++) bar_init(&bars[i], 1);
@@ -528,63 +460,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (threadIdx.x == 0) heads[blockIdx.x].parts = 0;
 
-    // this block's share [u0, u0 + left) of the call's units
-    long long total = 0, at0 = 0;
-    const long long mine = units_of<R, KS>(a, threadIdx.x);
-    at0 = scan_block(mine, ws, total);
-    const long long chunk0 = total;
-    if (a.n_seq > kThreads) {  // the rest of the sequences: their sum first
-        long long rest = 0, sum;
-        for (int b = kThreads + threadIdx.x; b < a.n_seq; b += kThreads) rest += units_of<R, KS>(a, b);
-        scan_block(rest, ws, sum);
-        total += sum;
-    }
-    // at least one step a warp, so that a small call is not cut into crumbs
-    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(kWarps));
-    const long long u0 = per * blockIdx.x;
-    if (u0 >= total) return;
-    if (threadIdx.x == 0) found[0] = -1;
-    __syncthreads();
-    auto place = [&](int b, long long at, long long n) {
-        if (u0 >= at && u0 < at + n) {
-            found[0] = b;
-            ws[0] = u0 - at;
-        }
-    };
-    if (u0 < chunk0) {
-        place(threadIdx.x, at0, mine);
-    } else {
-        long long before = chunk0;
-        for (int b0 = kThreads; b0 < a.n_seq; b0 += kThreads) {
-            const long long n = units_of<R, KS>(a, b0 + threadIdx.x);
-            long long sum;
-            const long long at = before + scan_block(n, ws, sum);
-            __syncthreads();
-            if (u0 < before + sum) {
-                place(b0 + threadIdx.x, at, n);
-                break;
-            }
-            before += sum;
-        }
-    }
-    __syncthreads();
-    if (found[0] < 0) return;  // (the lengths changed under the call)
+    using P = SplitPlan<R, KS>;
     Cursor c;
-    c.b = found[0];
-    c.rt = 0;
-    c.left = min(per, total - u0);
-    {
-        long long u = ws[0];
-        for (;; c.rt++) {
-            c.t = tile_of(a, c.b, c.rt, R);
-            c.steps = steps_of<KS>(c.t);
-            if (u < static_cast<long long>(c.steps) * a.KV) break;
-            u -= static_cast<long long>(c.steps) * a.KV;
-        }
-        c.g = static_cast<int>(u / c.steps);
-        c.s = static_cast<int>(u % c.steps);
-        c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
-    }
+    // at least one step a warp, so that a small call is not cut into crumbs
+    const long long per = find_share<P, kWarps>(a, c, ws, found, kWarps);
+    if (per == 0) return;
 
     // producer: a second cursor that runs up to NST steps ahead; ids of this warp's next 32 steps in the lanes
     Cursor pc = c;
@@ -595,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage_key[NST];
     auto produce = [&]() {
         while (more && ps >= pc.end) {
-            more = next_tile<R, KS>(a, pc);
+            more = next_tile<P>(a, pc);
             ps = pc.s + warp;
             fresh = true;
         }
@@ -637,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     Core<T, HD, R> core;
     bool first_tile = true, dead = false;
-    for (bool go = true; go; go = next_tile<R, KS>(a, c), first_tile = false) {
+    for (bool go = true; go; go = next_tile<P>(a, c), first_tile = false) {
         core.begin(a, c, lane);
         for (int s = c.s + warp; s < c.end; s += kWarps) {
             const int st = got % NST;
@@ -706,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!whole && c.s == 0 && threadIdx.x == 0) {  // this block begins the tile: it says who has the rest
             Head h;
-            h.parts = 1 + static_cast<int>((c.steps - c.end + per - 1) / per);
+            h.parts = parts_of(c.steps, c.end, per);
             h.slot = first_tile ? 0 : 1;
             h.b = c.b;
             h.rt = c.rt;
@@ -759,19 +639,18 @@ __global__ void __launch_bounds__(kThreads) k_attend_join(AttendArgs a, const He
     }
 }
 
-constexpr size_t kHeadBytes = 16384;  // of up to 512 blocks
-
 template <typename T, int HD, int R>
 tl_status run_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
     using S = Shape<T, HD>;
     static_assert(S::SMEM <= 232448, "shared memory of a block");
     CUtensorMap mk, mv;
     const int rows = std::min(S::KS, 1 << a.shift);
-    TL_TRY(encode_pages(&mk, c->k, c, rows));
-    TL_TRY(encode_pages(&mv, c->v, c, rows));
+    const int panels = std::is_same<T, float>::value ? 1 : HD / 64;
+    TL_TRY(encode_pages(&mk, c->k, c, rows, panels));
+    TL_TRY(encode_pages(&mv, c->v, c, rows, panels));
     TL_CUDA_TRY(cudaFuncSetAttribute(k_attend_split<T, HD, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      static_cast<int>(S::SMEM)));
-    const int grid = std::min(sm_count(), 512);
+    const int grid = std::min(sm_count(), kMaxBlocks);
     Head* heads = static_cast<Head*>(workspace);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeadBytes);
     k_attend_split<T, HD, R><<<grid, kThreads, S::SMEM, s>>>(mk, mv, a, heads, parts);
@@ -804,7 +683,7 @@ tl_status run_split_hd(const AttendArgs& a, const tl_paged_cache* c, void* works
 }  // namespace
 
 size_t split_workspace(int hd) {
-    return kHeadBytes + static_cast<size_t>(std::min(sm_count(), 512)) * 2 * 16 * (hd + 4) * 4;
+    return kHeadBytes + static_cast<size_t>(std::min(sm_count(), kMaxBlocks)) * 2 * 16 * (hd + 4) * 4;
 }
 
 tl_status attend_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
@@ -817,6 +696,13 @@ tl_status attend_split(const AttendArgs& a, const tl_paged_cache* c, void* works
 using namespace tl;
 using namespace tl::paged;
 
+namespace {
+// Rows per sequence and kv head, on average, from which the 256-row tiles pay.
+bool many_rows(const tl_paged_cache* c, size_t n_tokens, size_t n_heads, size_t n_seq) {
+    return c->dtype != TL_F32 && n_tokens * (n_heads / c->n_kv_heads) > 16 * n_seq;
+}
+}  // namespace
+
 extern "C" {
 
 tl_status tl_paged_attention_workspace(const tl_paged_cache* cache, size_t n_tokens, size_t n_heads, size_t n_seq,
@@ -826,8 +712,9 @@ tl_status tl_paged_attention_workspace(const tl_paged_cache* cache, size_t n_tok
     TL_REQUIRE(bytes, "tl_paged_attention_workspace: no result");
     TL_REQUIRE(n_heads > 0 && n_heads % cache->n_kv_heads == 0, "tl_paged_attention_workspace: %zu heads, %zu kv heads",
                n_heads, cache->n_kv_heads);
-    (void)n_tokens; (void)n_seq; (void)max_blocks;
-    *bytes = split_workspace(static_cast<int>(cache->head_dim));
+    (void)max_blocks;
+    const int hd = static_cast<int>(cache->head_dim);
+    *bytes = many_rows(cache, n_tokens, n_heads, n_seq) ? chunk_workspace(hd) : split_workspace(hd);
     return TL_OK;
 }
 
@@ -843,7 +730,7 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     TL_REQUIRE(out && q && block_table && q_start && seq_lens, "tl_paged_attention: null pointer");
     TL_REQUIRE(max_blocks > 0 && n_seq <= 0x7fffffffull && max_blocks <= 0x7fffffffull / n_seq,
                "tl_paged_attention: %zu sequences x %zu blocks", n_seq, max_blocks);
-    TL_REQUIRE(n_tokens <= 0x7fffffffull / n_heads, "tl_paged_attention: %zu tokens x %zu heads", n_tokens, n_heads);
+    TL_REQUIRE(n_tokens <= 0x3fffffffull / n_heads, "tl_paged_attention: %zu tokens x %zu heads", n_tokens, n_heads);
     TL_REQUIRE(q_stride >= n_heads * cache->head_dim && q_stride <= (1ull << 36), "tl_paged_attention: q_stride %zu",
                q_stride);
     TL_REQUIRE(aligned16(out) && aligned16(q) && q_stride * dtype_size(cache->dtype) % 16 == 0,
@@ -872,8 +759,9 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.n_blocks = static_cast<int>(cache->n_blocks);
     a.shift = __builtin_ctzll(cache->block_size);
     a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
-    a.scale = scale;
-    return attend_split(a, cache, workspace, as_stream(stream));
+    a.scale = scale == 0.f ? 1e-30f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
+    return many_rows(cache, n_tokens, n_heads, n_seq) ? attend_chunk(a, cache, workspace, as_stream(stream))
+                                                      : attend_split(a, cache, workspace, as_stream(stream));
 }
 
 }  // extern "C"

@@ -73,6 +73,149 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs& a, int b, int rt, int 
     return t;
 }
 
+// ---- division of a call's work among the blocks -----------------------------
+// The steps of all tiles lie in one line: sequence by sequence, row tile by row
+// tile, kv head by kv head.  Block i takes the steps [i * per, (i + 1) * per).
+// `Plan` says how many rows a tile has (R) and how many steps.
+
+// What a block leaves behind of a tile that it begins and others end.
+struct Head {
+    int parts, slot, b, rt, g;
+};
+constexpr int kMaxBlocks = 512;
+constexpr size_t kHeadBytes = 16384;  // heads of up to kMaxBlocks blocks
+static_assert(sizeof(Head) * kMaxBlocks <= kHeadBytes, "heads");
+
+// Place in the line: tile (b, rt, g) and the steps [s, end) of it that belong to this block.
+struct Cursor {
+    int b, rt, g;
+    int s, end, steps;
+    long long left;  // steps of the block from this tile's step s on
+    Tile t;
+};
+
+template <class Plan>
+__device__ __forceinline__ void enter(const AttendArgs& a, Cursor& c) {
+    c.t = tile_of(a, c.b, c.rt, Plan::R);
+    c.steps = Plan::steps(c.t);
+    c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
+}
+// To the next tile that has rows; false when the block's share is done.
+template <class Plan>
+__device__ __forceinline__ bool next_tile(const AttendArgs& a, Cursor& c) {
+    c.left -= c.end - c.s;
+    if (c.left <= 0) return false;
+    c.s = 0;
+    if (++c.g == a.KV) {
+        c.g = 0;
+        c.rt++;
+        while (c.rt * Plan::R >= c.t.n * a.group) {  // sequences without rows have no steps
+            if (++c.b >= a.n_seq) return false;
+            c.rt = 0;
+            rows_of(a, c.b, c.t.first, c.t.n);
+        }
+    }
+    enter<Plan>(a, c);
+    return true;
+}
+
+// Exclusive running sum over the block's NW warps; `total` gets the sum.
+template <int NW>
+__device__ __forceinline__ long long scan_block(long long v, long long* ws, long long& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(FULL, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) ws[warp] = x;
+    __syncthreads();
+    long long before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        if (w < warp) before += ws[w];
+        sum += ws[w];
+    }
+    total = sum;
+    return x - v + before;
+}
+
+template <class Plan>
+__device__ __forceinline__ long long steps_of_sequence(const AttendArgs& a, int b) {
+    if (b >= a.n_seq) return 0;
+    int first, n;
+    rows_of(a, b, first, n);
+    long long u = 0;
+    for (int rt = 0; rt * Plan::R < n * a.group; rt++) u += Plan::steps(tile_of(a, b, rt, Plan::R));
+    return u * a.KV;
+}
+
+// This block's share: `c` at its first tile; returns the steps of a full share, 0 if there is nothing
+// for this block.  All NW warps call it.  ws: [NW], found: [1], in shared memory.
+template <class Plan, int NW>
+__device__ long long find_share(const AttendArgs& a, Cursor& c, long long* ws, int* found, int least) {
+    constexpr int NT = NW * 32;
+    long long total = 0;
+    const long long mine = steps_of_sequence<Plan>(a, threadIdx.x);
+    const long long at0 = scan_block<NW>(mine, ws, total);
+    const long long chunk0 = total;
+    if (a.n_seq > NT) {  // the rest of the sequences: their sum first
+        long long rest = 0, sum;
+        for (int b = NT + threadIdx.x; b < a.n_seq; b += NT) rest += steps_of_sequence<Plan>(a, b);
+        scan_block<NW>(rest, ws, sum);
+        total += sum;
+    }
+    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(least));
+    const long long u0 = per * blockIdx.x;
+    if (u0 >= total) return 0;
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    auto place = [&](int b, long long at, long long n) {
+        if (u0 >= at && u0 < at + n) {
+            *found = b;
+            ws[0] = u0 - at;
+        }
+    };
+    if (u0 < chunk0) {
+        place(threadIdx.x, at0, mine);
+    } else {
+        long long before = chunk0;
+        for (int b0 = NT; b0 < a.n_seq; b0 += NT) {
+            const long long n = steps_of_sequence<Plan>(a, b0 + threadIdx.x);
+            long long sum;
+            const long long at = before + scan_block<NW>(n, ws, sum);
+            __syncthreads();
+            if (u0 < before + sum) {
+                place(b0 + threadIdx.x, at, n);
+                break;
+            }
+            before += sum;
+        }
+    }
+    __syncthreads();
+    if (*found < 0) return 0;  // (the lengths changed under the call)
+    c.b = *found;
+    c.rt = 0;
+    c.left = min(per, total - u0);
+    long long u = ws[0];
+    for (;; c.rt++) {
+        c.t = tile_of(a, c.b, c.rt, Plan::R);
+        c.steps = Plan::steps(c.t);
+        if (u < static_cast<long long>(c.steps) * a.KV) break;
+        u -= static_cast<long long>(c.steps) * a.KV;
+    }
+    c.g = static_cast<int>(u / c.steps);
+    c.s = static_cast<int>(u % c.steps);
+    c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
+    return per;
+}
+// The number of blocks that share a tile whose first block ends at step `end` of `steps`.
+__device__ __forceinline__ int parts_of(int steps, int end, long long per) {
+    return 1 + static_cast<int>((steps - end + per - 1) / per);
+}
+
 // One (token, head) by one warp, straight from the pages in fp32: lane l holds
 // dims l * HD / 32 ...  Reads the attended keys only.
 template <typename T, int HD>
@@ -117,13 +260,15 @@ __device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h
 }
 
 // Map of one side (K or V) of the pages: {64 or hd columns, rows of all kv heads, column
-// panels, pages}; a box is `rows` rows of every panel of one page, zero where the page does not exist.
-// 16-bit types: panels of 64 columns, SWIZZLE_128B; fp32: one panel, no swizzle.
-tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache* c, int rows);
+// panels, pages}; a box is `rows` rows of `panels` panels of one page, zero where the page does not
+// exist.  16-bit types: panels of 64 columns, SWIZZLE_128B; fp32: one panel, no swizzle.
+tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache* c, int rows, int panels);
 
-// Work of few query rows per sequence (tl_paged_attn.cu) and of many (tl_paged_attn_tc.cu).
+// Few query rows per sequence (tl_paged_attn.cu), and many (tl_paged_attn_tc.cu; not fp32).
 size_t split_workspace(int hd);
 tl_status attend_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s);
+size_t chunk_workspace(int hd);
+tl_status attend_chunk(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace tl

@@ -1,0 +1,647 @@
+// tl_paged_attn_tc.cu -- paged attention of many query rows (chunks of a
+// prompt) on the 5th-generation tensor cores; fp16 and bf16 caches.
+//
+// With 128 rows a K / V tile of 128 keys costs 512 cycles of the matrix unit a
+// product pair and 64 KB of reading; at full rate 128-row tiles would ask L2
+// for 128 bytes a cycle and SM, more than it gives.  So a block works on 256
+// rows of one kv head at a time, as two streams of 128 rows that share every
+// K / V tile:
+//   S_i[128 x 128] = Q_i K^T      tcgen05.mma, tensor memory
+//   P_i            = 2^(S_i scale - m_i)   one thread a row, 16-bit, over S_i
+//   O_i[128 x hd] += P_i V        tcgen05.mma, P_i from tensor memory
+// While the threads of one stream take exponentials, the matrix unit works for
+// the other.  A tile of at most 128 rows (the tail of a chunk, a single token
+// beside chunks) has its rows in both streams, which then take the key tiles in
+// turn and are added at the end.
+//   - V comes as [keys][hd] from its pages and is the N-major operand as it
+//     lies: nothing is transposed.
+//   - The row maximum moves only when it grows by more than 2^8 (then O is
+//     rescaled in tensor memory); exponents up to 2^8 stay in 16 bits' range and
+//     the final O / l is exact all the same.
+//   - Persistent blocks with equal shares of the key tiles (tl_paged_attn.cuh);
+//     a row tile that two blocks share is joined by a second kernel.
+// Warps: 0-3 stream 0, 4-7 stream 1 (softmax, epilogue), 8 TMA, 9 MMA.
+// Every mbarrier wait is bounded (~2 s): on expiry the roles stop, copies and
+// MMAs in flight drain, tensor memory is freed.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "tl_paged_attn.cuh"
+
+namespace tl {
+namespace paged {
+namespace {
+
+using namespace tc;
+
+constexpr int kRows = 256, kHalf = 128, kKB = 128;
+constexpr int kWarps = 10, kThreads = kWarps * 32;
+constexpr float kRescale = 8.f;  // log2 units
+
+// One step: 256 rows x 128 keys, or (tiles of at most 128 rows) 128 rows x 256 keys.
+struct ChunkPlan {
+    static constexpr int R = kRows;
+    static __device__ __forceinline__ int key_tiles(const Tile& t) {
+        return t.hi <= t.lo ? 1 : (t.hi - 1) / kKB - t.lo / kKB + 1;
+    }
+    static __device__ __forceinline__ int steps(const Tile& t) {
+        const int n = key_tiles(t);
+        return t.nrows > kHalf ? n : (n + 1) / 2;
+    }
+};
+
+template <int HD>
+struct Shape {
+    static constexpr int PANELS = HD / 64;
+    static constexpr int PANEL = kKB * 128;       // bytes of 64 columns of 128 rows
+    static constexpr int STAGE = PANELS * PANEL;  // K or V of 128 keys
+    static constexpr int NST = HD == 128 ? 5 : 10;
+    static constexpr size_t SMEM = 2 * static_cast<size_t>(STAGE) + static_cast<size_t>(NST) * STAGE + 256 +
+                                   2 * 2 * kHalf * 4 + 128;
+};
+
+// K-major operand: rows of 64 columns (128 bytes), SWIZZLE_128B: sdesc_k128.
+// N-major operand of 16-bit values, SWIZZLE_128B: rows are k, 64 columns each;
+// 8-row atoms 1024 bytes apart (stride offset), column panels `panel` bytes
+// apart (leading offset).
+__device__ __forceinline__ uint64_t sdesc_n128(uint32_t addr, uint32_t panel) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
+    d |= static_cast<uint64_t>(panel >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+// Instruction descriptor, kind::f16: D fp32, A and B of one 16-bit type, M 128; B K-major or N-major.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_n_major) {
+    const uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
+    return (1u << 4) | (f << 7) | (f << 10) | ((b_n_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void tma_panel(void* dst, const CUtensorMap* map, int row, int panel, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(su32(dst)), "l"(map), "r"(0), "r"(row), "r"(panel), "r"(page), "r"(su32(bar))
+        : "memory");
+}
+__device__ __forceinline__ uint32_t sw128(int r, int c) {
+    return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
+}
+// 32 columns, without waiting for them.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half*) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16*) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The key tiles [jb, je) of a cursor's part of a row tile, and which of them each stream takes.
+struct Part {
+    int jb, je, kb0;  // key tile j covers positions (kb0 + j) * 128 ..
+    bool two;         // two streams of rows (else the streams take key tiles in turn)
+    int end0;         // two: stream 0's last key tile + 1 (its tokens end earlier)
+    __device__ __forceinline__ bool active(int i) const {
+        if (two) return i == 1 || end0 > jb;
+        return i == 0 || je > jb + 1;
+    }
+    __device__ __forceinline__ int begin(int i) const { return two ? jb : jb + i; }
+    __device__ __forceinline__ int end(int i) const { return two && i == 0 ? end0 : je; }
+    __device__ __forceinline__ int stride() const { return two ? 1 : 2; }
+};
+__device__ __forceinline__ Part part_of(const AttendArgs& a, const Cursor& c) {
+    Part p;
+    const int n = ChunkPlan::key_tiles(c.t);
+    p.two = c.t.nrows > kHalf;
+    p.jb = p.two ? c.s : 2 * c.s;
+    p.je = min(n, p.two ? c.end : 2 * c.end);
+    p.kb0 = c.t.lo / kKB;
+    p.end0 = p.je;
+    if (p.two) {
+        int lo, hi;
+        attended(a, c.t.p0 + (c.t.r0 + kHalf - 1) / a.group, lo, hi);
+        p.end0 = hi <= 0 ? 0 : max(0, min(p.je, (hi - 1) / kKB - p.kb0 + 1));
+    }
+    return p;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attend_chunk(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, AttendArgs a,
+                   Head* heads, float* parts) {
+    using S = Shape<HD>;
+    constexpr int NST = S::NST;
+    extern __shared__ __align__(1024) uint8_t smem_chunk[];
+    uint8_t* sQ = smem_chunk;  // [2 streams]
+    uint8_t* ring = sQ + 2 * S::STAGE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + NST * S::STAGE);
+    uint64_t* empty = full + NST;
+    uint64_t* s_full = empty + NST;  // [2] S_i written (and every MMA before it done)
+    uint64_t* p_full = s_full + 2;   // [2] P_i written: 4 warps
+    uint64_t* q_full = p_full + 2;   // [2] Q_i written: 4 warps
+    uint64_t* o_full = q_full + 2;   // [2] the stream's last product done
+    uint64_t* xbar = o_full + 2;     // both streams' 8 warps
+    uint64_t* drain = xbar + 1;
+    static_assert((2 * 10 + 10) * 8 <= 256, "barriers");
+    float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);  // [2][128] max, [2][128] sum
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xch + 4 * kHalf);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* found = reinterpret_cast<int*>(tmem_slot + 2);
+    long long* ws = reinterpret_cast<long long*>(ring);  // the scan runs before the ring is used
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) heads[blockIdx.x].parts = 0;
+    Cursor c;
+    const long long per = find_share<ChunkPlan, kWarps>(a, c, ws, found, 2);
+    if (per == 0) return;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NST; i++) {
+            bar_init(&full[i], 1);
+            bar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            bar_init(&s_full[i], 1);
+            bar_init(&p_full[i], 4);
+            bar_init(&q_full[i], 4);
+            bar_init(&o_full[i], 1);
+        }
+        bar_init(xbar, 8);
+        bar_init(drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_proxy_async();  // the scan's writes to the ring precede the copies into it
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tS = tmem, tO = tmem + 256;  // S_i at + 128 i, O_i at + 128 i
+
+    auto fail = [&] { *abort_flag = 1; };
+    auto wait = [&](uint64_t* b, uint32_t parity) { return bar_wait_ab(b, parity, abort_flag); };
+
+    if (warp == 8) {
+        // ---- TMA: K_j, V_j of each key tile; lane = one page's rows of one panel ----
+        const int rows = min(kKB, 1 << a.shift);  // rows of a copy
+        const int pages = kKB / rows;
+        const int pg = lane / S::PANELS, panel = lane % S::PANELS;
+        uint32_t n = 0;  // loads issued
+        bool ok = true;
+        for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
+            const Part p = part_of(a, c);
+            const int off = pg * rows;
+            auto id_of = [&](int j) { return pg < pages && j < p.je ? page_of(a, c.b, (p.kb0 + j) * kKB + off) : -1; };
+            int id = id_of(p.jb);
+            for (int j = p.jb; ok && j < p.je; j++) {
+                const int id_next = id_of(j + 1);
+                const int key0 = (p.kb0 + j) * kKB + off;
+                const int row = (c.g << a.shift) + (key0 & ((1 << a.shift) - 1));
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    const uint32_t st = n % NST;
+                    if (!__all_sync(FULL, n < NST || wait(&empty[st], (n / NST - 1) & 1))) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) bar_expect_tx(&full[st], S::STAGE);
+                    __syncwarp();
+                    if (pg < pages)
+                        tma_panel(ring + st * S::STAGE + panel * S::PANEL + off * 128, kv ? &map_v : &map_k, row, panel, id,
+                                  &full[st]);
+                    n++;
+                }
+                id = id_next;
+            }
+        }
+        if (!ok) fail();
+        // every copy issued lands before the block ends
+        for (uint32_t k = n > NST ? n - NST : 0; k < n; k++) bar_wait(&full[k % NST], (k / NST) & 1);
+    } else if (warp == 9) {
+        if (lane == 0) {
+            // ---- MMA ----
+            constexpr uint32_t id_s = idesc<T>(kKB, false), id_o = idesc<T>(HD, true);
+            uint32_t n0 = 0;              // loads before this tile
+            uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+            bool ok = true;
+            for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
+                const Part p = part_of(a, c);
+                auto scores = [&](int i, int j) -> bool {  // S_i = Q_i K_j^T
+                    const uint32_t n = n0 + 2 * (j - p.jb), st = n % NST;
+                    if (!wait(&full[st], (n / NST) & 1)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int d = 0; d < S::PANELS; d++) {
+                        const uint64_t da = sdesc_k128(su32(sQ + i * S::STAGE + d * S::PANEL));
+                        const uint64_t db = sdesc_k128(su32(ring + st * S::STAGE + d * S::PANEL));
+#pragma unroll
+                        for (int k = 0; k < 4; k++) umma_f16(tS + 128 * i, da + 2 * k, db + 2 * k, id_s, (d | k) != 0);
+                    }
+                    umma_commit(&s_full[i]);
+                    if (!p.two || i == 1) umma_commit(&empty[st]);  // K_j is read (stream 1 is its last reader)
+                    return true;
+                };
+                auto values = [&](int i, int j) -> bool {  // O_i (+)= P_i V_j
+                    if (!wait(&p_full[i], np[i] & 1)) return false;
+                    np[i]++;
+                    const uint32_t n = n0 + 2 * (j - p.jb) + 1, st = n % NST;
+                    if (!wait(&full[st], (n / NST) & 1)) return false;
+                    tc_fence_after();
+                    const uint64_t db = sdesc_n128(su32(ring + st * S::STAGE), S::PANEL);
+#pragma unroll
+                    for (int k = 0; k < kKB / 16; k++)
+                        umma_f16_ts(tO + 128 * i, tS + 128 * i + 8 * k, db + 128 * k, id_o, j != p.begin(i) || k != 0);
+                    if (!p.two || i == 1) umma_commit(&empty[st]);
+                    return true;
+                };
+                const int stride = p.stride();
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    if (ok && p.active(i)) {
+                        ok = wait(&q_full[i], nq[i] & 1);
+                        nq[i]++;
+                        tc_fence_after();
+                        ok = ok && scores(i, p.begin(i));
+                    }
+                for (int j = p.jb; ok && j < p.je; j += stride)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int ji = p.two ? j : j + i;
+                        if (!ok || ji >= p.end(i)) continue;
+                        ok = values(i, ji);
+                        if (ok && ji + stride < p.end(i)) ok = scores(i, ji + stride);
+                        else if (ok) umma_commit(&o_full[i]);
+                    }
+                n0 += 2 * (p.je - p.jb);
+            }
+            if (!ok) fail();
+            umma_commit(drain);  // completes once every MMA issued above has
+            bar_wait(drain, 0);
+        }
+    } else {
+        // ---- softmax and epilogue: thread = row r of stream i ----
+        const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tS + 128 * i + lane_off, to = tO + 128 * i + lane_off;
+        const float scale = a.scale * 1.4426950408889634f;  // log2 units
+        const float sl = fabsf(scale);
+        uint32_t n0 = 0, ns = 0, no = 0, nx = 0;
+        bool ok = true, first_tile = true;
+        for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c), first_tile = false) {
+            const Part p = part_of(a, c);
+            const int row = p.two ? i * kHalf + r : r;  // of the tile
+            const bool in = row < c.t.nrows;
+            const int fr = c.t.r0 + (in ? row : 0);
+            const int tok = c.t.first + fr / a.group, h = c.g * a.group + fr % a.group;
+            const bool act = p.active(i);
+            int lo, hi;
+            attended(a, c.t.p0 + fr / a.group, lo, hi);
+            float m = -INFINITY, l = 0.f;
+            if (act) {
+                {  // the Q row into the swizzled K-major panels
+                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                                                      static_cast<size_t>(tok) * a.q_stride +
+                                                                      static_cast<size_t>(h) * HD);
+#pragma unroll
+                    for (int d = 0; d < HD / 8; d++) {
+                        const uint4 v = in ? src[d] : make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(sQ + i * S::STAGE + (d / 8) * S::PANEL + sw128(r, d & 7)) = v;
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&q_full[i]);
+                }
+                const int stride = p.stride();
+                for (int j = p.begin(i); j < p.end(i); j += stride) {
+                    const int key0 = (p.kb0 + j) * kKB;
+                    const int pid = lane < kKB / 8 ? page_of(a, c.b, key0 + 8 * lane) : 0;
+                    // every lane waits; the outcome is warp-uniform (tensor-memory access is warp-wide)
+                    if (!__all_sync(FULL, wait(&s_full[i], ns & 1))) {
+                        ok = false;
+                        break;
+                    }
+                    ns++;
+                    tc_fence_after();
+                    uint32_t u[128];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) tmem_ld32_async(ts + 32 * q, u + 32 * q);
+                    const uint32_t pages = __ballot_sync(FULL, pid >= 0);  // bit k: keys 8 k .. 8 k + 7 exist
+                    const bool inner = !in || (key0 >= lo && key0 <= hi - kKB);
+                    tmem_wait_ld();
+                    if (scale < 0.f) {
+#pragma unroll
+                        for (int e = 0; e < 128; e++) u[e] ^= 0x80000000u;
+                    }
+                    if (!__all_sync(FULL, inner) || pages != FULL) {
+#pragma unroll
+                        for (int e = 0; e < 128; e++) {
+                            const int key = key0 + e;
+                            if (!(key >= lo && key < hi && ((pages >> (e / 8)) & 1))) u[e] = 0xff800000u;
+                        }
+                    }
+                    float mx[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) mx[e] = __uint_as_float(u[e]);
+#pragma unroll
+                    for (int e = 8; e < 128; e++) mx[e & 7] = fmaxf(mx[e & 7], __uint_as_float(u[e]));
+#pragma unroll
+                    for (int w = 4; w > 0; w >>= 1)
+#pragma unroll
+                        for (int e = 0; e < w; e++) mx[e] = fmaxf(mx[e], mx[e + w]);
+                    const float top = mx[0] * sl;
+                    float f = 1.f;
+                    if (top > m + kRescale || (m == -INFINITY && top > -INFINITY)) {
+                        if (m != -INFINITY) f = ex2(m - top);
+                        m = top;
+                    }
+                    if (__any_sync(FULL, f != 1.f)) {  // S of this tile is done, so the products before it are
+                        l *= f;
+#pragma unroll 1
+                        for (int q = 0; q < HD / 32; q++) {
+                            float o[32];
+                            tmem_ld32(to + 32 * q, o);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] *= f;
+                            tmem_st32(to + 32 * q, o);
+                        }
+                    }
+                    // masked scores and rows that see nothing: 2^(-inf) = 0
+                    const float base = m == -INFINITY ? 0.f : -m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int e = 0; e < 128; e += 2) {
+                        const float x = ex2(fmaf(__uint_as_float(u[e]), sl, base));
+                        const float y = ex2(fmaf(__uint_as_float(u[e + 1]), sl, base));
+                        sum[(e / 2) & 3] += x + y;
+                        u[e / 2] = pack2(x, y, static_cast<T*>(nullptr));
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) w[e] = u[16 * q + e];
+                        tmem_st16(ts + 16 * q, w);
+                    }
+                    if (key0 < c.t.lo || key0 > c.t.hi - kKB) {
+                        // rows of V that no query attends to may hold anything: no 0 x NaN.  (Both streams
+                        // write the same zeros; each before its own product.)
+                        const uint32_t n = n0 + 2 * (j - p.jb) + 1, st = n % NST;
+                        if (!__all_sync(FULL, wait(&full[st], (n / NST) & 1))) {
+                            ok = false;
+                            break;
+                        }
+                        const int key = key0 + r;
+                        if (key < c.t.lo || key >= c.t.hi) {
+#pragma unroll
+                            for (int d = 0; d < HD / 8; d++)
+                                *reinterpret_cast<uint4*>(ring + st * S::STAGE + (d / 8) * S::PANEL + sw128(r, d & 7)) =
+                                    make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&p_full[i]);
+                }
+                if (ok && !__all_sync(FULL, wait(&o_full[i], no & 1))) ok = false;
+                no++;
+                tc_fence_after();
+            }
+            n0 += 2 * (p.je - p.jb);
+            // ---- epilogue: this thread's columns [c0, c1) of the row's sum over the streams ----
+            float w0 = 1.f, w1 = 0.f, mt = m, lt = l;
+            const bool fold = !p.two && p.active(1);  // two streams of keys: add them
+            if (fold) {
+                xch[i * kHalf + r] = m;
+                xch[(2 + i) * kHalf + r] = l;
+                __syncwarp();
+                if (lane == 0) bar_arrive(xbar);
+                if (!__all_sync(FULL, wait(xbar, nx & 1))) ok = false;
+                nx++;
+                const float m0 = xch[r], m1 = xch[kHalf + r];
+                mt = fmaxf(m0, m1);
+                w0 = mt == -INFINITY ? 1.f : ex2(m0 - mt);
+                w1 = mt == -INFINITY ? 1.f : ex2(m1 - mt);
+                lt = xch[2 * kHalf + r] * w0 + xch[3 * kHalf + r] * w1;
+                tc_fence_after();
+            }
+            if (!ok) break;
+            const bool whole = c.s == 0 && c.end == c.steps;
+            const bool writer = p.two || fold || i == 0;
+            const int q0 = fold ? i * (HD / 64) : 0, q1 = fold ? (i + 1) * (HD / 64) : HD / 32;  // 32-column groups
+            float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * kRows * (HD + 4);
+            if (writer) {
+                const float inv = lt != 0.f ? 1.f / lt : 0.f;
+                float z = lt * 0.f;  // NaN once a value is not finite
+                const bool t0 = fold || act;
+                const uint32_t ta = fold ? tO + lane_off : to;
+#pragma unroll 1
+                for (int q = q0; q < q1; q++) {
+                    float o[32];
+                    if (t0) {
+                        tmem_ld32(ta + 32 * q, o);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0.f;
+                    }
+                    if (fold) {
+                        float o1[32];
+                        tmem_ld32(tO + 128 + lane_off + 32 * q, o1);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = o[e] * w0 + o1[e] * w1;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) z = fmaf(o[e], 0.f, z);
+                    if (!in) continue;
+                    if (whole) {
+                        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
+                                                              (static_cast<size_t>(tok) * a.H + h) * HD + 32 * q);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            uint4 v;
+                            uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                vw[k] = pack2(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv, static_cast<T*>(nullptr));
+                            dst[e] = v;
+                        }
+                    } else {  // [4-column group][row], so that a warp's stores are whole lines
+                        float4* dst = reinterpret_cast<float4*>(part) + kRows;
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            dst[static_cast<size_t>(8 * q + e) * kRows + row] =
+                                make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    }
+                }
+                // not finite: a value that this row must not see may have met it as 0 x infinity (see tl_paged_attn.cu)
+                const bool redo = in && z != z;
+                if (whole) {
+                    for (unsigned bad = __ballot_sync(FULL, redo); bad; bad &= bad - 1) {
+                        const int src = __ffs(bad) - 1;
+                        __syncwarp();
+                        attend_row<T, HD>(a, c.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, h, src), lane);
+                    }
+                } else if (in) {
+                    float* hd = part + 4 * row;  // {max, sum, redo, redo of the other columns}
+                    if (!fold || i == 0) {
+                        hd[0] = mt;
+                        hd[1] = lt;
+                        hd[2] = redo ? 1.f : 0.f;
+                    }
+                    if (!fold || i == 1) hd[3] = redo ? 1.f : 0.f;
+                }
+            }
+            if (!whole && c.s == 0 && threadIdx.x == 0) {  // this block begins the tile: it says who has the rest
+                Head hd;
+                hd.parts = parts_of(c.steps, c.end, per);
+                hd.slot = first_tile ? 0 : 1;
+                hd.b = c.b;
+                hd.rt = c.rt;
+                hd.g = c.g;
+                heads[blockIdx.x] = hd;
+            }
+            if (fold) {  // both have read the accumulators: the next tile may overwrite them
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(xbar);
+                if (!__all_sync(FULL, wait(xbar, nx & 1))) ok = false;
+                nx++;
+            }
+        }
+        if (!ok) fail();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// Joins the parts of the tile that block blockIdx.x began (part i > 0: the first tile of block blockIdx.x + i).
+// Block y takes 32 rows: lane = row, warp = one 8th of the columns.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) k_attend_chunk_join(AttendArgs a, const Head* heads, const float* parts) {
+    pdl_wait();
+    const Head h = heads[blockIdx.x];
+    if (h.parts == 0) return;
+    const Tile t = tile_of(a, h.b, h.rt, kRows);
+    if (static_cast<int>(blockIdx.y) * 32 >= t.nrows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = blockIdx.y * 32 + lane;
+    const bool in = row < t.nrows;
+    constexpr size_t rec = static_cast<size_t>(kRows) * (HD / 4 + 1);  // float4s of a part
+    constexpr int G = HD / 4 / 8;                                      // 4-column groups of a warp
+    const float4* p0 = reinterpret_cast<const float4*>(parts) + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
+    const float4* p1 = reinterpret_cast<const float4*>(parts) + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;
+    auto part = [&](int i) { return i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec; };
+    float M = -INFINITY, bad = 0.f;
+    if (in)
+        for (int i = 0; i < h.parts; i++) {
+            const float4 s = part(i)[row];
+            M = fmaxf(M, s.x);
+            bad += s.z + s.w;
+        }
+    float L = 0.f;
+    float4 acc[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) acc[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in)
+        for (int i = 0; i < h.parts; i++) {
+            const float4* p = part(i);
+            const float4 s = p[row];
+            const float f = M == -INFINITY ? 1.f : ex2(s.x - M);
+            L += s.y * f;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const float4 v = p[static_cast<size_t>(1 + warp * G + g) * kRows + row];
+                acc[g].x += v.x * f;
+                acc[g].y += v.y * f;
+                acc[g].z += v.z * f;
+                acc[g].w += v.w * f;
+            }
+        }
+    const int fr = t.r0 + (in ? row : 0), tok = t.first + fr / a.group, hh = h.g * a.group + fr % a.group;
+    const unsigned again = __ballot_sync(FULL, in && bad > 0.f);
+    if (in && !(bad > 0.f)) {
+        const float inv = L != 0.f ? 1.f / L : 0.f;
+        uint2* dst = reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD) + warp * G;
+#pragma unroll
+        for (int g = 0; g < G; g++)
+            dst[g] = make_uint2(pack2(acc[g].x * inv, acc[g].y * inv, static_cast<T*>(nullptr)),
+                                pack2(acc[g].z * inv, acc[g].w * inv, static_cast<T*>(nullptr)));
+    }
+    if (warp == 0)
+        for (unsigned b = again; b; b &= b - 1) {
+            const int src = __ffs(b) - 1;
+            attend_row<T, HD>(a, h.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, hh, src), lane);
+        }
+}
+
+template <typename T, int HD>
+tl_status run_chunk(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
+    using S = Shape<HD>;
+    static_assert(S::SMEM <= 232448, "shared memory of a block");
+    CUtensorMap mk, mv;
+    const int rows = std::min(kKB, 1 << a.shift);
+    TL_TRY(encode_pages(&mk, c->k, c, rows, 1));
+    TL_TRY(encode_pages(&mv, c->v, c, rows, 1));
+    TL_CUDA_TRY(cudaFuncSetAttribute(k_attend_chunk<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(S::SMEM)));
+    const int grid = std::min(sm_count(), kMaxBlocks);
+    Head* heads = static_cast<Head*>(workspace);
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeadBytes);
+    k_attend_chunk<T, HD><<<grid, kThreads, S::SMEM, s>>>(mk, mv, a, heads, parts);
+    TL_TRY(check_launch("paged_attention"));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, kRows / 32);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_attend_chunk_join<T, HD>, a, static_cast<const Head*>(heads),
+                                   static_cast<const float*>(parts)));
+    return TL_OK;
+}
+
+}  // namespace
+
+size_t chunk_workspace(int hd) {
+    return kHeadBytes + static_cast<size_t>(std::min(sm_count(), kMaxBlocks)) * 2 * kRows * (hd + 4) * 4;
+}
+
+tl_status attend_chunk(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
+    const bool half = c->dtype == TL_F16;
+    if (c->head_dim == 128)
+        return half ? run_chunk<__half, 128>(a, c, workspace, s) : run_chunk<__nv_bfloat16, 128>(a, c, workspace, s);
+    return half ? run_chunk<__half, 64>(a, c, workspace, s) : run_chunk<__nv_bfloat16, 64>(a, c, workspace, s);
+}
+
+}  // namespace paged
+}  // namespace tl
