@@ -66,6 +66,16 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
+// Waits by polling (the copies are short, and a suspended wait may wake late); false after ~2 s.
+__device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity) {
+    if (bar_test_now(b, parity)) return true;
+    const unsigned long long t0 = gtime();
+    for (unsigned i = 1;; i++) {
+        if (bar_test_now(b, parity)) return true;
+        if ((i & 255) == 0 && gtime() - t0 > kTimeoutNs) return false;
+    }
+}
+
 // Keys per step, stages per warp, and the bytes of one side of a stage.
 template <typename T, int HD>
 struct Shape {
@@ -151,12 +161,12 @@ struct Core {
         for (int i = 0; i < 2; i++) {
             const int r = lane / 4 + 8 * i;
             const bool in = r < c.t.nrows;
-            const int fr = c.t.r0 + (in ? r : 0);
-            const int tok = fr / a.group, h = c.g * a.group + fr % a.group;
-            attended(a, c.t.p0 + tok, lo[i], hi[i]);
+            int tok, h;
+            row_of(a, c, r, tok, h);
+            attended(a, c.t.p0 + (tok - c.t.first), lo[i], hi[i]);
             if (!in) hi[i] = 0;
             const uint32_t* src = reinterpret_cast<const uint32_t*>(
-                qb + static_cast<size_t>(c.t.first + tok) * a.q_stride + static_cast<size_t>(h) * HD) + (lane & 3);
+                qb + static_cast<size_t>(tok) * a.q_stride + static_cast<size_t>(h) * HD) + (lane & 3);
 #pragma unroll
             for (int k = 0; k < HD / 16; k++) {
                 q[k][i] = in ? src[8 * k] : 0u;
@@ -321,9 +331,9 @@ struct Core<float, HD, R> {
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const bool in = r < c.t.nrows;
-            const int fr = c.t.r0 + (in ? r : 0);
-            const int tok = fr / a.group, h = c.g * a.group + fr % a.group;
-            load(q[r], qb + static_cast<size_t>(c.t.first + tok) * a.q_stride + static_cast<size_t>(h) * HD + lane * D);
+            int tok, h;
+            row_of(a, c, r, tok, h);
+            load(q[r], qb + static_cast<size_t>(tok) * a.q_stride + static_cast<size_t>(h) * HD + lane * D);
 #pragma unroll
             for (int d = 0; d < D; d++) {
                 if (!in) q[r][d] = 0.f;
@@ -334,7 +344,7 @@ struct Core<float, HD, R> {
 #pragma unroll
         for (int g = 0; g < RG; g++) {
             const int r = 4 * g + lane / 8;
-            attended(a, c.t.p0 + (c.t.r0 + r) / a.group, lo[g], hi[g]);
+            attended(a, c.t.p0 + div_group(a, c.t.r0 + r), lo[g], hi[g]);
             if (r >= c.t.nrows) hi[g] = 0;
             l[g] = 0.f;
         }
@@ -441,7 +451,8 @@ struct Core<float, HD, R> {
 
 template <typename T, int HD, int R>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_attend_split(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, AttendArgs a,
+    k_attend_split(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                   const __grid_constant__ AttendArgs a,
                    Head* heads, float* parts) {
     using S = Shape<T, HD>;
     constexpr int KS = S::KS, NST = S::NST;
@@ -451,8 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* ring = base + static_cast<size_t>(warp) * NST * 2 * S::SIDE;
     float* join = reinterpret_cast<float*>(base + static_cast<size_t>(kWarps) * NST * 2 * S::SIDE);
     uint64_t* bars = reinterpret_cast<uint64_t*>(join + kWarps * S::JOIN) + warp * NST;
-    long long* ws = reinterpret_cast<long long*>(join + kWarps * S::JOIN) + kWarps * NST;  // [kWarps]
-    int* found = reinterpret_cast<int*>(ws + kWarps);
+    long long* ws = reinterpret_cast<long long*>(join + kWarps * S::JOIN) + kWarps * NST;  // [kWarps + 2]
 
     if (lane == 0) {
         for (int i = 0; i < NST; i++) bar_init(&bars[i], 1);
@@ -463,76 +473,85 @@ __global__ void __launch_bounds__(kThreads, 1)
     using P = SplitPlan<R, KS>;
     Cursor c;
     // at least one step a warp, so that a small call is not cut into crumbs
-    const long long per = find_share<P, kWarps>(a, c, ws, found, kWarps);
+    const int per = find_share<P, kWarps>(a, c, ws, kWarps);
     if (per == 0) return;
 
     // producer: a second cursor that runs up to NST steps ahead; ids of this warp's next 32 steps in the lanes
     Cursor pc = c;
-    int ps = pc.s + warp, pid_at = 0, pid0 = -1, pid1 = -1;
-    bool more = true, fresh = true;
-    int put = 0, got = 0;
+    int ps = pc.s + warp, pid_at = 32, pid0 = -1, pid1 = -1;
+    bool more = true;
+    int put_st = 0, got_st = 0, ahead = 0;
+    uint32_t got_parity = 0;
     uint32_t valid_bits = 0;  // 2 bits for each stage
     int stage_key[NST];
-    auto produce = [&]() {
-        while (more && ps >= pc.end) {
-            more = next_tile<P>(a, pc);
-            ps = pc.s + warp;
-            fresh = true;
-        }
-        if (!more) return;
-        if (fresh || pid_at == 32) {
-            const long long key = (static_cast<long long>(pc.t.lo / KS) + ps + static_cast<long long>(kWarps) * lane) * KS;
-            const int k32 = key < 0x7fffff00ll ? static_cast<int>(key) : -1;
-            pid0 = page_of(a, pc.b, k32);
-            pid1 = (KS == 16 && a.shift == 3) ? page_of(a, pc.b, k32 < 0 ? -1 : k32 + 8) : pid0;
-            pid_at = 0;
-            fresh = false;
-        }
-        const int id0 = __shfl_sync(FULL, pid0, pid_at), id1 = __shfl_sync(FULL, pid1, pid_at);
-        pid_at++;
-        const int st = put % NST;
-        const int key0 = (pc.t.lo / KS + ps) * KS;
-        const uint32_t v = (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u);
-        valid_bits = (valid_bits & ~(3u << (2 * st))) | (v << (2 * st));
 #pragma unroll
-        for (int i = 0; i < NST; i++)
-            if (i == st) stage_key[i] = key0;
-        if (lane == 0) {
-            uint8_t* k = ring + st * 2 * S::SIDE;
-            uint8_t* vv = k + S::SIDE;
-            const int row = (pc.g << a.shift) + (key0 & ((1 << a.shift) - 1));
-            bar_expect_tx(&bars[st], 2 * S::SIDE);
-            tma_page(k, &map_k, row, id0, &bars[st]);
-            tma_page(vv, &map_v, row, id0, &bars[st]);
-            if (KS == 16 && a.shift == 3) {
-                tma_page(k + S::SIDE / 2, &map_k, pc.g << 3, id1, &bars[st]);
-                tma_page(vv + S::SIDE / 2, &map_v, pc.g << 3, id1, &bars[st]);
-            }
-        }
-        put++;
-        ps += kWarps;
-    };
+    for (int i = 0; i < NST; i++) stage_key[i] = 0;
     __syncwarp();
-    for (int i = 0; i < NST; i++) produce();
 
     Core<T, HD, R> core;
     bool first_tile = true, dead = false;
+#pragma unroll 1
     for (bool go = true; go; go = next_tile<P>(a, c), first_tile = false) {
-        core.begin(a, c, lane);
-        for (int s = c.s + warp; s < c.end; s += kWarps) {
-            const int st = got % NST;
-            dead |= !bar_wait(&bars[st], (got / NST) & 1);
+        bool begun = false;
+#pragma unroll 1
+        for (int s = c.s + warp;; s += kWarps) {
+#pragma unroll 1
+            while (more && ahead < NST) {  // one step into the ring
+                if (ps >= pc.end) {
+                    more = next_tile<P>(a, pc);
+                    ps = pc.s + warp;
+                    pid_at = 32;
+                    continue;
+                }
+                if (pid_at == 32) {
+                    const int blk = (pc.t.lo / KS + ps) + kWarps * lane;  // below 2^31 / KS + 256
+                    const int key = blk < kMaxLen / KS ? blk * KS : -1;
+                    pid0 = page_of(a, pc.b, key);
+                    pid1 = (KS == 16 && a.shift == 3) ? page_of(a, pc.b, key < 0 ? -1 : key + 8) : pid0;
+                    pid_at = 0;
+                }
+                const int id0 = __shfl_sync(FULL, pid0, pid_at), id1 = __shfl_sync(FULL, pid1, pid_at);
+                pid_at++;
+                const int key0 = (pc.t.lo / KS + ps) * KS;
+                const uint32_t v = (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u);
+                valid_bits = (valid_bits & ~(3u << (2 * put_st))) | (v << (2 * put_st));
+#pragma unroll
+                for (int i = 0; i < NST; i++)
+                    if (i == put_st) stage_key[i] = key0;
+                if (lane == 0) {
+                    uint8_t* k = ring + put_st * 2 * S::SIDE;
+                    uint8_t* vv = k + S::SIDE;
+                    const int row = (pc.g << a.shift) + (key0 & ((1 << a.shift) - 1));
+                    bar_expect_tx(&bars[put_st], 2 * S::SIDE);
+                    tma_page(k, &map_k, row, id0, &bars[put_st]);
+                    tma_page(vv, &map_v, row, id0, &bars[put_st]);
+                    if (KS == 16 && a.shift == 3) {
+                        tma_page(k + S::SIDE / 2, &map_k, pc.g << 3, id1, &bars[put_st]);
+                        tma_page(vv + S::SIDE / 2, &map_v, pc.g << 3, id1, &bars[put_st]);
+                    }
+                }
+                put_st = put_st + 1 == NST ? 0 : put_st + 1;
+                ahead++;
+                ps += kWarps;
+            }
+            if (!begun) {
+                core.begin(a, c, lane);
+                begun = true;
+            }
+            if (s >= c.end) break;
+            dead |= !spin(&bars[got_st], (got_parity >> got_st) & 1);
+            got_parity ^= 1u << got_st;
             StepInfo si;
-            si.valid = (valid_bits >> (2 * st)) & 3u;
+            si.valid = (valid_bits >> (2 * got_st)) & 3u;
             si.key0 = 0;
 #pragma unroll
             for (int i = 0; i < NST; i++)
-                if (i == st) si.key0 = stage_key[i];
-            const uint8_t* k = ring + st * 2 * S::SIDE;
+                if (i == got_st) si.key0 = stage_key[i];
+            const uint8_t* k = ring + got_st * 2 * S::SIDE;
             core.step(a, c, si, k, k + S::SIDE, lane);
-            got++;
+            got_st = got_st + 1 == NST ? 0 : got_st + 1;
+            ahead--;
             __syncwarp();  // every lane has read the stage
-            produce();
         }
         // A result that is not finite: a value that one row must not see may have met it as 0 x infinity,
         // or an infinite value the split weights.  Such a tile is done over row by row, which gives the
@@ -541,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool whole = c.s == 0 && c.end == c.steps;
         float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * R * (HD + 4);
         const int any_redo = __syncthreads_or(redo);
+#pragma unroll 1
         for (int pass = 0; pass * 8 < c.t.nrows; pass++) {
             if (pass) __syncthreads();
             core.dump(join + warp * S::JOIN, pass, lane);
@@ -563,7 +583,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int d = 0; d < HD / 32; d++) acc[d] += j[w * S::JOIN + 4 + lane + 32 * d] * f;
                 }
-                const int fr = c.t.r0 + row, tok = c.t.first + fr / a.group, h = c.g * a.group + fr % a.group;
+                int tok, h;
+                row_of(a, c, row, tok, h);
                 if (whole) {
                     if (any_redo) {
                         attend_row<T, HD>(a, c.b, tok, h, lane);
@@ -599,16 +620,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the parts of the tile that block blockIdx.x began: part i > 0 is the first tile of block blockIdx.x + i.
 template <typename T, int HD, int R>
-__global__ void __launch_bounds__(kThreads) k_attend_join(AttendArgs a, const Head* heads, const float* parts) {
+__global__ void __launch_bounds__(kThreads) k_attend_join(const __grid_constant__ AttendArgs a, const Head* heads, const float* parts) {
     pdl_wait();
     const Head h = heads[blockIdx.x];
     if (h.parts == 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Tile t = tile_of(a, h.b, h.rt, R);
+    Cursor c;
+    c.g = h.g;
+    c.t = tile_of(a, h.b, h.rt, R);
     constexpr size_t rec = static_cast<size_t>(R) * (HD + 4);
     const float* p0 = parts + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
     const float* p1 = parts + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;  // parts 1 .. are 2 * rec apart
-    for (int row = warp; row < t.nrows; row += kWarps) {
+    for (int row = warp; row < c.t.nrows; row += kWarps) {
         float M = -INFINITY, bad = 0.f;
         for (int i = lane; i < h.parts; i += 32) {
             const float* p = (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4);
@@ -617,7 +640,8 @@ __global__ void __launch_bounds__(kThreads) k_attend_join(AttendArgs a, const He
         }
         M = warp_max(M);
         bad = warp_max(bad);
-        const int fr = t.r0 + row, tok = t.first + fr / a.group, hh = h.g * a.group + fr % a.group;
+        int tok, hh;
+        row_of(a, c, row, tok, hh);
         if (bad > 0.f) {
             attend_row<T, HD>(a, h.b, tok, hh, lane);
             continue;
@@ -755,9 +779,11 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.H = static_cast<int>(n_heads);
     a.KV = static_cast<int>(cache->n_kv_heads);
     a.group = a.H / a.KV;
+    a.group_inv = ~0ull / static_cast<unsigned long long>(a.group) + 1;
     a.max_blocks = static_cast<int>(max_blocks);
     a.n_blocks = static_cast<int>(cache->n_blocks);
     a.shift = __builtin_ctzll(cache->block_size);
+    a.cap = static_cast<int>(std::min<size_t>(max_blocks << a.shift, kMaxLen));
     a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
     a.scale = scale == 0.f ? 1e-30f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
     return many_rows(cache, n_tokens, n_heads, n_seq) ? attend_chunk(a, cache, workspace, as_stream(stream))

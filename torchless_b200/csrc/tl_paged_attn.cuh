@@ -10,6 +10,8 @@
 namespace tl {
 namespace paged {
 
+constexpr int kMaxLen = 0x7fff0000;  // longer lengths count as this one
+
 struct AttendArgs {
     void* out;           // [n_tokens][H][hd]
     const void* q;       // rows q_stride elements apart
@@ -20,9 +22,16 @@ struct AttendArgs {
     const int32_t* seq_lens;  // [n_seq]
     size_t q_stride, block_stride;
     int n_seq, n_tokens, H, KV, group, max_blocks, n_blocks, shift;  // block size 1 << shift
+    int cap;      // positions that a table can name, at most kMaxLen
     int window;   // 0: none
     float scale;
+    unsigned long long group_inv;  // ceil(2^64 / group)
 };
+
+// r / group, r >= 0 (exact: r < 2^32, and the inverse is off by less than 2^-32 relative)
+__device__ __forceinline__ int div_group(const AttendArgs& a, int r) {
+    return a.group == 1 ? r : static_cast<int>(__umul64hi(static_cast<unsigned long long>(r), a.group_inv));
+}
 
 // 2^x (hardware approximation, 2 ulp; 2^-inf = +0)
 __device__ __forceinline__ float ex2(float x) {
@@ -37,11 +46,14 @@ __device__ __forceinline__ void rows_of(const AttendArgs& a, int b, int& first, 
     n = max(0, min(a.q_start[b + 1], a.n_tokens) - first);
 }
 
+// Position of the first query row of a sequence with n of them.
+__device__ __forceinline__ int first_pos(const AttendArgs& a, int b, int n) { return min(a.seq_lens[b], kMaxLen) - n; }
+
 // Positions [lo, hi) that the query at position p of a sequence may attend to
 // (pages that do not exist are left out later, key by key).
-__device__ __forceinline__ void attended(const AttendArgs& a, long long p, int& lo, int& hi) {
-    hi = static_cast<int>(min(p + 1, static_cast<long long>(a.max_blocks) << a.shift));
-    lo = a.window > 0 ? static_cast<int>(max(0ll, p + 1 - a.window)) : 0;
+__device__ __forceinline__ void attended(const AttendArgs& a, int p, int& lo, int& hi) {
+    hi = min(p + 1, a.cap);
+    lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
 }
 
 // The page of position key of sequence b; -1 if there is none.
@@ -58,7 +70,7 @@ __device__ __forceinline__ int page_of(const AttendArgs& a, int b, int key) {
 struct Tile {
     int first, n;        // the sequence's token rows
     int r0, nrows;       // rows of the tile
-    long long p0;        // position of the sequence's first token row
+    int p0;              // position of the sequence's first token row
     int lo, lo_last;     // first attended position of the tile's first and last token
     int hi, hi_first;    // end of the attended positions of the last and first token
 };
@@ -67,9 +79,9 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs& a, int b, int rt, int 
     rows_of(a, b, t.first, t.n);
     t.r0 = rt * rows;
     t.nrows = min(rows, t.n * a.group - t.r0);
-    t.p0 = static_cast<long long>(a.seq_lens[b]) - t.n;
-    attended(a, t.p0 + t.r0 / a.group, t.lo, t.hi_first);
-    attended(a, t.p0 + (t.r0 + t.nrows - 1) / a.group, t.lo_last, t.hi);
+    t.p0 = first_pos(a, b, t.n);
+    attended(a, t.p0 + div_group(a, t.r0), t.lo, t.hi_first);
+    attended(a, t.p0 + div_group(a, max(0, t.r0 + t.nrows - 1)), t.lo_last, t.hi);
     return t;
 }
 
@@ -90,7 +102,7 @@ static_assert(sizeof(Head) * kMaxBlocks <= kHeadBytes, "heads");
 struct Cursor {
     int b, rt, g;
     int s, end, steps;
-    long long left;  // steps of the block from this tile's step s on
+    int left;  // steps of the block from this tile's step s on
     Tile t;
 };
 
@@ -98,7 +110,7 @@ template <class Plan>
 __device__ __forceinline__ void enter(const AttendArgs& a, Cursor& c) {
     c.t = tile_of(a, c.b, c.rt, Plan::R);
     c.steps = Plan::steps(c.t);
-    c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
+    c.end = min(c.steps, c.s + c.left);
 }
 // To the next tile that has rows; false when the block's share is done.
 template <class Plan>
@@ -142,51 +154,69 @@ __device__ __forceinline__ long long scan_block(long long v, long long* ws, long
     return x - v + before;
 }
 
+// Steps of sequence b's tiles rt0, rt0 + stride, ... of one kv head.
 template <class Plan>
-__device__ __forceinline__ long long steps_of_sequence(const AttendArgs& a, int b) {
+__device__ __noinline__ long long steps_of_sequence(const AttendArgs& a, int b, int rt0, int stride) {
     if (b >= a.n_seq) return 0;
     int first, n;
     rows_of(a, b, first, n);
     long long u = 0;
-    for (int rt = 0; rt * Plan::R < n * a.group; rt++) u += Plan::steps(tile_of(a, b, rt, Plan::R));
-    return u * a.KV;
+    for (int rt = rt0; rt * Plan::R < n * a.group; rt += stride) u += Plan::steps(tile_of(a, b, rt, Plan::R));
+    return u;
+}
+__device__ __forceinline__ long long warp_sum_ll(long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
 }
 
 // This block's share: `c` at its first tile; returns the steps of a full share, 0 if there is nothing
-// for this block.  All NW warps call it.  ws: [NW], found: [1], in shared memory.
+// for this block.  All NW warps call it.  ws: [NW + 2] in shared memory.
 template <class Plan, int NW>
-__device__ long long find_share(const AttendArgs& a, Cursor& c, long long* ws, int* found, int least) {
+__device__ __forceinline__ int find_share(const AttendArgs& a, Cursor& c, long long* ws, int least) {
     constexpr int NT = NW * 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // a thread (few tiles each) or a warp (few sequences) adds up a sequence
+    const bool wide = a.n_seq <= NW;
+    const int unit = wide ? warp : threadIdx.x;
+    auto steps_at = [&](int b) -> long long {  // of sequence b; wide: lane 0 has it
+        if (!wide) return steps_of_sequence<Plan>(a, b, 0, 1) * a.KV;
+        const long long s = warp_sum_ll(steps_of_sequence<Plan>(a, b, lane, 32)) * a.KV;
+        return lane == 0 ? s : 0;
+    };
     long long total = 0;
-    const long long mine = steps_of_sequence<Plan>(a, threadIdx.x);
+    const long long mine = steps_at(unit);
     const long long at0 = scan_block<NW>(mine, ws, total);
     const long long chunk0 = total;
     if (a.n_seq > NT) {  // the rest of the sequences: their sum first
         long long rest = 0, sum;
-        for (int b = NT + threadIdx.x; b < a.n_seq; b += NT) rest += steps_of_sequence<Plan>(a, b);
+        for (int b = NT + threadIdx.x; b < a.n_seq; b += NT) rest += steps_at(b);
         scan_block<NW>(rest, ws, sum);
         total += sum;
     }
-    const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(least));
+    const unsigned t32 = static_cast<unsigned>(min(total, 0xffff0000ll));  // (32-bit division where it is enough)
+    const long long per = max(total <= 0xffff0000ll ? static_cast<long long>((t32 + gridDim.x - 1) / gridDim.x)
+                                                    : (total + gridDim.x - 1) / gridDim.x,
+                              static_cast<long long>(least));
+    if (per > 0x40000000ll) return 0;  // (days of work: no such memory)
     const long long u0 = per * blockIdx.x;
     if (u0 >= total) return 0;
-    if (threadIdx.x == 0) *found = -1;
+    if (threadIdx.x == 0) ws[NW + 1] = -1;
     __syncthreads();
     auto place = [&](int b, long long at, long long n) {
         if (u0 >= at && u0 < at + n) {
-            *found = b;
-            ws[0] = u0 - at;
+            ws[NW] = u0 - at;
+            ws[NW + 1] = b;
         }
     };
     if (u0 < chunk0) {
-        place(threadIdx.x, at0, mine);
+        place(unit, at0, mine);
     } else {
         long long before = chunk0;
         for (int b0 = NT; b0 < a.n_seq; b0 += NT) {
-            const long long n = steps_of_sequence<Plan>(a, b0 + threadIdx.x);
+            const long long n = steps_at(b0 + threadIdx.x);
             long long sum;
             const long long at = before + scan_block<NW>(n, ws, sum);
-            __syncthreads();
             if (u0 < before + sum) {
                 place(b0 + threadIdx.x, at, n);
                 break;
@@ -195,25 +225,50 @@ __device__ long long find_share(const AttendArgs& a, Cursor& c, long long* ws, i
         }
     }
     __syncthreads();
-    if (*found < 0) return 0;  // (the lengths changed under the call)
-    c.b = *found;
-    c.rt = 0;
-    c.left = min(per, total - u0);
-    long long u = ws[0];
-    for (;; c.rt++) {
-        c.t = tile_of(a, c.b, c.rt, Plan::R);
-        c.steps = Plan::steps(c.t);
-        if (u < static_cast<long long>(c.steps) * a.KV) break;
-        u -= static_cast<long long>(c.steps) * a.KV;
+    if (ws[NW + 1] < 0) return 0;  // (the lengths changed under the call)
+    c.b = static_cast<int>(ws[NW + 1]);
+    c.left = static_cast<int>(min(per, total - u0));
+    // the row tile: 32 of them at a time, every warp for itself
+    long long u = ws[NW];
+    int first, n;
+    rows_of(a, c.b, first, n);
+    for (c.rt = 0;; c.rt += 32) {
+        const int rt = c.rt + lane;
+        const long long s = rt * Plan::R < n * a.group ? static_cast<long long>(Plan::steps(tile_of(a, c.b, rt, Plan::R))) * a.KV : 0;
+        long long x = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(FULL, x, o);
+            if (lane >= o) x += y;
+        }
+        const unsigned past = __ballot_sync(FULL, x > u);  // tiles that end behind u
+        if (past) {
+            const int k = __ffs(past) - 1;
+            u -= __shfl_sync(FULL, x - s, k);
+            c.rt += k;
+            break;
+        }
+        u -= __shfl_sync(FULL, x, 31);
+        if ((c.rt + 32) * Plan::R >= n * a.group) return 0;  // (as above)
     }
-    c.g = static_cast<int>(u / c.steps);
-    c.s = static_cast<int>(u % c.steps);
-    c.end = static_cast<int>(min(static_cast<long long>(c.steps), c.s + c.left));
-    return per;
+    c.t = tile_of(a, c.b, c.rt, Plan::R);
+    c.steps = Plan::steps(c.t);
+    c.g = u < 0x100000000ll ? static_cast<int>(static_cast<unsigned>(u) / static_cast<unsigned>(c.steps))
+                            : static_cast<int>(u / c.steps);
+    c.s = static_cast<int>(u - static_cast<long long>(c.g) * c.steps);
+    c.end = min(c.steps, c.s + c.left);
+    return static_cast<int>(per);
 }
 // The number of blocks that share a tile whose first block ends at step `end` of `steps`.
-__device__ __forceinline__ int parts_of(int steps, int end, long long per) {
-    return 1 + static_cast<int>((steps - end + per - 1) / per);
+__device__ __forceinline__ int parts_of(int steps, int end, int per) {
+    return 1 + (steps - end + per - 1) / per;
+}
+
+// Row r0 + r of a tile: its token row and its q head (rows that do not exist: the tile's first).
+__device__ __forceinline__ void row_of(const AttendArgs& a, const Cursor& c, int r, int& tok, int& h) {
+    const int fr = c.t.r0 + (r < c.t.nrows ? r : 0), i = div_group(a, fr);
+    tok = c.t.first + i;
+    h = c.g * a.group + fr - i * a.group;
 }
 
 // One (token, head) by one warp, straight from the pages in fp32: lane l holds
@@ -223,10 +278,10 @@ __device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h
     constexpr int D = HD / 32;
     int first, n;
     rows_of(a, b, first, n);
-    const long long p = static_cast<long long>(a.seq_lens[b]) - n + (t - first);
+    const int p = first_pos(a, b, n) + (t - first);
     int lo, hi;
     attended(a, p, lo, hi);
-    const int g = h / a.group;
+    const int g = div_group(a, h);
     const T* qp = static_cast<const T*>(a.q) + static_cast<size_t>(t) * a.q_stride + static_cast<size_t>(h) * HD + lane * D;
     float q[D], acc[D];
 #pragma unroll

@@ -103,6 +103,15 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t pack2(float x, float y, __half*) {
@@ -137,7 +146,7 @@ __device__ __forceinline__ Part part_of(const AttendArgs& a, const Cursor& c) {
     p.end0 = p.je;
     if (p.two) {
         int lo, hi;
-        attended(a, c.t.p0 + (c.t.r0 + kHalf - 1) / a.group, lo, hi);
+        attended(a, c.t.p0 + div_group(a, c.t.r0 + kHalf - 1), lo, hi);
         p.end0 = hi <= 0 ? 0 : max(0, min(p.je, (hi - 1) / kKB - p.kb0 + 1));
     }
     return p;
@@ -145,7 +154,8 @@ __device__ __forceinline__ Part part_of(const AttendArgs& a, const Cursor& c) {
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_attend_chunk(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, AttendArgs a,
+    k_attend_chunk(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                   const __grid_constant__ AttendArgs a,
                    Head* heads, float* parts) {
     using S = Shape<HD>;
     constexpr int NST = S::NST;
@@ -164,13 +174,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);  // [2][128] max, [2][128] sum
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xch + 4 * kHalf);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* found = reinterpret_cast<int*>(tmem_slot + 2);
     long long* ws = reinterpret_cast<long long*>(ring);  // the scan runs before the ring is used
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) heads[blockIdx.x].parts = 0;
     Cursor c;
-    const long long per = find_share<ChunkPlan, kWarps>(a, c, ws, found, 2);
+    const int per = find_share<ChunkPlan, kWarps>(a, c, ws, 2);
     if (per == 0) return;
 
     if (threadIdx.x == 0) {
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = tmem, tO = tmem + 256;  // S_i at + 128 i, O_i at + 128 i
 
     auto fail = [&] { *abort_flag = 1; };
-    auto wait = [&](uint64_t* b, uint32_t parity) { return bar_wait_ab(b, parity, abort_flag); };
+    auto wait = [&](uint64_t* b, uint32_t parity) { return bar_spin_ab(b, parity, abort_flag); };
 
     if (warp == 8) {
         // ---- TMA: K_j, V_j of each key tile; lane = one page's rows of one panel ----
@@ -244,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ---- MMA ----
             constexpr uint32_t id_s = idesc<T>(kKB, false), id_o = idesc<T>(HD, true);
             uint32_t n0 = 0;              // loads before this tile
-            uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+            uint32_t nq = 0, np = 0;      // phases of the streams' barriers
             bool ok = true;
             for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
                 const Part p = part_of(a, c);
@@ -264,8 +273,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return true;
                 };
                 auto values = [&](int i, int j) -> bool {  // O_i (+)= P_i V_j
-                    if (!wait(&p_full[i], np[i] & 1)) return false;
-                    np[i]++;
+                    if (!wait(&p_full[i], (np >> i) & 1)) return false;
+                    np ^= 1u << i;
                     const uint32_t n = n0 + 2 * (j - p.jb) + 1, st = n % NST;
                     if (!wait(&full[st], (n / NST) & 1)) return false;
                     tc_fence_after();
@@ -277,21 +286,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return true;
                 };
                 const int stride = p.stride();
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-                    if (ok && p.active(i)) {
-                        ok = wait(&q_full[i], nq[i] & 1);
-                        nq[i]++;
-                        tc_fence_after();
-                        ok = ok && scores(i, p.begin(i));
-                    }
-                for (int j = p.jb; ok && j < p.je; j += stride)
-#pragma unroll
+                // begin: the first scores of both streams; then values and next scores, in turn
+#pragma unroll 1
+                for (int j = p.jb - stride; ok && j < p.je; j += stride)
+#pragma unroll 1
                     for (int i = 0; i < 2; i++) {
                         const int ji = p.two ? j : j + i;
-                        if (!ok || ji >= p.end(i)) continue;
-                        ok = values(i, ji);
-                        if (ok && ji + stride < p.end(i)) ok = scores(i, ji + stride);
+                        const bool start = j < p.jb;
+                        if (!ok || !p.active(i) || ji >= p.end(i)) continue;
+                        if (start) {
+                            ok = wait(&q_full[i], (nq >> i) & 1);
+                            nq ^= 1u << i;
+                            tc_fence_after();
+                        } else {
+                            ok = values(i, ji);
+                        }
+                        const int jn = start ? p.begin(i) : ji + stride;
+                        if (ok && jn < p.end(i)) ok = scores(i, jn);
                         else if (ok) umma_commit(&o_full[i]);
                     }
                 n0 += 2 * (p.je - p.jb);
@@ -313,30 +324,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Part p = part_of(a, c);
             const int row = p.two ? i * kHalf + r : r;  // of the tile
             const bool in = row < c.t.nrows;
-            const int fr = c.t.r0 + (in ? row : 0);
-            const int tok = c.t.first + fr / a.group, h = c.g * a.group + fr % a.group;
+            int tok, h;
+            row_of(a, c, row, tok, h);
             const bool act = p.active(i);
             int lo, hi;
-            attended(a, c.t.p0 + fr / a.group, lo, hi);
+            attended(a, c.t.p0 + (tok - c.t.first), lo, hi);
             float m = -INFINITY, l = 0.f;
             if (act) {
-                {  // the Q row into the swizzled K-major panels
-                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                                                      static_cast<size_t>(tok) * a.q_stride +
-                                                                      static_cast<size_t>(h) * HD);
-#pragma unroll
-                    for (int d = 0; d < HD / 8; d++) {
-                        const uint4 v = in ? src[d] : make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(sQ + i * S::STAGE + (d / 8) * S::PANEL + sw128(r, d & 7)) = v;
+                {  // this warp's 32 Q rows into the swizzled K-major panels, row by row
+                    const unsigned long long mine =
+                        in ? static_cast<unsigned long long>(tok) * a.q_stride + static_cast<unsigned long long>(h) * HD : ~0ull;
+                    constexpr int CH = HD / 8, RPI = 32 / CH;  // 16-byte pieces of a row, rows a load
+#pragma unroll 8
+                    for (int q = 0; q < 32 / RPI; q++) {
+                        const int rr = q * RPI + lane / CH, d = lane % CH;
+                        const unsigned long long at = __shfl_sync(FULL, mine, rr);
+                        const uint4 v = at != ~0ull ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at)[d]
+                                                    : make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(sQ + i * S::STAGE + (d / 8) * S::PANEL + sw128((warp & 3) * 32 + rr, d & 7)) = v;
                     }
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&q_full[i]);
                 }
+                auto page_at = [&](int j) { return lane < kKB / 8 ? page_of(a, c.b, (p.kb0 + j) * kKB + 8 * lane) : 0; };
+                int pid_next = page_at(p.begin(i));
                 const int stride = p.stride();
                 for (int j = p.begin(i); j < p.end(i); j += stride) {
                     const int key0 = (p.kb0 + j) * kKB;
-                    const int pid = lane < kKB / 8 ? page_of(a, c.b, key0 + 8 * lane) : 0;
+                    const int pid = pid_next;
+                    pid_next = j + stride < p.end(i) ? page_at(j + stride) : 0;
                     // every lane waits; the outcome is warp-uniform (tensor-memory access is warp-wide)
                     if (!__all_sync(FULL, wait(&s_full[i], ns & 1))) {
                         ok = false;
@@ -344,32 +361,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     ns++;
                     tc_fence_after();
-                    uint32_t u[128];
-#pragma unroll
-                    for (int q = 0; q < 4; q++) tmem_ld32_async(ts + 32 * q, u + 32 * q);
                     const uint32_t pages = __ballot_sync(FULL, pid >= 0);  // bit k: keys 8 k .. 8 k + 7 exist
-                    const bool inner = !in || (key0 >= lo && key0 <= hi - kKB);
-                    tmem_wait_ld();
-                    if (scale < 0.f) {
+                    const bool edge = !__all_sync(FULL, !in || (key0 >= lo && key0 <= hi - kKB)) || pages != FULL;
+                    // Masked columns, and the sign of a negative scale, go into the scores in tensor memory first;
+                    // only the border tiles of a row need that, and the loops below stay short.
+                    if (edge || scale < 0.f) {
+                        const uint32_t sign = scale < 0.f ? 0x80000000u : 0u;
+#pragma unroll 1
+                        for (int q = 0; q < 4; q++) {
+                            const int k0 = key0 + 32 * q;
+                            const int x0 = max(0, min(32, lo - k0)), x1 = max(0, min(32, hi - k0));
+                            uint32_t keep = x1 > x0 ? (x1 == 32 ? ~0u : (1u << x1) - 1) & ~(x0 == 32 ? ~0u : (1u << x0) - 1) : 0u;
+                            const uint32_t pq = pages >> (4 * q);
+                            keep &= ((pq & 1) ? 0xffu : 0u) | ((pq & 2) ? 0xff00u : 0u) | ((pq & 4) ? 0xff0000u : 0u) |
+                                    ((pq & 8) ? 0xff000000u : 0u);
+                            uint32_t u[32];
+                            tmem_ld32_async(ts + 32 * q, u);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 128; e++) u[e] ^= 0x80000000u;
+                            for (int e = 0; e < 32; e++) u[e] = ((keep >> e) & 1) ? u[e] ^ sign : 0xff800000u;
+                            tmem_st16_async(ts + 32 * q, u);
+                            tmem_st16_async(ts + 32 * q + 16, u + 16);
+                        }
+                        tmem_wait_st();
                     }
-                    if (!__all_sync(FULL, inner) || pages != FULL) {
+                    // the scores are read twice, 32 columns at a time: 128 of them do not fit beside the rest
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    {
+                        uint32_t u[2][32];
+                        tmem_ld32_async(ts, u[0]);
 #pragma unroll
-                        for (int e = 0; e < 128; e++) {
-                            const int key = key0 + e;
-                            if (!(key >= lo && key < hi && ((pages >> (e / 8)) & 1))) u[e] = 0xff800000u;
+                        for (int q = 0; q < 4; q++) {
+                            tmem_wait_ld();
+                            if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[(q + 1) & 1]);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(u[q & 1][e]));
                         }
                     }
-                    float mx[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) mx[e] = __uint_as_float(u[e]);
-#pragma unroll
-                    for (int e = 8; e < 128; e++) mx[e & 7] = fmaxf(mx[e & 7], __uint_as_float(u[e]));
-#pragma unroll
-                    for (int w = 4; w > 0; w >>= 1)
-#pragma unroll
-                        for (int e = 0; e < w; e++) mx[e] = fmaxf(mx[e], mx[e + w]);
+                    mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     const float top = mx[0] * sl;
                     float f = 1.f;
                     if (top > m + kRescale || (m == -INFINITY && top > -INFINITY)) {
@@ -390,21 +419,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // masked scores and rows that see nothing: 2^(-inf) = 0
                     const float base = m == -INFINITY ? 0.f : -m;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    {
+                        uint32_t u[2][32];
+                        tmem_ld32_async(ts, u[0]);
 #pragma unroll
-                    for (int e = 0; e < 128; e += 2) {
-                        const float x = ex2(fmaf(__uint_as_float(u[e]), sl, base));
-                        const float y = ex2(fmaf(__uint_as_float(u[e + 1]), sl, base));
-                        sum[(e / 2) & 3] += x + y;
-                        u[e / 2] = pack2(x, y, static_cast<T*>(nullptr));
+                        for (int q = 0; q < 4; q++) {
+                            tmem_wait_ld();
+                            if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[(q + 1) & 1]);
+                            uint32_t (&v)[32] = u[q & 1];
+                            uint32_t w[16];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const float x = ex2(fmaf(__uint_as_float(v[e]), sl, base));
+                                const float y = ex2(fmaf(__uint_as_float(v[e + 1]), sl, base));
+                                sum[(e / 2) & 3] += x + y;
+                                w[e / 2] = pack2(x, y, static_cast<T*>(nullptr));
+                            }
+                            tmem_st16_async(ts + 16 * q, w);  // over scores that have been read
+                        }
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e++) w[e] = u[16 * q + e];
-                        tmem_st16(ts + 16 * q, w);
-                    }
+                    tmem_wait_st();
                     if (key0 < c.t.lo || key0 > c.t.hi - kKB) {
                         // rows of V that no query attends to may hold anything: no 0 x NaN.  (Both streams
                         // write the same zeros; each before its own product.)
@@ -458,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float z = lt * 0.f;  // NaN once a value is not finite
                 const bool t0 = fold || act;
                 const uint32_t ta = fold ? tO + lane_off : to;
+                uint8_t* stage_out = sQ + i * S::STAGE;
 #pragma unroll 1
                 for (int q = q0; q < q1; q++) {
                     float o[32];
@@ -475,10 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e++) z = fmaf(o[e], 0.f, z);
-                    if (!in) continue;
-                    if (whole) {
-                        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
-                                                              (static_cast<size_t>(tok) * a.H + h) * HD + 32 * q);
+                    if (whole) {  // into this stream's Q tile, which every product has read
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             uint4 v;
@@ -486,9 +519,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 vw[k] = pack2(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv, static_cast<T*>(nullptr));
-                            dst[e] = v;
+                            *reinterpret_cast<uint4*>(stage_out + (q / 2) * S::PANEL + sw128(r, (4 * q + e) & 7)) = v;
                         }
-                    } else {  // [4-column group][row], so that a warp's stores are whole lines
+                    } else if (in) {  // [4-column group][row], so that a warp's stores are whole lines
                         float4* dst = reinterpret_cast<float4*>(part) + kRows;
 #pragma unroll
                         for (int e = 0; e < 8; e++)
@@ -499,6 +532,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // not finite: a value that this row must not see may have met it as 0 x infinity (see tl_paged_attn.cu)
                 const bool redo = in && z != z;
                 if (whole) {
+                    // whole lines of the rows of this warp, 16 bytes a lane
+                    __syncwarp();
+                    const int nch = 4 * (q1 - q0), sh = __ffs(nch) - 1;  // 16-byte pieces of a row: 4, 8 or 16
+                    const unsigned long long mine =
+                        in ? (static_cast<unsigned long long>(tok) * a.H + h) * HD + 32 * q0 : ~0ull;
+                    for (int k = lane; k < 32 * nch; k += 32) {
+                        const int rr = k >> sh, d = 4 * q0 + (k & (nch - 1));
+                        const unsigned long long at = __shfl_sync(FULL, mine, rr);
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage_out + (d / 8) * S::PANEL +
+                                                                        sw128((warp & 3) * 32 + rr, d & 7));
+                        if (at != ~0ull) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + 8 * (k & (nch - 1))) = v;
+                    }
+                    __syncwarp();
                     for (unsigned bad = __ballot_sync(FULL, redo); bad; bad &= bad - 1) {
                         const int src = __ffs(bad) - 1;
                         __syncwarp();
@@ -544,15 +590,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the parts of the tile that block blockIdx.x began (part i > 0: the first tile of block blockIdx.x + i).
 // Block y takes 32 rows: lane = row, warp = one 8th of the columns.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_attend_chunk_join(AttendArgs a, const Head* heads, const float* parts) {
+__global__ void __launch_bounds__(256) k_attend_chunk_join(const __grid_constant__ AttendArgs a, const Head* heads, const float* parts) {
     pdl_wait();
     const Head h = heads[blockIdx.x];
     if (h.parts == 0) return;
-    const Tile t = tile_of(a, h.b, h.rt, kRows);
-    if (static_cast<int>(blockIdx.y) * 32 >= t.nrows) return;
+    Cursor c;
+    c.g = h.g;
+    c.t = tile_of(a, h.b, h.rt, kRows);
+    if (static_cast<int>(blockIdx.y) * 32 >= c.t.nrows) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.y * 32 + lane;
-    const bool in = row < t.nrows;
+    const bool in = row < c.t.nrows;
     constexpr size_t rec = static_cast<size_t>(kRows) * (HD / 4 + 1);  // float4s of a part
     constexpr int G = HD / 4 / 8;                                      // 4-column groups of a warp
     const float4* p0 = reinterpret_cast<const float4*>(parts) + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
@@ -584,7 +632,8 @@ __global__ void __launch_bounds__(256) k_attend_chunk_join(AttendArgs a, const H
                 acc[g].w += v.w * f;
             }
         }
-    const int fr = t.r0 + (in ? row : 0), tok = t.first + fr / a.group, hh = h.g * a.group + fr % a.group;
+    int tok, hh;
+    row_of(a, c, row, tok, hh);
     const unsigned again = __ballot_sync(FULL, in && bad > 0.f);
     if (in && !(bad > 0.f)) {
         const float inv = L != 0.f ? 1.f / L : 0.f;
