@@ -39,16 +39,19 @@ using namespace tc;
 constexpr int kRows = 256, kHalf = 128, kKB = 128;
 constexpr int kWarps = 10, kThreads = kWarps * 32;
 constexpr float kRescale = 8.f;  // log2 units
+constexpr int kPoly = 3, kPolyOf = 8;  // pairs of weights, of so many, on the FMA pipe
 
-// One step: 256 rows x 128 keys, or (tiles of at most 128 rows) 128 rows x 256 keys.
+// One step: 256 rows x 128 keys, or (tiles of at most 128 rows) 128 rows x 256 keys.  Beginning and ending a
+// tile takes about as long as kTileCost steps, which count as steps before its first key tile.
 struct ChunkPlan {
     static constexpr int R = kRows;
+    static constexpr int kTileCost = 2;
     static __device__ __forceinline__ int key_tiles(const Tile& t) {
         return t.hi <= t.lo ? 1 : (t.hi - 1) / kKB - t.lo / kKB + 1;
     }
     static __device__ __forceinline__ int steps(const Tile& t) {
         const int n = key_tiles(t);
-        return t.nrows > kHalf ? n : (n + 1) / 2;
+        return kTileCost + (t.nrows > kHalf ? n : (n + 1) / 2);
     }
 };
 
@@ -81,6 +84,40 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_n_major) {
     const uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
     return (1u << 4) | (f << 7) | (f << 10) | ((b_n_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
            (static_cast<uint32_t>(128 >> 4) << 24);
+}
+
+__device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+    return bar_spin_ab(b, parity, abort_flag);
+}
+
+// The larger of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x of a pair on the FMA pipe: x = n + f with n whole and |f| <= 1/2, 2^f by a polynomial of degree 4
+// (constant term 1, relative error 2.8e-6, fitted to 2^f on [-1/2, 1/2]), n added to its exponent.
+// x below -127 gives 0 or less than 2^-126; NaN gives a value that no product with it leaves finite.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the low bits become n
+    const float2 minus = make_float2(-12582912.f, -12582912.f), neg = make_float2(-1.f, -1.f);
+    x.x = max_nan(x.x, -127.f);
+    x.y = max_nan(x.y, -127.f);
+    const float2 t = fadd2(x, magic);
+    const float2 f = ffma2(fadd2(t, minus), neg, x);
+    float2 p = make_float2(0.009582852944731712f, 0.009582852944731712f);
+    p = ffma2(p, f, make_float2(0.055906426161527634f, 0.055906426161527634f));
+    p = ffma2(p, f, make_float2(0.24024099111557007f, 0.24024099111557007f));
+    p = ffma2(p, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
+    p = ffma2(p, f, make_float2(1.f, 1.f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 __device__ __forceinline__ void tma_panel(void* dst, const CUtensorMap* map, int row, int panel, int page, uint64_t* bar) {
@@ -128,10 +165,7 @@ struct Part {
     int jb, je, kb0;  // key tile j covers positions (kb0 + j) * 128 ..
     bool two;         // two streams of rows (else the streams take key tiles in turn)
     int end0;         // two: stream 0's last key tile + 1 (its tokens end earlier)
-    __device__ __forceinline__ bool active(int i) const {
-        if (two) return i == 1 || end0 > jb;
-        return i == 0 || je > jb + 1;
-    }
+    __device__ __forceinline__ bool active(int i) const { return begin(i) < end(i); }
     __device__ __forceinline__ int begin(int i) const { return two ? jb : jb + i; }
     __device__ __forceinline__ int end(int i) const { return two && i == 0 ? end0 : je; }
     __device__ __forceinline__ int stride() const { return two ? 1 : 2; }
@@ -140,8 +174,9 @@ __device__ __forceinline__ Part part_of(const AttendArgs& a, const Cursor& c) {
     Part p;
     const int n = ChunkPlan::key_tiles(c.t);
     p.two = c.t.nrows > kHalf;
-    p.jb = p.two ? c.s : 2 * c.s;
-    p.je = min(n, p.two ? c.end : 2 * c.end);
+    const int s = max(0, c.s - ChunkPlan::kTileCost), e = max(0, c.end - ChunkPlan::kTileCost);
+    p.jb = p.two ? s : 2 * s;
+    p.je = min(n, p.two ? e : 2 * e);
     p.kb0 = c.t.lo / kKB;
     p.end0 = p.je;
     if (p.two) {
@@ -165,12 +200,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + NST * S::STAGE);
     uint64_t* empty = full + NST;
     uint64_t* s_full = empty + NST;  // [2] S_i written (and every MMA before it done)
-    uint64_t* p_full = s_full + 2;   // [2] P_i written: 4 warps
-    uint64_t* q_full = p_full + 2;   // [2] Q_i written: 4 warps
+    uint64_t* p_full = s_full + 2;   // [2][2] halves of P_i (64 keys) written: 4 warps
+    uint64_t* q_full = p_full + 4;   // [2] Q_i written: 4 warps
     uint64_t* o_full = q_full + 2;   // [2] the stream's last product done
     uint64_t* xbar = o_full + 2;     // both streams' 8 warps
     uint64_t* drain = xbar + 1;
-    static_assert((2 * 10 + 10) * 8 <= 256, "barriers");
+    static_assert((2 * 10 + 12) * 8 <= 256, "barriers");
     float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);  // [2][128] max, [2][128] sum
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xch + 4 * kHalf);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -179,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) heads[blockIdx.x].parts = 0;
     Cursor c;
-    const int per = find_share<ChunkPlan, kWarps>(a, c, ws, 2);
+    const int per = find_share<ChunkPlan, kWarps>(a, c, ws, ChunkPlan::kTileCost + 1);
     if (per == 0) return;
 
     if (threadIdx.x == 0) {
@@ -189,7 +224,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; i++) {
             bar_init(&s_full[i], 1);
-            bar_init(&p_full[i], 4);
+            bar_init(&p_full[2 * i], 4);
+            bar_init(&p_full[2 * i + 1], 4);
             bar_init(&q_full[i], 4);
             bar_init(&o_full[i], 1);
         }
@@ -210,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tS = tmem, tO = tmem + 256;  // S_i at + 128 i, O_i at + 128 i
 
     auto fail = [&] { *abort_flag = 1; };
-    auto wait = [&](uint64_t* b, uint32_t parity) { return bar_spin_ab(b, parity, abort_flag); };
+    // waits poll: the hand-offs here are short and frequent
+    auto wait = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || wait_slow(b, parity, abort_flag); };
 
     if (warp == 8) {
         // ---- TMA: K_j, V_j of each key tile; lane = one page's rows of one panel ----
@@ -273,15 +310,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return true;
                 };
                 auto values = [&](int i, int j) -> bool {  // O_i (+)= P_i V_j
-                    if (!wait(&p_full[i], (np >> i) & 1)) return false;
-                    np ^= 1u << i;
                     const uint32_t n = n0 + 2 * (j - p.jb) + 1, st = n % NST;
                     if (!wait(&full[st], (n / NST) & 1)) return false;
-                    tc_fence_after();
                     const uint64_t db = sdesc_n128(su32(ring + st * S::STAGE), S::PANEL);
 #pragma unroll
-                    for (int k = 0; k < kKB / 16; k++)
-                        umma_f16_ts(tO + 128 * i, tS + 128 * i + 8 * k, db + 128 * k, id_o, j != p.begin(i) || k != 0);
+                    for (int hf = 0; hf < 2; hf++) {
+                        if (!wait(&p_full[2 * i + hf], (np >> i) & 1)) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 4 * hf; k < 4 * hf + 4; k++)
+                            umma_f16_ts(tO + 128 * i, tS + 128 * i + 8 * k, db + 128 * k, id_o, j != p.begin(i) || k != 0);
+                    }
+                    np ^= 1u << i;
                     if (!p.two || i == 1) umma_commit(&empty[st]);
                     return true;
                 };
@@ -319,8 +359,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float scale = a.scale * 1.4426950408889634f;  // log2 units
         const float sl = fabsf(scale);
         uint32_t n0 = 0, ns = 0, no = 0, nx = 0;
-        bool ok = true, first_tile = true;
-        for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c), first_tile = false) {
+        bool ok = true, first_tile = true, go = true;
+        // a tile's Q rows are fetched before the epilogue of the tile before: 16 bytes a lane, whole rows
+        constexpr int CH = HD / 8, RPI = 32 / CH, QL = 32 / RPI;  // pieces of a row, rows a load, loads
+        uint4 qv[QL];
+        auto fetch_q = [&](const Cursor& t) {
+            const bool two = t.t.nrows > kHalf;
+            const int rw = two ? i * kHalf + r : r;
+            int tk, hh;
+            row_of(a, t, rw, tk, hh);
+            const unsigned long long mine = rw < t.t.nrows ? static_cast<unsigned long long>(tk) * a.q_stride +
+                                                                 static_cast<unsigned long long>(hh) * HD : ~0ull;
+#pragma unroll
+            for (int q = 0; q < QL; q++) {
+                const unsigned long long at = __shfl_sync(FULL, mine, q * RPI + lane / CH);
+                qv[q] = at != ~0ull ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at)[lane % CH]
+                                    : make_uint4(0, 0, 0, 0);
+            }
+        };
+        fetch_q(c);
+#pragma unroll 1
+        while (ok && go) {
             const Part p = part_of(a, c);
             const int row = p.two ? i * kHalf + r : r;  // of the tile
             const bool in = row < c.t.nrows;
@@ -331,22 +390,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             attended(a, c.t.p0 + (tok - c.t.first), lo, hi);
             float m = -INFINITY, l = 0.f;
             if (act) {
-                {  // this warp's 32 Q rows into the swizzled K-major panels, row by row
-                    const unsigned long long mine =
-                        in ? static_cast<unsigned long long>(tok) * a.q_stride + static_cast<unsigned long long>(h) * HD : ~0ull;
-                    constexpr int CH = HD / 8, RPI = 32 / CH;  // 16-byte pieces of a row, rows a load
-#pragma unroll 8
-                    for (int q = 0; q < 32 / RPI; q++) {
-                        const int rr = q * RPI + lane / CH, d = lane % CH;
-                        const unsigned long long at = __shfl_sync(FULL, mine, rr);
-                        const uint4 v = at != ~0ull ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at)[d]
-                                                    : make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(sQ + i * S::STAGE + (d / 8) * S::PANEL + sw128((warp & 3) * 32 + rr, d & 7)) = v;
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&q_full[i]);
+                // this warp's 32 Q rows into the swizzled K-major panels
+#pragma unroll
+                for (int q = 0; q < QL; q++) {
+                    const int rr = q * RPI + lane / CH, d = lane % CH;
+                    *reinterpret_cast<uint4*>(sQ + i * S::STAGE + (d / 8) * S::PANEL + sw128((warp & 3) * 32 + rr, d & 7)) = qv[q];
                 }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&q_full[i]);
                 auto page_at = [&](int j) { return lane < kKB / 8 ? page_of(a, c.b, (p.kb0 + j) * kKB + 8 * lane) : 0; };
                 int pid_next = page_at(p.begin(i));
                 const int stride = p.stride();
@@ -386,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_wait_st();
                     }
                     // the scores are read twice, 32 columns at a time: 128 of them do not fit beside the rest
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float mx[2] = {-INFINITY, -INFINITY};
                     {
                         uint32_t u[2][32];
                         tmem_ld32_async(ts, u[0]);
@@ -395,11 +447,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tmem_wait_ld();
                             if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[(q + 1) & 1]);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(u[q & 1][e]));
+                            for (int e = 0; e < 32; e += 2)
+                                mx[(e / 2) & 1] = max3(mx[(e / 2) & 1], __uint_as_float(u[q & 1][e]), __uint_as_float(u[q & 1][e + 1]));
                         }
                     }
-                    mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    const float top = mx[0] * sl;
+                    const float top = fmaxf(mx[0], mx[1]) * sl;
                     float f = 1.f;
                     if (top > m + kRescale || (m == -INFINITY && top > -INFINITY)) {
                         if (m != -INFINITY) f = ex2(m - top);
@@ -418,28 +470,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     // masked scores and rows that see nothing: 2^(-inf) = 0
                     const float base = m == -INFINITY ? 0.f : -m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    {
-                        uint32_t u[2][32];
-                        tmem_ld32_async(ts, u[0]);
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            tmem_wait_ld();
-                            if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[(q + 1) & 1]);
-                            uint32_t (&v)[32] = u[q & 1];
-                            uint32_t w[16];
-#pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                const float x = ex2(fmaf(__uint_as_float(v[e]), sl, base));
-                                const float y = ex2(fmaf(__uint_as_float(v[e + 1]), sl, base));
-                                sum[(e / 2) & 3] += x + y;
-                                w[e / 2] = pack2(x, y, static_cast<T*>(nullptr));
-                            }
-                            tmem_st16_async(ts + 16 * q, w);  // over scores that have been read
-                        }
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_wait_st();
                     if (key0 < c.t.lo || key0 > c.t.hi - kKB) {
                         // rows of V that no query attends to may hold anything: no 0 x NaN.  (Both streams
                         // write the same zeros; each before its own product.)
@@ -457,10 +487,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         fence_proxy_async();
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&p_full[i]);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    {
+                        const float2 sl2 = make_float2(sl, sl), base2 = make_float2(base, base);
+                        uint32_t u[2][32];
+                        tmem_ld32_async(ts, u[0]);
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            tmem_wait_ld();
+                            if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[(q + 1) & 1]);
+                            const uint32_t (&v)[32] = u[q & 1];
+                            uint32_t w[16];
+#pragma unroll
+                            for (int e = 0; e < 16; e++) {
+                                float2 x = ffma2(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sl2, base2);
+                                // the special function unit takes 8 cycles for what the FMA pipe starts in 1: some
+                                // of the pairs go there
+                                if (e % kPolyOf < kPoly) x = ex2_poly(x);
+                                else x = make_float2(ex2(x.x), ex2(x.y));
+                                sum[e & 1] = fadd2(sum[e & 1], x);
+                                w[e] = pack2(x.x, x.y, static_cast<T*>(nullptr));
+                            }
+                            tmem_st16_async(ts + 16 * q, w);  // over scores that have been read
+                            if (q & 1) {  // half of the weights: the products of their keys may begin
+                                tmem_wait_st();
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) bar_arrive(&p_full[2 * i + q / 2]);
+                            }
+                        }
+                    }
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 }
+            }
+            Cursor nc = c;
+            go = next_tile<ChunkPlan>(a, nc);
+            if (go) fetch_q(nc);
+            if (act) {
                 if (ok && !__all_sync(FULL, wait(&o_full[i], no & 1))) ok = false;
                 no++;
                 tc_fence_after();
@@ -534,16 +597,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (whole) {
                     // whole lines of the rows of this warp, 16 bytes a lane
                     __syncwarp();
-                    const int nch = 4 * (q1 - q0), sh = __ffs(nch) - 1;  // 16-byte pieces of a row: 4, 8 or 16
                     const unsigned long long mine =
                         in ? (static_cast<unsigned long long>(tok) * a.H + h) * HD + 32 * q0 : ~0ull;
-                    for (int k = lane; k < 32 * nch; k += 32) {
-                        const int rr = k >> sh, d = 4 * q0 + (k & (nch - 1));
-                        const unsigned long long at = __shfl_sync(FULL, mine, rr);
-                        const uint4 v = *reinterpret_cast<const uint4*>(stage_out + (d / 8) * S::PANEL +
-                                                                        sw128((warp & 3) * 32 + rr, d & 7));
-                        if (at != ~0ull) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + 8 * (k & (nch - 1))) = v;
-                    }
+                    auto copy_out = [&](auto pieces) {
+                        constexpr int nch = decltype(pieces)::value;  // 16-byte pieces of a row
+#pragma unroll 4
+                        for (int k = 0; k < nch; k++) {
+                            const int rr = (32 / nch) * k + lane / nch, d = 4 * q0 + lane % nch;
+                            const unsigned long long at = __shfl_sync(FULL, mine, rr);
+                            const uint4 v = *reinterpret_cast<const uint4*>(stage_out + (d / 8) * S::PANEL +
+                                                                            sw128((warp & 3) * 32 + rr, d & 7));
+                            if (at != ~0ull) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + 8 * (lane % nch)) = v;
+                        }
+                    };
+                    if (fold) copy_out(std::integral_constant<int, HD / 16>());
+                    else copy_out(std::integral_constant<int, HD / 8>());
                     __syncwarp();
                     for (unsigned bad = __ballot_sync(FULL, redo); bad; bad &= bad - 1) {
                         const int src = __ffs(bad) - 1;
@@ -576,6 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!__all_sync(FULL, wait(xbar, nx & 1))) ok = false;
                 nx++;
             }
+            c = nc;
+            first_tile = false;
         }
         if (!ok) fail();
     }
