@@ -86,6 +86,12 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_n_major) {
            (static_cast<uint32_t>(128 >> 4) << 24);
 }
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t y;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(y));
+    return y != 0;
+}
 __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
     return bar_spin_ab(b, parity, abort_flag);
 }
@@ -211,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     long long* ws = reinterpret_cast<long long*>(ring);  // the scan runs before the ring is used
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (uniform for the compiler)
     if (threadIdx.x == 0) heads[blockIdx.x].parts = 0;
     Cursor c;
     const int per = find_share<ChunkPlan, kWarps>(a, c, ws, ChunkPlan::kTileCost + 1);
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(FULL, *tmem_slot, 0);
     const uint32_t tS = tmem, tO = tmem + 256;  // S_i at + 128 i, O_i at + 128 i
 
     auto fail = [&] { *abort_flag = 1; };
@@ -286,71 +292,74 @@ __global__ void __launch_bounds__(kThreads, 1)
         // every copy issued lands before the block ends
         for (uint32_t k = n > NST ? n - NST : 0; k < n; k++) bar_wait(&full[k % NST], (k / NST) & 1);
     } else if (warp == 9) {
-        if (lane == 0) {
-            // ---- MMA ----
-            constexpr uint32_t id_s = idesc<T>(kKB, false), id_o = idesc<T>(HD, true);
-            uint32_t n0 = 0;              // loads before this tile
-            uint32_t nq = 0, np = 0;      // phases of the streams' barriers
-            bool ok = true;
-            for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
-                const Part p = part_of(a, c);
-                auto scores = [&](int i, int j) -> bool {  // S_i = Q_i K_j^T
-                    const uint32_t n = n0 + 2 * (j - p.jb), st = n % NST;
-                    if (!wait(&full[st], (n / NST) & 1)) return false;
-                    tc_fence_after();
-#pragma unroll
-                    for (int d = 0; d < S::PANELS; d++) {
-                        const uint64_t da = sdesc_k128(su32(sQ + i * S::STAGE + d * S::PANEL));
-                        const uint64_t db = sdesc_k128(su32(ring + st * S::STAGE + d * S::PANEL));
-#pragma unroll
-                        for (int k = 0; k < 4; k++) umma_f16(tS + 128 * i, da + 2 * k, db + 2 * k, id_s, (d | k) != 0);
-                    }
-                    umma_commit(&s_full[i]);
-                    if (!p.two || i == 1) umma_commit(&empty[st]);  // K_j is read (stream 1 is its last reader)
-                    return true;
-                };
-                auto values = [&](int i, int j) -> bool {  // O_i (+)= P_i V_j
-                    const uint32_t n = n0 + 2 * (j - p.jb) + 1, st = n % NST;
-                    if (!wait(&full[st], (n / NST) & 1)) return false;
-                    const uint64_t db = sdesc_n128(su32(ring + st * S::STAGE), S::PANEL);
-#pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        if (!wait(&p_full[2 * i + hf], (np >> i) & 1)) return false;
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = 4 * hf; k < 4 * hf + 4; k++)
-                            umma_f16_ts(tO + 128 * i, tS + 128 * i + 8 * k, db + 128 * k, id_o, j != p.begin(i) || k != 0);
-                    }
-                    np ^= 1u << i;
-                    if (!p.two || i == 1) umma_commit(&empty[st]);
-                    return true;
-                };
-                const int stride = p.stride();
-                // begin: the first scores of both streams; then values and next scores, in turn
+        // ---- MMA: the whole warp keeps step, so that addresses and descriptors stay in uniform registers;
+        // one elected lane issues ----
+        constexpr uint32_t id_s = idesc<T>(kKB, false), id_o = idesc<T>(HD, true);
+        const uint64_t dq = sdesc_k128(su32(sQ)), dk = sdesc_k128(su32(ring)), dv = sdesc_n128(su32(ring), S::PANEL);
+        constexpr uint32_t STEP = S::STAGE >> 4, PSTEP = S::PANEL >> 4;
+        uint32_t n0 = 0;              // loads before this tile
+        uint32_t nq = 0, np = 0;      // phases of the streams' barriers
+        auto wait_all = [&](uint64_t* b, uint32_t parity) { return __all_sync(FULL, wait(b, parity)); };
+        bool ok = true;
 #pragma unroll 1
-                for (int j = p.jb - stride; ok && j < p.je; j += stride)
+        for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
+            const Part p = part_of(a, c);
+            const int stride = p.stride();
+            // begin: the first scores of both streams; then values and next scores, in turn
 #pragma unroll 1
-                    for (int i = 0; i < 2; i++) {
-                        const int ji = p.two ? j : j + i;
-                        const bool start = j < p.jb;
-                        if (!ok || !p.active(i) || ji >= p.end(i)) continue;
-                        if (start) {
-                            ok = wait(&q_full[i], (nq >> i) & 1);
-                            nq ^= 1u << i;
+            for (int j = p.jb - stride; ok && j < p.je; j += stride)
+#pragma unroll 1
+                for (int i = 0; i < 2; i++) {
+                    const int ji = p.two ? j : j + i;
+                    const bool start = j < p.jb;
+                    if (!p.active(i) || ji >= p.end(i)) continue;
+                    if (start) {
+                        if (!(ok = wait_all(&q_full[i], (nq >> i) & 1))) break;
+                        nq ^= 1u << i;
+                    } else {  // O_i (+)= P_i V_j
+                        const uint32_t n = n0 + 2 * (ji - p.jb) + 1, st = n % NST;
+                        if (!(ok = wait_all(&full[st], (n / NST) & 1))) break;
+                        const uint64_t db = dv + st * STEP;
+                        const uint32_t first = ji != p.begin(i);
+#pragma unroll
+                        for (int hf = 0; hf < 2; hf++) {
+                            if (!(ok = wait_all(&p_full[2 * i + hf], (np >> i) & 1))) break;
                             tc_fence_after();
-                        } else {
-                            ok = values(i, ji);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 4 * hf; k < 4 * hf + 4; k++)
+                                    umma_f16_ts(tO + 128 * i, tS + 128 * i + 8 * k, db + 128 * k, id_o, k == 0 ? first : 1u);
+                                if (hf && (!p.two || i == 1)) umma_commit(&empty[st]);  // V_j is read
+                            }
                         }
-                        const int jn = start ? p.begin(i) : ji + stride;
-                        if (ok && jn < p.end(i)) ok = scores(i, jn);
-                        else if (ok) umma_commit(&o_full[i]);
+                        if (!ok) break;
+                        np ^= 1u << i;
                     }
-                n0 += 2 * (p.je - p.jb);
-            }
-            if (!ok) fail();
-            umma_commit(drain);  // completes once every MMA issued above has
-            bar_wait(drain, 0);
+                    const int jn = start ? p.begin(i) : ji + stride;
+                    if (jn < p.end(i)) {  // S_i = Q_i K_j^T
+                        const uint32_t n = n0 + 2 * (jn - p.jb), st = n % NST;
+                        if (!(ok = wait_all(&full[st], (n / NST) & 1))) break;
+                        tc_fence_after();
+                        const uint64_t da = dq + i * STEP, db = dk + st * STEP;
+                        if (elect_one()) {
+#pragma unroll
+                            for (int d = 0; d < S::PANELS; d++)
+#pragma unroll
+                                for (int k = 0; k < 4; k++)
+                                    umma_f16(tS + 128 * i, da + d * PSTEP + 2 * k, db + d * PSTEP + 2 * k, id_s, (d | k) != 0);
+                            umma_commit(&s_full[i]);
+                            if (!p.two || i == 1) umma_commit(&empty[st]);  // K_j is read (stream 1 is its last reader)
+                        }
+                    } else if (elect_one()) {
+                        umma_commit(&o_full[i]);
+                    }
+                }
+            n0 += 2 * (p.je - p.jb);
         }
+        if (!ok) fail();
+        __syncwarp();
+        if (elect_one()) umma_commit(drain);  // completes once every MMA issued above has
+        bar_wait(drain, 0);
     } else {
         // ---- softmax and epilogue: thread = row r of stream i ----
         const int i = warp >> 2, r = (warp & 3) * 32 + lane;
