@@ -39,7 +39,6 @@ using namespace tc;
 constexpr int kRows = 256, kHalf = 128, kKB = 128;
 constexpr int kWarps = 10, kThreads = kWarps * 32;
 constexpr float kRescale = 8.f;  // log2 units
-constexpr int kPoly = 3, kPolyOf = 8;  // pairs of weights, of so many, on the FMA pipe
 
 // One step: 256 rows x 128 keys, or (tiles of at most 128 rows) 128 rows x 256 keys.  Beginning and ending a
 // tile takes about as long as kTileCost steps, which count as steps before its first key tile.
@@ -102,30 +101,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-// 2^x of a pair on the FMA pipe: x = n + f with n whole and |f| <= 1/2, 2^f by a polynomial of degree 4
-// (constant term 1, relative error 2.8e-6, fitted to 2^f on [-1/2, 1/2]), n added to its exponent.
-// x below -127 gives 0 or less than 2^-126; NaN gives a value that no product with it leaves finite.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-    const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the low bits become n
-    const float2 minus = make_float2(-12582912.f, -12582912.f), neg = make_float2(-1.f, -1.f);
-    x.x = max_nan(x.x, -127.f);
-    x.y = max_nan(x.y, -127.f);
-    const float2 t = fadd2(x, magic);
-    const float2 f = ffma2(fadd2(t, minus), neg, x);
-    float2 p = make_float2(0.009582852944731712f, 0.009582852944731712f);
-    p = ffma2(p, f, make_float2(0.055906426161527634f, 0.055906426161527634f));
-    p = ffma2(p, f, make_float2(0.24024099111557007f, 0.24024099111557007f));
-    p = ffma2(p, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
-    p = ffma2(p, f, make_float2(1.f, 1.f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-
 __device__ __forceinline__ void tma_panel(void* dst, const CUtensorMap* map, int row, int panel, int page, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
@@ -496,9 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         fence_proxy_async();
                     }
-                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    float sum[2] = {0.f, 0.f};
                     {
-                        const float2 sl2 = make_float2(sl, sl), base2 = make_float2(base, base);
                         uint32_t u[2][32];
                         tmem_ld32_async(ts, u[0]);
 #pragma unroll
@@ -509,13 +483,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             uint32_t w[16];
 #pragma unroll
                             for (int e = 0; e < 16; e++) {
-                                float2 x = ffma2(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sl2, base2);
-                                // the special function unit takes 8 cycles for what the FMA pipe starts in 1: some
-                                // of the pairs go there
-                                if (e % kPolyOf < kPoly) x = ex2_poly(x);
-                                else x = make_float2(ex2(x.x), ex2(x.y));
-                                sum[e & 1] = fadd2(sum[e & 1], x);
-                                w[e] = pack2(x.x, x.y, static_cast<T*>(nullptr));
+                                const float x = ex2(fmaf(__uint_as_float(v[2 * e]), sl, base));
+                                const float y = ex2(fmaf(__uint_as_float(v[2 * e + 1]), sl, base));
+                                sum[0] += x;
+                                sum[1] += y;
+                                w[e] = pack2(x, y, static_cast<T*>(nullptr));
                             }
                             tmem_st16_async(ts + 16 * q, w);  // over scores that have been read
                             if (q & 1) {  // half of the weights: the products of their keys may begin
@@ -526,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
-                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    l += sum[0] + sum[1];
                 }
             }
             Cursor nc = c;
