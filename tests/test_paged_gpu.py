@@ -413,6 +413,23 @@ def test_sample_rows_that_cannot_be_sampled(T):
     run_sample(x, r, np.full(8, T))
 
 
+@pytest.mark.parametrize("n", [4093, 4096, 45000, 128001, 270000])
+@pytest.mark.parametrize("off", [0, 1, 3])
+def test_sample_sizes_and_alignments(n, off):
+    """Rows around a segment's size, rows that do not fit shared memory, rows longer than the cells; rows
+    that begin off 16 bytes.  Peaked and flat rows, with few and many logits kept."""
+    rng = np.random.default_rng(n + off)
+    x = torch.as_tensor((rng.standard_normal((4, n + 5)) * np.array([[0.3], [1.0], [3.0], [8.0]])).astype(np.float32)).cuda()
+    v = x[:, off:off + n]
+    xs = v.cpu().numpy()
+    for k, p, m in ((None, None, None), (40, 0.9, 0.02), (3000, 0.97, None), (None, 0.5, None), (None, 0.999, 1e-5)):
+        r, T = rng.random(4).astype(np.float32), rng.uniform(0.5, 1.2, 4).astype(np.float32)
+        full = lambda a, f: None if a is None else f([a] * 4)
+        got = ops().sample_rows(v, f32(r), f32(T), full(k, i32), full(p, f32), full(m, f32)).cpu().numpy()
+        want = [plain.sample(xs[i], r[i], T[i], k, p, m) for i in range(4)]
+        np.testing.assert_array_equal(got, want)
+
+
 def test_sample_strided_rows():
     rng = np.random.default_rng(8)
     x = torch.as_tensor(rng.standard_normal((6, 1111)).astype(np.float32)).cuda()

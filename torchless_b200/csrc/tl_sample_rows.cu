@@ -21,7 +21,7 @@ struct SampleRowsArgs {
     int n;
     const float *r, *temperature, *top_p, *min_p;
     const int32_t* top_k;
-    int fits;  // the row fits shared memory
+    int segs;  // segments of kSeg logits
 };
 
 // Order-preserving key of a logit: larger logit, larger key; -0 and +0 the same.
@@ -33,9 +33,46 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
-// The weight of a logit as a multiple of 2^-40.
-__device__ __forceinline__ unsigned long long weight_of(float x, float top, double inv_t) {
-    return __double2ull_rn(exp((static_cast<double>(x) - static_cast<double>(top)) * inv_t) * kOne);
+// 32-bit to 64-bit floating point by integer operations (the conversion instruction runs at a quarter of the rate of
+// the 64-bit arithmetic).  Zero and subnormals become about 2^-127, infinity about 2^128: no weight changes by 2^-40.
+__device__ __forceinline__ double widen(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return __hiloint2double(static_cast<int>((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + (896u << 20))), static_cast<int>(u << 29));
+}
+
+__constant__ double kPow2[32] = {  // 2^(j / 32)
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484,
+    1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407,
+    1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
+    1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474,
+    1.9571441241754002};
+
+// A row's scale: weights are 2^((x - top) * c / 32), c = 32 log2(e) / temperature.
+struct Scale {
+    double top, c;
+    const double* pow2;  // kPow2 in shared memory
+};
+
+// The weight of a logit as a multiple of 2^-40.  2^(t / 32) = 2^(k >> 5) 2^((k & 31) / 32) 2^(f / 32) with t = k + f,
+// |f| <= 1/2; the last factor by its series to the 5th power of f ln2 / 32 (what is left out is below 2^-48), all in
+// 64 bits, then rounded to a multiple of 2^-40 by adding 2^52.
+__device__ __forceinline__ unsigned long long weight_of(float x, const Scale& s) {
+    const double t = fmax((widen(x) - s.top) * s.c, -1400.0);  // 2^(-1400 / 32) rounds to 0
+    const double magic = 6755399441055744.0;                   // 1.5 * 2^52: k in the low bits
+    const double r = t + magic;
+    const int k = __double2loint(r);
+    const double f = t - (r - magic);
+    double q = 3.9737099845494154e-11;
+    q = fma(q, f, 9.172562701824643e-09);
+    q = fma(q, f, 1.6938509724371819e-06);
+    q = fma(q, f, 0.00023459619820224677);
+    q = fma(q, f, 0.02166084939249829);
+    q = fma(q, f, 1.0);
+    q *= s.pow2[k & 31];
+    const double v = __hiloint2double(__double2hiint(q) + (((k >> 5) + 40) << 20), __double2loint(q));
+    return static_cast<unsigned long long>(__double_as_longlong(v + 4503599627370496.0)) & 0xfffffffffffffull;
 }
 
 __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long* red) {
@@ -60,8 +97,8 @@ struct Scratch {
 // ways below give up on come here (thousands of equal logits at a cut, cuts far down a row).  The kept set is a
 // threshold: every logit whose key is above `key`, and of those equal to it the first `ties` by index.
 template <typename T>
-__device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float p, float mp, float r, double inv_t, float top,
-                                                 uint32_t bk, Scratch& sc) {
+__device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float p, float mp, float r, const Scale& ws, uint32_t bk,
+                                                 Scratch& sc) {
     unsigned long long *red = sc.red, *bins = sc.bins;
     uint32_t *sk = sc.sk, *si = sc.si, *s_sel = sc.sel;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -71,9 +108,11 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
     // top-k: the k-th largest key, 8 bits at a time
     if (k > 0 && k < n) {
         uint32_t prefix = 0, left = static_cast<uint32_t>(k);
+#pragma unroll 1
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (tid < 256) bins[tid] = 0;
             __syncthreads();
+#pragma unroll 1
             for (int i = tid; i < n; i += kThreads) {
                 const uint32_t u = key_of(to_f32<T>(x[i]));
                 if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8)))
@@ -101,27 +140,30 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
     // top-p: the same by sums of weights over what top-k keeps
     if (p < 1.f) {
         unsigned long long sum = 0;
+#pragma unroll 1
         for (int i = tid; i < n; i += kThreads) {
             const float v = to_f32<T>(x[i]);
-            if (key_of(v) > kkey) sum += weight_of(v, top, inv_t);
+            if (key_of(v) > kkey) sum += weight_of(v, ws);
         }
         sum = block_sum_u64(sum, red);
-        if (kties != ~0ull) sum += kties * weight_of(logit_of(kkey), top, inv_t);
+        if (kties != ~0ull) sum += kties * weight_of(logit_of(kkey), ws);
         const double want = static_cast<double>(p) * static_cast<double>(sum);  // stop at the first prefix that reaches it
         uint32_t prefix = 0;
         unsigned long long above = 0;  // weight of the keys above the prefix's range
+#pragma unroll 1
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (tid < 256) bins[tid] = 0;
             __syncthreads();
+#pragma unroll 1
             for (int i = tid; i < n; i += kThreads) {
                 const float v = to_f32<T>(x[i]);
                 const uint32_t u = key_of(v);
                 if (u > kkey && (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))))
-                    atomicAdd(&bins[(u >> shift) & 255], weight_of(v, top, inv_t));
+                    atomicAdd(&bins[(u >> shift) & 255], weight_of(v, ws));
             }
             __syncthreads();
             if (tid == 0 && kties != ~0ull && (shift == 24 || (kkey >> (shift + 8)) == (prefix >> (shift + 8))))
-                bins[(kkey >> shift) & 255] += kties * weight_of(logit_of(kkey), top, inv_t);
+                bins[(kkey >> shift) & 255] += kties * weight_of(logit_of(kkey), ws);
             __syncthreads();
             if (tid == 0) {
                 unsigned long long at = above;
@@ -138,7 +180,7 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
             above = sc.above;
             __syncthreads();
         }
-        const unsigned long long w = weight_of(logit_of(prefix), top, inv_t);
+        const unsigned long long w = weight_of(logit_of(prefix), ws);
         // ties of equal weight: as many as the sum still lacks, at least one
         unsigned long long m = 1;
         if (w > 0 && static_cast<double>(above) < want) {
@@ -175,8 +217,8 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
         bool in = u > key;
         if (u == key) in = rank++ < ties;
         if (!in) return 0;
-        if (mp > 0.f && exp((static_cast<double>(v) - static_cast<double>(top)) * inv_t) < static_cast<double>(mp) && u != bk) return 0;
-        return weight_of(v, top, inv_t);
+        const unsigned long long w = weight_of(v, ws);
+        return mp > 0.f && u != bk && static_cast<double>(w) < static_cast<double>(mp) * kOne ? 0 : w;
     };
     unsigned long long mine = 0, rank = before;
     for (int i = i0; i < i1; i++) mine += kept(i, rank);
@@ -189,6 +231,7 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
     if (lane == 31) red[warp] = c;
     __syncthreads();
     unsigned long long at = c - mine, total = 0;
+#pragma unroll 1
     for (int w = 0; w < 32; w++) {
         if (w < warp) at += red[w];
         total += red[w];
@@ -196,6 +239,7 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
     const double goal = static_cast<double>(r) * static_cast<double>(total);
     uint32_t found = 0xffffffffu, last = 0;
     rank = before;
+#pragma unroll 1
     for (int i = i0; i < i1; i++) {
         const unsigned long long w = kept(i, rank);
         if (!w) continue;
@@ -214,6 +258,7 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
         si[warp] = last;
     }
     __syncthreads();
+#pragma unroll 1
     for (int w = 0; w < 32; w++) {
         found = min(found, sk[w]);
         last = max(last, si[w]);
@@ -222,41 +267,70 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
 }
 
 // ---- the fast ways -----------------------------------------------------------
-// A row is read from global memory once and stays in shared memory where it fits.  A logit and its index make one
-// 64-bit number whose order is the row's order (larger logit first, lower index first), so that every cut is one
-// such number.  Weights are computed in 64 bits and summed as integers: a result does not depend on the order of
-// sums, and a running sum that passes close to a border is on the right side of it.
+// A row is read from global memory once and stays in shared memory where it fits (else it is read again from L2).
+// A logit and its index make one 64-bit number whose order is the row's order (larger logit first, lower index
+// first), so that every cut is one such number.  Weights are computed in 64 bits and summed as integers: a result
+// does not depend on the order of sums, and a running sum that passes close to a border is on the right side of it.
 //   k <= kSmallK  The k-th largest of the threads' maxima bounds the k-th largest logit from below: the few
 //                 logits that reach it are sorted, and everything after that happens on the list.
 //   otherwise     Logits are counted in 2048 bins of equal width below the largest.  The count gives the bin of
 //                 the k-th exactly, and the bins around the top-p cut nearly (mass = count x weight of the bin's
 //                 middle); the logits of those bins are sorted, the weights above them summed exactly, and the
 //                 cut read off.  If it is not inside, or there are too many, sample_by_radix takes the row.
-//   draw          sums of kept weights of 4096 consecutive logits at a time, then the warp, lane and logit in
-//                 which the running sum crosses.
-// A block per row: bound by the 64-bit exponentials of the rows that keep thousands of logits and by
-// barriers, not by reading.
-constexpr int kSmallK = 256, kBins = 2048, kList = 4096, kSegs = 16;
+//   draw          sums of kept weights of 128 consecutive logits (one a warp, 4 a lane), then the lane and logit
+//                 in which the running sum crosses.
+// A block per row.  An instruction that is executed once costs some 35 cycles (its line of code comes from L2), so
+// for one row the length of the path counts as much as the work on it; with many rows the 64-bit arithmetic of the
+// rows that keep thousands of logits does.
+constexpr int kSmallK = 256, kBins = 2048, kList = 4096, kSeg = 4 * kThreads, kMaxSegs = 64;
 constexpr int kWarps = kThreads / 32;
 constexpr float kDepth = 20.f;  // the bins reach to weights of e^-20
 
 struct Row {
-    const float* v;  // in shared memory
-    int n;
+    const float* v;  // positions [0, segs * kSeg) in shared memory; logit i is position i + pad, the others are -inf
+    const void* x;   // the row in global memory
+    int n, pad, segs;
     float top;
-    double inv_t;
+    double c;        // weights are 2^((x - top) * c / 32)
     float bin_scale;
-    __device__ __forceinline__ int bin(float x) const { return min(kBins - 1, static_cast<int>((top - x) * bin_scale)); }
+    unsigned long long* cells;  // sums of the weights of 128 positions: [segs][kWarps]
+    __device__ __forceinline__ int bin(float f) const { return min(kBins - 1, static_cast<int>((top - f) * bin_scale)); }
 };
+
+// The 4 positions of this thread in segment s.
+template <typename T, bool SMEM>
+__device__ __forceinline__ void four(const Row& R, int s, float (&f)[4]) {
+    const int j = s * kSeg + 4 * threadIdx.x;
+    if (SMEM) {
+        const float4 q = *reinterpret_cast<const float4*>(R.v + j);
+        f[0] = q.x; f[1] = q.y; f[2] = q.z; f[3] = q.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) f[e] = j + e < R.n ? to_f32<T>(static_cast<const T*>(R.x)[j + e]) : -INFINITY;
+    }
+}
 
 __device__ __forceinline__ unsigned long long place_of(float x, uint32_t i) {
     return (static_cast<unsigned long long>(key_of(x)) << 32) | (0xffffffffu - i);
 }
 __device__ __forceinline__ uint32_t index_of(unsigned long long place) { return 0xffffffffu - static_cast<uint32_t>(place); }
+__device__ __forceinline__ float logit_at(unsigned long long place) { return logit_of(static_cast<uint32_t>(place >> 32)); }
 
-// Sorts list[0, n) in descending order; n <= kList, the list has room up to the next power of two.
-__device__ void sort_list(unsigned long long* list, int n) {
-    int size = 32;
+// Sorts list[0, n) in descending order; the list has room up to the next power of two.
+__device__ __noinline__ void sort_list(unsigned long long* list, int n, Scratch& sc) {
+    if (n <= kSmallK) {  // the place of each is the number of larger ones: 4 threads count for each
+        const int t = threadIdx.x >> 2;
+        const unsigned long long mine = t < n ? list[t] : 0;
+        int rank = 0;
+        for (int j = threadIdx.x & 3; j < n; j += 4) rank += list[j] > mine;
+        rank += __shfl_xor_sync(FULL, rank, 1);
+        rank += __shfl_xor_sync(FULL, rank, 2);
+        __syncthreads();
+        if (t < n && (threadIdx.x & 3) == 0) list[rank] = mine;
+        __syncthreads();
+        return;
+    }
+    int size = 512;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
     __syncthreads();
@@ -275,406 +349,462 @@ __device__ void sort_list(unsigned long long* list, int n) {
 }
 
 // Exclusive running sum over the block; `total` gets the sum.
-__device__ unsigned long long scan_u64(unsigned long long v, unsigned long long* red, unsigned long long& total) {
+__device__ __noinline__ unsigned long long scan_u64(unsigned long long v, unsigned long long* red, unsigned long long& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned long long c = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(FULL, c, o);
-        if (lane >= o) c += y;
-    }
-    __syncthreads();
-    if (lane == 31) red[warp] = c;
-    __syncthreads();
-    unsigned long long w = red[lane], sum = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(FULL, sum, o);
-        if (lane >= o) sum += y;
-    }
-    total = __shfl_sync(FULL, sum, 31);
-    return c - v + (warp ? __shfl_sync(FULL, sum, warp - 1) : 0ull);
-}
-
-// In a descending list: how many elements it takes until the weights, on top of `above`, reach `want`
-// (n + 1 if they do not); `reached` gets the sum up to there.  n <= kList.
-__device__ int prefix_reaching(const Row& R, const unsigned long long* list, int n, unsigned long long above, double want,
-                               Scratch& sc, unsigned long long& reached) {
-    constexpr int PER = kList / kThreads;
-    unsigned long long w[PER], mine = 0;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int i = threadIdx.x * PER + e;
-        w[e] = i < n ? weight_of(logit_of(static_cast<uint32_t>(list[i] >> 32)), R.top, R.inv_t) : 0;
-        mine += w[e];
-    }
-    unsigned long long total;
-    unsigned long long at = above + scan_u64(mine, sc.red, total);
-    if (threadIdx.x == 0) {
-        sc.sel[0] = static_cast<uint32_t>(n + 1);
-        sc.above = above + total;
-    }
-    __syncthreads();
-    int hit = 0x7fffffff;
-    unsigned long long sum = 0;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int i = threadIdx.x * PER + e;
-        at += w[e];
-        if (i < n && hit == 0x7fffffff && static_cast<double>(at) >= want) {
-            hit = i + 1;
-            sum = at;
+    unsigned long long mine = v, base = 0, sum = 0;
+#pragma unroll 1
+    for (int turn = 0; turn < 2; turn++) {  // over the lanes, then over the warps
+        unsigned long long c = mine;
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(FULL, c, o);
+            if (lane >= o) c += y;
+        }
+        if (turn == 0) {
+            base = c - mine;
+            __syncthreads();
+            if (lane == 31) red[warp] = c;
+            __syncthreads();
+            mine = red[lane];
+        } else {
+            sum = c;
         }
     }
-    if (hit != 0x7fffffff) atomicMin(&sc.sel[0], static_cast<uint32_t>(hit));
+    total = __shfl_sync(FULL, sum, 31);
+    const unsigned long long up = __shfl_sync(FULL, sum, max(0, warp - 1));
+    return base + (warp ? up : 0ull);
+}
+
+// In a descending list: how many elements it takes until the weights, on top of `above`, reach `want`; n + 1 if
+// they do not.  n <= kList.
+__device__ __noinline__ int prefix_reaching(const Row& R, const Scale& ws, const unsigned long long* list, int n,
+                                            unsigned long long above, double want, Scratch& sc) {
+    const int per = (n + kThreads - 1) / kThreads, i0 = threadIdx.x * per, i1 = min(n, i0 + per);
+    unsigned long long mine = 0, total;
+#pragma unroll 1
+    for (int i = i0; i < i1; i++) mine += weight_of(logit_at(list[i]), ws);
+    unsigned long long at = above + scan_u64(mine, sc.red, total);
+    if (threadIdx.x == 0) sc.sel[0] = static_cast<uint32_t>(n + 1);
     __syncthreads();
-    if (hit == static_cast<int>(sc.sel[0])) sc.above = sum;
+    if (static_cast<double>(at + mine) >= want) {
+#pragma unroll 1
+        for (int i = i0; i < i1; i++) {
+            at += weight_of(logit_at(list[i]), ws);
+            if (static_cast<double>(at) >= want) {
+                atomicMin(&sc.sel[0], static_cast<uint32_t>(i + 1));
+                break;
+            }
+        }
+    }
     __syncthreads();
-    reached = sc.above;
     return static_cast<int>(sc.sel[0]);
 }
 
-// The row's logits that `keep` holds for, into the list; their number (which may be more than fit).
-template <class F>
-__device__ int collect(const Row& R, unsigned long long* list, uint32_t* count, F keep) {
+// The logits (above -inf) that `keep(x, position)` holds for, into the list; their number (which may be more than
+// fit).  `done(segment)` follows each segment, with the whole warp.
+template <typename T, bool SMEM, class F, class G>
+__device__ __forceinline__ int collect(const Row& R, unsigned long long* list, uint32_t* count, F keep, G done) {
     if (threadIdx.x == 0) *count = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < R.n; i0 += kThreads) {
-        const int i = i0 + threadIdx.x;
-        const float x = i < R.n ? R.v[i] : -INFINITY;
-        const bool in = i < R.n && keep(x, i);
-        const unsigned who = __ballot_sync(FULL, in);
-        if (who) {
-            uint32_t at = 0;
-            if ((threadIdx.x & 31) == 0) at = atomicAdd(count, __popc(who));
-            at = __shfl_sync(FULL, at, 0) + __popc(who & ((1u << (threadIdx.x & 31)) - 1));
-            if (in && at < kList) list[at] = place_of(x, i);
+#pragma unroll 1
+    for (int s = 0; s < R.segs; s++) {
+        float f[4];
+        four<T, SMEM>(R, s, f);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int j = s * kSeg + 4 * threadIdx.x + e;
+            if (keep(f[e], j - R.pad) && f[e] > -INFINITY) {
+                const uint32_t at = atomicAdd(count, 1u);
+                if (at < kList) list[at] = place_of(f[e], j - R.pad);
+            }
         }
+        done(s);
     }
     __syncthreads();
     return static_cast<int>(*count);
 }
 
 // A short list in descending order holds everything that top-k left: the rest of the settings and the draw.
-__device__ uint32_t draw_from_list(const Row& R, unsigned long long* list, int m, float p, float mp, float r, Scratch& sc) {
+__device__ __noinline__ uint32_t draw_from_list(const Scale& ws, const unsigned long long* list, int m, float p, float mp,
+                                                float r, Scratch& sc) {
     unsigned long long* w = sc.bins;  // kSmallK weights
-    static_assert(kSmallK <= 256 && kSmallK <= kThreads, "one thread a weight");
+    static_assert(kSmallK <= 256 && 4 * kSmallK <= kThreads, "four threads an element");
     const int t = threadIdx.x;
-    const unsigned long long mine = t < m ? weight_of(logit_of(static_cast<uint32_t>(list[t] >> 32)), R.top, R.inv_t) : 0;
+    const unsigned long long mine = t < m ? weight_of(logit_at(list[t]), ws) : 0;
     if (t < kSmallK) w[t] = mine;
-    unsigned long long total;
+    unsigned long long total, kept_sum;
     const unsigned long long before = scan_u64(mine, sc.red, total);
     bool in = t < m;
     if (p < 1.f) in = in && (t == 0 || static_cast<double>(before) < static_cast<double>(p) * static_cast<double>(total));
-    if (mp > 0.f && in && t > 0) {
-        const double d = static_cast<double>(logit_of(static_cast<uint32_t>(list[t] >> 32))) - static_cast<double>(R.top);
-        in = d == 0.0 || exp(d * R.inv_t) >= static_cast<double>(mp);
-    }
+    if (mp > 0.f && in && (list[t] >> 32) != (list[0] >> 32)) in = static_cast<double>(mine) >= static_cast<double>(mp) * kOne;
     const int keep = __syncthreads_count(in);  // a prefix
-    unsigned long long kept_sum;
     scan_u64(t < keep ? mine : 0, sc.red, kept_sum);
     const double goal = static_cast<double>(r) * static_cast<double>(kept_sum);
+    // the running sum at each kept element, in index order: 4 threads add for each
+    const int e = t >> 2;
+    const uint32_t idx = e < keep ? index_of(list[e]) : 0u;
+    unsigned long long s = 0;
+#pragma unroll 1
+    for (int j = t & 3; j < keep; j += 4)
+        if (index_of(list[j]) <= idx) s += w[j];
+    s += __shfl_xor_sync(FULL, s, 1);
+    s += __shfl_xor_sync(FULL, s, 2);
     uint32_t found = 0xffffffffu, last = 0;
-    if (t < keep && mine > 0) {  // the running sum at this element, in index order
-        const uint32_t idx = index_of(list[t]);
-        unsigned long long s = 0;
-        for (int j = 0; j < keep; j++)
-            if (index_of(list[j]) <= idx) s += w[j];
+    if (e < keep && w[e] > 0) {
         last = idx;
         if (static_cast<double>(s) >= goal) found = idx;
     }
+    if (t == 0) {
+        sc.sel[0] = 0xffffffffu;
+        sc.sel[1] = 0;
+    }
+    __syncthreads();
     found = __reduce_min_sync(FULL, found);
     last = __reduce_max_sync(FULL, last);
-    __syncthreads();
     if ((t & 31) == 0) {
-        sc.sk[t >> 5] = found;
-        sc.si[t >> 5] = last;
+        atomicMin(&sc.sel[0], found);
+        atomicMax(&sc.sel[1], last);
     }
     __syncthreads();
-    found = __reduce_min_sync(FULL, sc.sk[t & 31]);
-    last = __reduce_max_sync(FULL, sc.si[t & 31]);
-    return found != 0xffffffffu ? found : last;
+    return sc.sel[0] != 0xffffffffu ? sc.sel[0] : sc.sel[1];
 }
 
-// Draw over the whole row among the logits not below `cut` whose weight reaches mp.
-__device__ uint32_t draw_from_row(const Row& R, unsigned long long cut, float mp, float r, Scratch& sc, unsigned long long* segs) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = 4 * ((R.n + kSegs * 4 * kThreads - 1) / (kSegs * 4 * kThreads));  // consecutive logits of a thread
-    const int seg = per * kThreads, nseg = (R.n + seg - 1) / seg;
-    auto weight = [&](int i) -> unsigned long long {
-        const float x = R.v[i];
-        if (place_of(x, i) < cut) return 0;
-        const double d = static_cast<double>(x) - static_cast<double>(R.top), e = exp(d * R.inv_t);
-        if (mp > 0.f && d != 0.0 && e < static_cast<double>(mp)) return 0;
-        return __double2ull_rn(e * kOne);
-    };
-    auto mine_of = [&](int s) {
-        unsigned long long m = 0;
-        const int i0 = s * seg + threadIdx.x * per;
-        for (int i = i0; i < min(R.n, i0 + per); i++) m += weight(i);
-        return m;
-    };
-    for (int s = 0; s < nseg; s++) {
-        unsigned long long m = mine_of(s);
+// This thread's 4 weights of segment s: of the logits not below `cut` whose weight reaches `least`.
+template <typename T, bool SMEM>
+__device__ __forceinline__ unsigned long long kept_weights(const Row& R, const Scale& ws, unsigned long long cut, double least, int s,
+                                                           unsigned long long (&w)[4]) {
+    float f[4];
+    four<T, SMEM>(R, s, f);
+    const float cut_x = cut ? logit_at(cut) : -INFINITY;
+    const int cut_i = static_cast<int>(index_of(cut));
+    unsigned long long sum = 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(FULL, m, o);
-        if (lane == 0) segs[s * kWarps + warp] = m;
+    for (int e = 0; e < 4; e++) {
+        const int i = s * kSeg + 4 * threadIdx.x + e - R.pad;
+        w[e] = 0;
+        if (f[e] > cut_x || (f[e] == cut_x && i <= cut_i)) {
+            w[e] = weight_of(f[e], ws);
+            if (static_cast<double>(w[e]) < least && f[e] != R.top) w[e] = 0;
+        }
+        sum += w[e];
     }
-    for (int i = nseg * kWarps + threadIdx.x; i < kSegs * kWarps; i += kThreads) segs[i] = 0;
-    __syncthreads();
-    const unsigned long long own = threadIdx.x < kSegs * kWarps ? segs[threadIdx.x] : 0;
-    unsigned long long total;
-    const unsigned long long at = scan_u64(own, sc.red, total);
+    return sum;
+}
+__device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+
+// The draw over the whole row, from the cells' sums.
+template <typename T, bool SMEM>
+__device__ __noinline__ uint32_t draw_from_cells(const Row& R, const Scale& ws, unsigned long long cut, double least, float r,
+                                                 Scratch& sc) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cells = R.segs * kWarps;
+    const int per = (cells + kThreads - 1) / kThreads, c0 = threadIdx.x * per, c1 = min(cells, c0 + per);
+    unsigned long long own = 0, total;
+#pragma unroll 1
+    for (int c = c0; c < c1; c++) own += R.cells[c];
+    unsigned long long at = scan_u64(own, sc.red, total);
     const double goal = static_cast<double>(r) * static_cast<double>(total);
-    // the first entry whose running sum reaches the goal and which holds weight
+    // the first cell whose running sum reaches the goal and which holds weight; if none does, the last with weight
     if (threadIdx.x == 0) {
         sc.sel[0] = 0xffffffffu;
         sc.sel[1] = 0;
     }
     __syncthreads();
-    if (own) {
-        if (static_cast<double>(at + own) >= goal) atomicMin(&sc.sel[0], static_cast<uint32_t>(threadIdx.x));
-        atomicMax(&sc.sel[1], static_cast<uint32_t>(threadIdx.x));
+#pragma unroll 1
+    for (int c = c0; c < c1; c++) {
+        const unsigned long long w = R.cells[c];
+        if (!w) continue;
+        at += w;
+        if (static_cast<double>(at) >= goal) atomicMin(&sc.sel[0], static_cast<uint32_t>(c));
+        atomicMax(&sc.sel[1], static_cast<uint32_t>(c));
+        if (static_cast<double>(at) >= goal) break;
     }
     __syncthreads();
-    const bool crossed = sc.sel[0] != 0xffffffffu;
-    const int e = static_cast<int>(crossed ? sc.sel[0] : sc.sel[1]);  // (no crossing: the last logit with weight)
-    if (threadIdx.x == static_cast<unsigned>(e)) sc.above = at;
+    const int cell = static_cast<int>(sc.sel[0] != 0xffffffffu ? sc.sel[0] : sc.sel[1]);
+    if (cell >= c0 && cell < c1) {  // (if this thread went on behind the cell, `at` is too large: add up again)
+        unsigned long long b = 0;
+#pragma unroll 1
+        for (int c = c0; c < cell; c++) b += R.cells[c];
+        sc.above = b;
+        sc.sel[3] = threadIdx.x;
+    }
+    at = scan_u64(own, sc.red, total);
+    if (threadIdx.x == sc.sel[3]) sc.above += at;
     __syncthreads();
-    if (warp == e % kWarps) {
-        const int s = e / kWarps;
-        const unsigned long long m = mine_of(s);
+    if (warp == cell % kWarps) {
+        unsigned long long w[4];
+        const unsigned long long m = kept_weights<T, SMEM>(R, ws, cut, least, cell / kWarps, w);
         unsigned long long c = m;
-#pragma unroll
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
             const unsigned long long y = __shfl_up_sync(FULL, c, o);
             if (lane >= o) c += y;
         }
-        const unsigned long long before = sc.above + c - m;
-        const unsigned hit = __ballot_sync(FULL, m && static_cast<double>(before + m) >= goal), any = __ballot_sync(FULL, m != 0);
-        const int who = hit ? __ffs(hit) - 1 : 31 - __clz(any);
-        if (lane == who) {
-            unsigned long long sum = before;
-            const int i0 = s * seg + threadIdx.x * per;
-            uint32_t last = 0, found = 0xffffffffu;
-            for (int i = i0; i < min(R.n, i0 + per); i++) {
-                const unsigned long long w = weight(i);
-                if (!w) continue;
-                sum += w;
-                last = i;
-                if (found == 0xffffffffu && static_cast<double>(sum) >= goal) found = i;
+        unsigned long long sum = sc.above + c - m;
+        const unsigned hit = __ballot_sync(FULL, m && static_cast<double>(sum + m) >= goal), any = __ballot_sync(FULL, m != 0);
+        if (lane == (hit ? __ffs(hit) - 1 : 31 - __clz(any))) {
+            int last = 0, found = -1;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (!w[e]) continue;
+                sum += w[e];
+                last = e;
+                if (found < 0 && static_cast<double>(sum) >= goal) found = e;
             }
-            sc.sel[2] = found != 0xffffffffu ? found : last;
+            sc.sel[2] = static_cast<uint32_t>(cell / kWarps * kSeg + 4 * threadIdx.x + (found >= 0 ? found : last) - R.pad);
         }
     }
     __syncthreads();
     return sc.sel[2];
 }
 
-// Block = one row, all of it in shared memory.
+// sample_max: first strict maximum above -inf; NaN at index 0 keeps 0.
 template <typename T>
+__device__ __noinline__ uint32_t first_max(const T* x, int n, Scratch& sc) {
+    if (threadIdx.x == 0) sc.above = 0;
+    __syncthreads();
+    unsigned long long best = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const float f = to_f32<T>(x[i]);
+        if (f == f) best = max(best, place_of(f, i));
+    }
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(FULL, best, o));
+    if ((threadIdx.x & 31) == 0) atomicMax(&sc.above, best);
+    __syncthreads();
+    const float x0 = to_f32<T>(x[0]);
+    return x0 != x0 || !sc.above || logit_at(sc.above) == -INFINITY ? 0u : index_of(sc.above);
+}
+
+// The larger of two; NaN (the positive one) if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// Everything but greedy rows.
+template <typename T, bool SMEM>
+__device__ __forceinline__ uint32_t sample_row(const Row& R, const Scale& ws, uint32_t best, uint32_t bk, uint32_t lk, int k, float p,
+                                               float mp, float r, unsigned long long* list, uint32_t* hist, Scratch& sc) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const double least = mp > 0.f ? static_cast<double>(mp) * kOne : 0.0;
+    const bool by_k = k > 0 && k < R.n;
+    auto nothing = [](int) {};
+    if (by_k && k <= kSmallK) {
+        // the k-th largest of the threads' best keys, from below: bisection, to 2^-12 of where they lie
+        uint32_t lo = 0, hi = bk;
+        if (__syncthreads_count(best >= lk) >= k) lo = lk;
+        const uint32_t fine = (hi - lo) >> 12;
+#pragma unroll 1
+        while (hi - lo > fine) {
+            const uint32_t mid = lo + (hi - lo) / 2 + ((hi - lo) & 1);
+            if (__syncthreads_count(best >= mid) >= k) lo = mid;
+            else hi = mid - 1;
+        }
+        const float bound = lo <= key_of(-INFINITY) ? -INFINITY : logit_of(lo);
+        const int m = collect<T, SMEM>(R, list, &sc.sel[3], [&](float f, int) { return f >= bound; }, nothing);
+        if (m > kList) return 0xffffffffu;
+        sort_list(list, m, sc);
+        return draw_from_list(ws, list, min(k, m), p, mp, r, sc);
+    }
+    unsigned long long cut = 0;
+    bool summed = false;  // the cells hold the kept weights
+    if (by_k || p < 1.f) {
+        for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int s = 0; s < R.segs; s++) {
+            float f[4];
+            four<T, SMEM>(R, s, f);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (f[e] > -INFINITY) atomicAdd(&hist[R.bin(f[e])], 1u);
+        }
+        __syncthreads();
+        const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
+        unsigned long long all;
+        const uint32_t before = static_cast<uint32_t>(scan_u64(c0 + c1, sc.red, all));
+        uint32_t room = 0xffffffffu;  // logits left by top-k
+        if (by_k && static_cast<unsigned long long>(k) < all) {
+            const uint32_t uk = static_cast<uint32_t>(k);
+            if (before < uk && uk <= before + c0 + c1) {
+                const bool second = uk > before + c0;
+                sc.sel[0] = 2 * tid + second;
+                sc.sel[1] = uk - before - (second ? c0 : 0);  // which of its bin, from 1
+            }
+            __syncthreads();
+            const int b = static_cast<int>(sc.sel[0]), at = static_cast<int>(sc.sel[1]);
+            const int m = collect<T, SMEM>(R, list, &sc.sel[3], [&](float f, int) { return R.bin(f) == b; }, nothing);
+            if (m > kList) return 0xffffffffu;
+            sort_list(list, m, sc);
+            cut = list[at - 1];
+            room = uk;
+            __syncthreads();
+        }
+        if (p < 1.f && !(p > 0.f)) {  // the first of the order alone
+            const int m = collect<T, SMEM>(R, list, &sc.sel[3], [&](float f, int) { return f == R.top; }, nothing);
+            if (m > kList) return 0xffffffffu;
+            sort_list(list, m, sc);
+            return index_of(list[0]);
+        }
+        if (p < 1.f) {
+            // masses of the bins, from their counts and middles; those that top-k cut off are left out
+            const float step = kDepth / kBins;
+            const uint32_t k0 = min(c0, room > before ? room - before : 0u), k1 = min(c1, room > before + c0 ? room - before - c0 : 0u);
+            const float m0 = k0 * expf(-(2 * tid + 0.5f) * step), m1 = k1 * expf(-(2 * tid + 1.5f) * step);
+            const unsigned long long w0 = __float2ull_rn(m0 * 1073741824.f), w1 = __float2ull_rn(m1 * 1073741824.f);  // of 2^-30
+            unsigned long long mass;
+            const unsigned long long mb = scan_u64(w0 + w1, sc.red, mass);
+            // the bins in which the cut may lie: its mass 0.2 % up and down
+            const double goal = static_cast<double>(p) * static_cast<double>(mass), slack = 0.002 * static_cast<double>(mass);
+            if (tid == 0) sc.sel[0] = sc.sel[1] = kBins - 1;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                const double edge = q ? goal + slack : goal - slack;
+                if (static_cast<double>(mb + w0 + w1) >= edge)
+                    atomicMin(&sc.sel[q], static_cast<uint32_t>(2 * tid + (static_cast<double>(mb + w0) < edge)));
+            }
+            __syncthreads();
+            const int ba = static_cast<int>(sc.sel[0]), bb = static_cast<int>(sc.sel[1]);
+            __syncthreads();
+            // exact: the weights above those bins, by cells, and of everything; the list of the bins between
+            const float cut_x = cut ? logit_at(cut) : -INFINITY;
+            const int cut_i = static_cast<int>(index_of(cut));
+            unsigned long long over = 0, sum = 0, over_all, sum_all;
+            const int m = collect<T, SMEM>(
+                R, list, &sc.sel[3],
+                [&](float f, int i) {
+                    if (!(f > cut_x || (f == cut_x && i <= cut_i))) return false;
+                    const unsigned long long w = weight_of(f, ws);
+                    const int b = R.bin(f);
+                    sum += w;
+                    if (b < ba) over += w;
+                    return b >= ba && b <= bb;
+                },
+                [&](int s) {
+                    const unsigned long long w = warp_total(over);
+                    if (lane == 0) R.cells[s * kWarps + warp] = w;
+                    over_all = s ? over_all + w : w;
+                    over = 0;
+                });
+            unsigned long long t1;
+            scan_u64(lane == 0 ? over_all : 0, sc.red, t1);
+            over_all = t1;
+            scan_u64(sum, sc.red, sum_all);
+            const double want = static_cast<double>(p) * static_cast<double>(sum_all);
+            if (m > kList || !(static_cast<double>(over_all) < want || ba == 0)) return 0xffffffffu;
+            sort_list(list, m, sc);
+            const int t = prefix_reaching(R, ws, list, m, over_all, want, sc);
+            if (t > m) return 0xffffffffu;
+            cut = list[t - 1];
+            // the kept ones of the list join the cells, unless min-p takes some away again
+            summed = least == 0.0 || static_cast<double>(weight_of(logit_at(cut), ws)) >= least;
+            if (summed)
+                for (int i = tid; i < t; i += kThreads) {
+                    const int j = static_cast<int>(index_of(list[i])) + R.pad;
+                    atomicAdd(&R.cells[j / kSeg * kWarps + j % kSeg / 128], weight_of(logit_at(list[i]), ws));
+                }
+        }
+    }
+    if (!summed) {
+#pragma unroll 1
+        for (int s = 0; s < R.segs; s++) {
+            unsigned long long w[4];
+            const unsigned long long m = warp_total(kept_weights<T, SMEM>(R, ws, cut, least, s, w));
+            if (lane == 0) R.cells[s * kWarps + warp] = m;
+        }
+    }
+    __syncthreads();
+    return draw_from_cells<T, SMEM>(R, ws, cut, least, r, sc);
+}
+
+// Block = one row.
+template <typename T, bool SMEM>
 __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleRowsArgs a) {
     extern __shared__ __align__(16) unsigned long long smem_rows[];
     __shared__ Scratch sc;
-    __shared__ unsigned long long segs[kSegs * kWarps];
-    unsigned long long* list = smem_rows;                                 // kList
-    uint32_t* hist = reinterpret_cast<uint32_t*>(list + kList);           // kBins
-    float* v = reinterpret_cast<float*>(hist + kBins);                    // the row, when it fits
+    __shared__ double pow2[32];
+    unsigned long long* list = smem_rows;                                  // kList
+    uint32_t* hist = reinterpret_cast<uint32_t*>(list + kList);            // kBins
+    unsigned long long* cells = reinterpret_cast<unsigned long long*>(hist + kBins);
+    float* v = reinterpret_cast<float*>(cells + a.segs * kWarps);          // SMEM: the row
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T* x = static_cast<const T*>(a.logits) + static_cast<size_t>(row) * a.row_stride;
     const int n = a.n;
     const float temp = a.temperature[row];
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f, r = a.r[row];
-
-    // the largest logit, lowest index; NaN or +inf anywhere; the row into shared memory
-    uint32_t bk = 0, bi = 0xffffffffu;
-    int bad = 0;
-    auto see = [&](float f, int i) {
-        if (!(f < INFINITY)) bad = 1;
-        if (f == f) {
-            const uint32_t u = key_of(f);
-            if (u > bk) {  // (a thread's indexes rise)
-                bk = u;
-                bi = static_cast<uint32_t>(i);
-            }
-        }
-    };
-    constexpr int VE = 16 / sizeof(T);
-    const int head = a.fits ? min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T))) : n;
-    for (int i = tid; i < head; i += kThreads) {
-        const float f = to_f32<T>(x[i]);
-        see(f, i);
-        if (a.fits) v[i] = f;
+    if (!(temp > 0.f)) {
+        const uint32_t best = first_max<T>(x, n, sc);
+        if (tid == 0) a.out[row] = best;
+        return;
     }
-    if (a.fits) {
-        const int nv = (n - head) / VE;
+    if (tid < 32) pow2[tid] = kPow2[tid];
+
+    // each thread's largest logit (NaN if there is one); the row into shared memory, 16 bytes of it at a time
+    float own = -INFINITY;
+    int pad = 0;
+    constexpr int VE = 16 / sizeof(T);
+    if (SMEM) {
+        const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+        pad = (4 - (head & 3)) & 3;  // the first whole 16 bytes begin at a multiple of 4 positions
+        const int nv = (n - head) / VE, tail = head + nv * VE;
+        for (int j = tid; j < pad + head; j += kThreads) {
+            const float f = j < pad ? -INFINITY : to_f32<T>(x[j - pad]);
+            own = max_nan(own, f);
+            v[j] = f;
+        }
 #pragma unroll 4
         for (int q = tid; q < nv; q += kThreads) {
             const uint4 raw = *reinterpret_cast<const uint4*>(x + head + q * VE);
             const T* e = reinterpret_cast<const T*>(&raw);
+            float f[VE];
 #pragma unroll
             for (int c = 0; c < VE; c++) {
-                const float f = to_f32<T>(e[c]);
-                see(f, head + q * VE + c);
-                v[head + q * VE + c] = f;
+                f[c] = to_f32<T>(e[c]);
+                own = max_nan(own, f[c]);
             }
-        }
-        for (int i = head + nv * VE + tid; i < n; i += kThreads) {
-            const float f = to_f32<T>(x[i]);
-            see(f, i);
-            v[i] = f;
-        }
-    }
-    const uint32_t own_best = bk;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint32_t u = __shfl_xor_sync(FULL, bk, o), i = __shfl_xor_sync(FULL, bi, o);
-        if (u > bk || (u == bk && i < bi)) {
-            bk = u;
-            bi = i;
+            for (int c = 0; c < VE; c += 4)
+                *reinterpret_cast<float4*>(v + pad + head + q * VE + c) = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
         }
+        for (int j = pad + tail + tid; j < a.segs * kSeg; j += kThreads) {
+            const float f = j - pad < n ? to_f32<T>(x[j - pad]) : -INFINITY;
+            own = max_nan(own, f);
+            v[j] = f;
+        }
+    } else {
+#pragma unroll 4
+        for (int i = tid; i < n; i += kThreads) own = max_nan(own, to_f32<T>(x[i]));
     }
+    // the largest and the smallest of the threads' keys (of those that saw more than -inf)
+    const uint32_t best = key_of(own);
+    uint32_t bk = __reduce_max_sync(FULL, best), lk = __reduce_min_sync(FULL, own == -INFINITY ? 0xffffffffu : best);
     if (lane == 0) {
         sc.sk[warp] = bk;
-        sc.si[warp] = bi;
-    }
-    bad = __syncthreads_or(bad);
-    bk = sc.sk[lane];
-    bi = sc.si[lane];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint32_t u = __shfl_xor_sync(FULL, bk, o), i = __shfl_xor_sync(FULL, bi, o);
-        if (u > bk || (u == bk && i < bi)) {
-            bk = u;
-            bi = i;
-        }
-    }
-    const float top = bi == 0xffffffffu ? -INFINITY : logit_of(bk);
-    if (!(temp > 0.f)) {  // sample_max: first strict maximum above -inf; NaN at index 0 keeps 0
-        if (tid == 0) {
-            const float x0 = to_f32<T>(x[0]);
-            a.out[row] = (x0 != x0 || top == -INFINITY) ? 0u : bi;
-        }
-        return;
-    }
-    if (bad || top == -INFINITY) {
-        if (tid == 0) a.out[row] = static_cast<uint32_t>(n - 1);
-        return;
-    }
-    const double inv_t = 1.0 / static_cast<double>(temp);
-    __syncthreads();  // sk and si have been read
-    Row R{v, n, top, inv_t, static_cast<float>(kBins / (kDepth * static_cast<double>(temp)))};
-    uint32_t answer = 0xffffffffu;
-    bool done = false;
-    if (a.fits) {
-        const bool by_k = k > 0 && k < n;
-        if (by_k && k <= kSmallK) {
-            // the k-th largest of the threads' best keys, by bisection
-            uint32_t lo = 0, hi = bk;  // count(best >= lo) >= k or lo = 0
-            while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo) / 2 + ((hi - lo) & 1);
-                if (__syncthreads_count(own_best >= mid) >= k) lo = mid;
-                else hi = mid - 1;
-            }
-            const int m = collect(R, list, &sc.sel[3], [&](float f, int) { return key_of(f) >= lo; });
-            if (m <= kList) {
-                sort_list(list, m);
-                answer = draw_from_list(R, list, min(k, m), p, mp, r, sc);
-                done = true;
-            }
-        } else {
-            unsigned long long cut = 0;
-            done = true;
-            if (by_k || p < 1.f) {
-                for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-                __syncthreads();
-                for (int i = tid; i < n; i += kThreads) atomicAdd(&hist[R.bin(v[i])], 1u);
-                __syncthreads();
-            }
-            uint32_t room = 0xffffffffu;  // logits left by top-k
-            if (by_k) {
-                // the bin of the k-th
-                const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-                unsigned long long all;
-                const uint32_t before = static_cast<uint32_t>(scan_u64(c0 + c1, sc.red, all));
-                const uint32_t uk = static_cast<uint32_t>(k);
-                if (before < uk && uk <= before + c0 + c1) {
-                    const bool second = uk > before + c0;
-                    sc.sel[0] = 2 * tid + second;
-                    sc.sel[1] = uk - before - (second ? c0 : 0);  // which of the bin's, from 1
-                }
-                __syncthreads();
-                const int b = static_cast<int>(sc.sel[0]), at = static_cast<int>(sc.sel[1]);
-                const int m = collect(R, list, &sc.sel[3], [&](float f, int) { return R.bin(f) == b; });
-                if (m <= kList) {
-                    sort_list(list, m);
-                    cut = list[at - 1];
-                    room = uk;
-                } else {
-                    done = false;
-                }
-                __syncthreads();
-            }
-            if (done && p < 1.f) {
-                if (!(p > 0.f)) {
-                    cut = place_of(top, bi);
-                } else {
-                    // masses of the bins, from their counts and middles; those that top-k cut off are left out
-                    const float step = 20.f / kBins;
-                    const uint32_t c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-                    unsigned long long all;
-                    const uint32_t nb = static_cast<uint32_t>(scan_u64(c0 + c1, sc.red, all));
-                    const uint32_t k0 = min(c0, room > nb ? room - nb : 0u), k1 = min(c1, room > nb + c0 ? room - nb - c0 : 0u);
-                    const float m0 = k0 * expf(-(2 * tid + 0.5f) * step), m1 = k1 * expf(-(2 * tid + 1.5f) * step);
-                    constexpr double kMass = 1073741824.0;  // 2^30: sums of 2^22 logits fit
-                    const unsigned long long w0 = __double2ull_rn(m0 * kMass), w1 = __double2ull_rn(m1 * kMass);
-                    unsigned long long mass;
-                    const unsigned long long mb = scan_u64(w0 + w1, sc.red, mass);
-                    // the bins in which the cut may lie: its mass 0.2 % up and down
-                    const double goal = static_cast<double>(p) * static_cast<double>(mass), slack = 0.002 * static_cast<double>(mass);
-                    if (tid == 0) {
-                        sc.sel[0] = kBins - 1;
-                        sc.sel[1] = kBins - 1;
-                    }
-                    __syncthreads();
-                    if (static_cast<double>(mb + w0) >= goal - slack) atomicMin(&sc.sel[0], static_cast<uint32_t>(2 * tid));
-                    else if (static_cast<double>(mb + w0 + w1) >= goal - slack) atomicMin(&sc.sel[0], static_cast<uint32_t>(2 * tid + 1));
-                    if (static_cast<double>(mb + w0) >= goal + slack) atomicMin(&sc.sel[1], static_cast<uint32_t>(2 * tid));
-                    else if (static_cast<double>(mb + w0 + w1) >= goal + slack) atomicMin(&sc.sel[1], static_cast<uint32_t>(2 * tid + 1));
-                    __syncthreads();
-                    const int ba = static_cast<int>(sc.sel[0]), bb = static_cast<int>(sc.sel[1]);
-                    __syncthreads();
-                    // exact: the weights above those bins and of everything; the list of the bins between
-                    unsigned long long over = 0, sum = 0;
-                    const int m = collect(R, list, &sc.sel[3], [&](float f, int i) {
-                        if (place_of(f, i) < cut) return false;
-                        const unsigned long long w = weight_of(f, top, inv_t);
-                        const int b = R.bin(f);
-                        sum += w;
-                        if (b < ba) over += w;
-                        return b >= ba && b <= bb;
-                    });
-                    unsigned long long over_all, sum_all, reached;
-                    scan_u64(over, sc.red, over_all);
-                    scan_u64(sum, sc.red, sum_all);
-                    const double want = static_cast<double>(p) * static_cast<double>(sum_all);
-                    if (m <= kList && (static_cast<double>(over_all) < want || ba == 0)) {
-                        sort_list(list, m);
-                        const int t = prefix_reaching(R, list, m, over_all, want, sc, reached);
-                        if (t <= m) cut = max(cut, list[t - 1]);
-                        else done = false;
-                        __syncthreads();
-                    } else {
-                        done = false;
-                    }
-                }
-            }
-            if (done) answer = draw_from_row(R, cut, mp, r, sc, segs);
-        }
+        sc.si[warp] = lk;
     }
     __syncthreads();
-    if (!done) answer = sample_by_radix<T>(x, n, k, p, mp, r, inv_t, top, bk, sc);
+    bk = __reduce_max_sync(FULL, sc.sk[lane]);
+    lk = __reduce_min_sync(FULL, sc.si[lane]);
+    uint32_t answer = static_cast<uint32_t>(n - 1);
+    if (bk < 0xff800000u && bk > key_of(-INFINITY)) {  // neither NaN nor +inf, and something above -inf
+        const float top = logit_of(bk);
+        const int k = a.top_k ? a.top_k[row] : 0;
+        const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f, r = a.r[row];
+        const Scale ws{widen(top), 46.16624130844683 / static_cast<double>(temp), pow2};  // 32 / ln 2
+        const Row R{v, x, n, pad, a.segs, top, ws.c, kBins / (kDepth * temp), cells};
+        answer = 0xffffffffu;
+        if (a.segs <= kMaxSegs) answer = sample_row<T, SMEM>(R, ws, best, bk, lk, k, p, mp, r, list, hist, sc);
+        if (answer == 0xffffffffu) {
+            __syncthreads();
+            answer = sample_by_radix<T>(x, n, k, p, mp, r, ws, bk, sc);
+        }
+    }
     if (tid == 0) a.out[row] = answer;
 }
 
@@ -694,10 +824,12 @@ extern "C" tl_status tl_sample_rows(uint32_t* out, const void* logits, tl_dtype 
     TL_REQUIRE(n_rows <= 0x7fffffffull, "tl_sample_rows: n_rows = %zu", n_rows);
     TL_REQUIRE(out && logits && r && temperature, "tl_sample_rows: null pointer");
     TL_REQUIRE(reinterpret_cast<uintptr_t>(logits) % paged::dtype_size(dtype) == 0, "tl_sample_rows: logits misaligned");
-    const size_t base = kList * 8 + kBins * 4, most = 227 * 1024 - sizeof(Scratch) - kSegs * kWarps * 8 - 1024;
-    const bool fits = base + n * 4 <= most;
-    SampleRowsArgs a{out, logits, row_stride, static_cast<int>(n), r, temperature, top_p, min_p, top_k, fits};
-    const int smem = static_cast<int>(fits ? base + n * 4 : base);
+    // up to 3 positions before the first logit align it; a segment more than shared memory holds: read from L2
+    const int segs = static_cast<int>((n + 3 + kSeg - 1) / kSeg);
+    const size_t base = kList * 8 + kBins * 4 + static_cast<size_t>(std::min(segs, kMaxSegs)) * kWarps * 8;
+    const bool fits = base + static_cast<size_t>(segs) * kSeg * 4 <= 227 * 1024 - sizeof(Scratch) - 32 * 8 - 1024;
+    SampleRowsArgs a{out, logits, row_stride, static_cast<int>(n), r, temperature, top_p, min_p, top_k, segs};
+    const int smem = static_cast<int>(fits ? base + static_cast<size_t>(segs) * kSeg * 4 : base);
     const unsigned grid = static_cast<unsigned>(n_rows);
     const cudaStream_t s = as_stream(stream);
     auto run = [&](auto kernel) -> tl_status {
@@ -705,8 +837,8 @@ extern "C" tl_status tl_sample_rows(uint32_t* out, const void* logits, tl_dtype 
         kernel<<<grid, kThreads, smem, s>>>(a);
         return TL_OK;
     };
-    if (dtype == TL_F32) TL_TRY(run(k_sample_rows<float>));
-    else if (dtype == TL_F16) TL_TRY(run(k_sample_rows<__half>));
-    else TL_TRY(run(k_sample_rows<__nv_bfloat16>));
+    if (dtype == TL_F32) TL_TRY(fits ? run(k_sample_rows<float, true>) : run(k_sample_rows<float, false>));
+    else if (dtype == TL_F16) TL_TRY(fits ? run(k_sample_rows<__half, true>) : run(k_sample_rows<__half, false>));
+    else TL_TRY(fits ? run(k_sample_rows<__nv_bfloat16, true>) : run(k_sample_rows<__nv_bfloat16, false>));
     return check_launch("sample_rows");
 }
