@@ -334,8 +334,13 @@ __device__ __noinline__ void sort_list(unsigned long long* list, int n, Scratch&
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
     __syncthreads();
+#pragma unroll 1
     for (int k = 2; k <= size; k <<= 1)
+#pragma unroll 1
         for (int j = k >> 1; j > 0; j >>= 1) {
+            if (j >= 32) __syncthreads();  // (up to 32 apart, a warp's pairs lie in its own 64 elements)
+            else __syncwarp();
+#pragma unroll 1
             for (int t = threadIdx.x; t < size / 2; t += kThreads) {
                 const int a = 2 * t - (t & (j - 1)), b = a + j;  // (t with a 0 bit put in at j)
                 const unsigned long long x = list[a], y = list[b];
@@ -344,8 +349,8 @@ __device__ __noinline__ void sort_list(unsigned long long* list, int n, Scratch&
                     list[b] = x;
                 }
             }
-            __syncthreads();
         }
+    __syncthreads();
 }
 
 // Exclusive running sum over the block; `total` gets the sum.
@@ -660,8 +665,14 @@ __device__ __forceinline__ uint32_t sample_row(const Row& R, const Scale& ws, ui
             const unsigned long long w0 = __float2ull_rn(m0 * 1073741824.f), w1 = __float2ull_rn(m1 * 1073741824.f);  // of 2^-30
             unsigned long long mass;
             const unsigned long long mb = scan_u64(w0 + w1, sc.red, mass);
-            // the bins in which the cut may lie: its mass 0.2 % up and down
-            const double goal = static_cast<double>(p) * static_cast<double>(mass), slack = 0.002 * static_cast<double>(mass);
+            // The bins in which the cut may lie.  A logit's weight is off by up to half a bin's width (step / 2), as
+            // good as independently: four standard deviations, and 0.01 % of the mass.
+            unsigned long long squares;
+            scan_u64(__float2ull_rn((m0 * expf(-(2 * tid + 0.5f) * step) + m1 * expf(-(2 * tid + 1.5f) * step)) * 1073741824.f), sc.red,
+                     squares);
+            const double goal = static_cast<double>(p) * static_cast<double>(mass);
+            const double slack = 1e-4 * static_cast<double>(mass) +
+                                 4.0 * 0.289 * step * 32768.0 * sqrt(static_cast<double>(squares));  // (both are counted in 2^-30)
             if (tid == 0) sc.sel[0] = sc.sel[1] = kBins - 1;
             __syncthreads();
 #pragma unroll
