@@ -152,92 +152,188 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan(PlanArgs a) {
 }
 
 // ---- norm, rotation, cache write -------------------------------------------
-// hd / 8 lanes hold one head of one token, 8 dims each: 16-byte accesses, the
-// norm's sum by shuffles, and the rotation's partner dim is rot / 16 lanes away
-// in the same register.  One read and one write of every element: bound by HBM
-// (latency for few tokens).
+// A warp takes a share of one token's heads, 32 / L of them at a time, L = hd / 8 lanes a head and 8 dims a lane:
+// 16-byte accesses, and the token's angles and the norm's weights stay in registers over its heads.  The rotation's
+// partner dims lie half / 8 lanes away; their raw bits come by shuffles (for 16-bit types half as many as of the
+// fp32 values).  The next turns' heads are fetched before these are worked on, the first before the angles.  One read and one write of every element:
+// bound by HBM for many tokens, by latency for few; then a token's heads are spread over more warps.
 struct RopeArgs {
     const int32_t *positions, *slots;
     const float *cos_, *sin_, *wq, *wk;
     size_t row_stride, block_stride;
     float eps;
     int n_tokens, H, KV, n_pos, rot, shift, n_slots;
+    int parts;  // warps a token
 };
 
+// 8 elements as raw words, and as fp32.
+template <typename T>
+struct Raw8 {
+    static constexpr int W = sizeof(T) == 4 ? 8 : 4;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const T* p) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        if (W == 8) {
+            const uint4 b = reinterpret_cast<const uint4*>(p)[1];
+            w[W - 4] = b.x; w[W - 3] = b.y; w[W - 2] = b.z; w[W - 1] = b.w;
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const;
+};
+template <>
+__device__ __forceinline__ void Raw8<float>::get(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = __uint_as_float(w[j]);
+}
+template <>
+__device__ __forceinline__ void Raw8<__half>::get(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ void Raw8<__nv_bfloat16>::get(float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+}
+
+constexpr int kRopeWarps = 4;
+
 template <typename TI, typename TO, int HD>
-__global__ void __launch_bounds__(256) k_qk_norm_rope(TO* q_out, TO* kc, TO* vc, const TI* qkv, RopeArgs a) {
-    constexpr int L = HD / 8;  // lanes per head
-    const int rows = a.H + 2 * a.KV;
-    const int l = threadIdx.x % L;
-    const long long n = static_cast<long long>(a.n_tokens) * rows;
-    const long long per = gridDim.x * static_cast<long long>(256 / L);
-    // whole warps take the same number of turns, so that the shuffles see every lane
-    for (long long base = static_cast<long long>(blockIdx.x) * (256 / L) + threadIdx.x / 32 * (32 / L); base < n; base += per) {
-        const long long u = base + (threadIdx.x % 32) / L;
-        const bool in = u < n;
-        const int t = in ? static_cast<int>(u / rows) : 0;
-        const int hh = in ? static_cast<int>(u % rows) : 0;
-        const int pos = a.positions[t];
-        const bool live = in && pos >= 0 && pos < a.n_pos;
-        float x[8];
+__global__ void __launch_bounds__(kRopeWarps * 32) k_qk_norm_rope(TO* q_out, TO* kc, TO* vc, const TI* qkv,
+                                                                  const __grid_constant__ RopeArgs a) {
+    constexpr int L = HD / 8, PER = 32 / L, AHEAD = sizeof(TI) == 2 ? 6 : 3;  // lanes a head, heads at a time, turns fetched ahead
+    const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
+    const unsigned w = blockIdx.x * kRopeWarps + (threadIdx.x >> 5);
+    const int t = static_cast<int>(w / static_cast<unsigned>(a.parts)), part = static_cast<int>(w % static_cast<unsigned>(a.parts));
+    if (t >= a.n_tokens) return;
+    const int rows = a.H + 2 * a.KV, turns = (rows + PER - 1) / PER, per = (turns + a.parts - 1) / a.parts;
+    const int u0 = part * per, u1 = min(turns, u0 + per);
+    const TI* src = qkv + static_cast<size_t>(t) * a.row_stride + 8 * l;
+    Raw8<TI> next[AHEAD];
+    auto fetch = [&](int u) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = 0.f;
-        if (live) Vec8<TI>::load(x, qkv + static_cast<size_t>(t) * a.row_stride + static_cast<size_t>(hh) * HD + 8 * l);
-        const bool is_v = hh >= a.H + a.KV;
-        const float* w = hh < a.H ? a.wq : a.wk;
-        float ss = 0.f;
+        for (int i = 0; i < AHEAD; i++) {
+            const int hh = (u + i) * PER + sub;
+            if (u + i < u1 && hh < rows) next[i].load(src + static_cast<size_t>(hh) * HD);
+            else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) ss += x[j] * x[j];
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
-        if (!is_v && w != nullptr) {
-            const float inv = 1.0f / sqrtf(ss / static_cast<float>(HD) + a.eps);
-            float g[8];
-            Vec8<float>::load(g, w + 8 * l);
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = (x[j] * inv) * g[j];
+                for (int j = 0; j < Raw8<TI>::W; j++) next[i].w[j] = 0u;
+            }
         }
-        const int half = a.rot / 2, off = half / 8;  // the partner's distance in lanes
-        const bool lower = l < off, upper = l >= off && l < 2 * off;
-        float y[8];
-        const int from = (threadIdx.x & 31) + (lower ? off : upper ? -off : 0);
+    };
+    fetch(u0);
+    const int pos = a.positions[t];
+    if (pos < 0 || pos >= a.n_pos) return;  // a row of no sequence
+    const int slot = a.slots[t];
+
+    const int half = a.rot / 2, off = half / 8;
+    const bool lower = l < off, turned = l < 2 * off;
+    const int from = lane + (lower ? off : turned ? -off : 0), pl = l + (from - lane);  // the partner's lane, and within its head
+    float c[8], s[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = __shfl_sync(FULL, x[j], from);
-        if (live && !is_v && (lower || upper)) {
-            float c[8], s[8];
-            const size_t ang = static_cast<size_t>(pos) * half + 8 * (lower ? l : l - off);
-            Vec8<float>::load(c, a.cos_ + ang);
-            Vec8<float>::load(s, a.sin_ + ang);
+    for (int j = 0; j < 8; j++) {
+        c[j] = 1.f;
+        s[j] = 0.f;
+    }
+    if (turned) {
+        const size_t ang = static_cast<size_t>(pos) * half + 8 * (lower ? l : l - off);
+        Vec8<float>::load(c, a.cos_ + ang);
+        Vec8<float>::load(s, a.sin_ + ang);
+        if (lower) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = lower ? x[j] * c[j] - y[j] * s[j] : y[j] * s[j] + x[j] * c[j];
+            for (int j = 0; j < 8; j++) s[j] = -s[j];
         }
-        if (live) {
+    }
+    const bool cached = slot >= 0 && slot < a.n_slots;
+    const size_t at = cached ? static_cast<size_t>(slot >> a.shift) * a.block_stride +
+                                   static_cast<size_t>(slot & ((1 << a.shift) - 1)) * HD + 8 * l
+                             : 0;
+    float fa[8], fb[8];  // x' = (x fa + partner fb) / rms
+    int cur = -1;
+    const float* wt = nullptr;
+    for (int u = u0; u < u1; u += AHEAD) {
+        Raw8<TI> raw[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) raw[i] = next[i];
+        fetch(u + AHEAD);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (u + i >= u1) break;
+            const int hh = (u + i) * PER + sub;
+            const int kind = hh < a.H ? 0 : hh < a.H + a.KV ? 1 : 2;  // q, k, v
+            if (kind != cur && kind < 2) {  // the section's factors
+                wt = kind ? a.wk : a.wq;
+                float g[8], gy[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) g[j] = gy[j] = 1.f;
+                if (wt != nullptr) {
+                    Vec8<float>::load(g, wt + 8 * l);
+                    Vec8<float>::load(gy, wt + 8 * pl);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    fa[j] = g[j] * c[j];
+                    fb[j] = gy[j] * s[j];
+                }
+            }
+            cur = kind;
+            float x[8], y[8];
+            raw[i].get(x);
+            Raw8<TI> other;
+#pragma unroll
+            for (int j = 0; j < Raw8<TI>::W; j++) other.w[j] = __shfl_sync(FULL, raw[i].w[j], from);
+            float inv = 1.f;
+            if (a.wq != nullptr || a.wk != nullptr) {
+                float ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) ss += x[j] * x[j];
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
+                if (wt != nullptr) inv = rsqrtf(ss * (1.f / HD) + a.eps);  // (2 ulp)
+            }
+            if (hh >= rows) continue;  // (a last turn of fewer heads; the shuffles are behind)
+            if (kind < 2) {
+                if (turned) {
+                    other.get(y);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] = (x[j] * fa[j] + y[j] * fb[j]) * inv;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] = x[j] * fa[j] * inv;
+                }
+            }
             if (hh < a.H) {
                 Vec8<TO>::store(q_out + (static_cast<size_t>(t) * a.H + hh) * HD + 8 * l, x);
-            } else {
-                const int slot = a.slots[t];
-                if (slot >= 0 && slot < a.n_slots) {
-                    const int g = is_v ? hh - a.H - a.KV : hh - a.H;
-                    const size_t at = static_cast<size_t>(slot >> a.shift) * a.block_stride +
-                                      ((static_cast<size_t>(g) << a.shift) + (slot & ((1 << a.shift) - 1))) * HD + 8 * l;
-                    Vec8<TO>::store((is_v ? vc : kc) + at, x);
-                }
+            } else if (cached) {
+                const int g = kind == 2 ? hh - a.H - a.KV : hh - a.H;
+                Vec8<TO>::store((kind == 2 ? vc : kc) + at + (static_cast<size_t>(g) << a.shift) * HD, x);
             }
         }
     }
 }
 
 template <typename TI, typename TO>
-void launch_rope(void* q_out, const tl_paged_cache* c, const void* qkv, const RopeArgs& a, cudaStream_t s) {
-    const long long rows = static_cast<long long>(a.n_tokens) * (a.H + 2 * a.KV);
-    const long long per = 256 / (static_cast<int>(c->head_dim) / 8);
-    const int grid = static_cast<int>(std::min<long long>((rows + per - 1) / per, 8ll * sm_count() * 4));
+void launch_rope(void* q_out, const tl_paged_cache* c, const void* qkv, RopeArgs a, cudaStream_t s) {
+    const int per = 32 / (static_cast<int>(c->head_dim) / 8), turns = (a.H + 2 * a.KV + per - 1) / per;
+    // Few tokens: as many warps a token as fill the device (16 an SM), down to one turn each.
+    const long long want = 16ll * sm_count();
+    a.parts = static_cast<int>(std::max<long long>(1, std::min<long long>(turns, want / std::max(1, a.n_tokens))));
+    const long long warps = static_cast<long long>(a.n_tokens) * a.parts;
+    const unsigned grid = static_cast<unsigned>((warps + kRopeWarps - 1) / kRopeWarps);
     if (c->head_dim == 128)
-        k_qk_norm_rope<TI, TO, 128><<<grid, 256, 0, s>>>(static_cast<TO*>(q_out), static_cast<TO*>(c->k),
-                                                         static_cast<TO*>(c->v), static_cast<const TI*>(qkv), a);
+        k_qk_norm_rope<TI, TO, 128><<<grid, kRopeWarps * 32, 0, s>>>(
+            static_cast<TO*>(q_out), static_cast<TO*>(c->k), static_cast<TO*>(c->v), static_cast<const TI*>(qkv), a);
     else
-        k_qk_norm_rope<TI, TO, 64><<<grid, 256, 0, s>>>(static_cast<TO*>(q_out), static_cast<TO*>(c->k),
-                                                        static_cast<TO*>(c->v), static_cast<const TI*>(qkv), a);
+        k_qk_norm_rope<TI, TO, 64><<<grid, kRopeWarps * 32, 0, s>>>(
+            static_cast<TO*>(q_out), static_cast<TO*>(c->k), static_cast<TO*>(c->v), static_cast<const TI*>(qkv), a);
 }
 
 template <typename TI>
@@ -303,7 +399,7 @@ tl_status tl_qk_norm_rope(void* q_out, const tl_paged_cache* cache, const void* 
     RopeArgs a{positions, slots, cos_, sin_, q_weight, k_weight, row_stride, cache->block_stride, eps,
                static_cast<int>(n_tokens), static_cast<int>(n_heads), static_cast<int>(cache->n_kv_heads),
                static_cast<int>(n_pos), static_cast<int>(rot_dim), __builtin_ctzll(cache->block_size),
-               static_cast<int>(cache->n_blocks * cache->block_size)};
+               static_cast<int>(cache->n_blocks * cache->block_size), 1};
     const cudaStream_t s = as_stream(stream);
     if (dtype == TL_F32) launch_rope_to<float>(q_out, cache, qkv, a, s);
     else if (dtype == TL_F16) launch_rope_to<__half>(q_out, cache, qkv, a, s);
