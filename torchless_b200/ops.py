@@ -166,22 +166,35 @@ def quantize_i8(x, group: int = 64):
 
 
 class _On:
-    """Makes a tensor's device current for a call where it is not."""
+    """Makes a device current for a call where it is not."""
 
-    def __init__(self, device):
-        import torch
-        self.torch, self.device, self.before = torch, device, -1
+    __slots__ = ("index", "before")
+
+    def __init__(self, index):
+        self.index = index
 
     def __enter__(self):
-        cur = self.torch.cuda.current_device()
-        if cur != self.device.index:
-            self.before = cur
-            self.torch.cuda.set_device(self.device)
-        return ctypes.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
+        import torch
+        self.before = torch.cuda.current_device()
+        torch.cuda.set_device(self.index)
 
     def __exit__(self, *exc):
-        if self.before >= 0:
-            self.torch.cuda.set_device(self.before)
+        import torch
+        torch.cuda.set_device(self.before)
+
+
+def _launch(device, f, args) -> None:
+    """f(*args, current stream of `device`), with that device current."""
+    import torch
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        st = f(*args, stream)
+    else:
+        with _On(index):
+            st = f(*args, stream)
+    if st:
+        check(st)
 
 
 _DTYPES = None
@@ -198,9 +211,9 @@ def _dtype(t) -> int:
         raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}") from None
 
 
-def _arg(t, dtype, device, n=None, name="argument"):
-    """A contiguous tensor of `dtype` on `device` with n elements: its address."""
-    if t.dtype != dtype:
+def _arg(t, dtype, device, n, name):
+    """A contiguous tensor of `dtype` on `device` with n elements (None: any): its address."""
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not {device}")
@@ -213,17 +226,16 @@ def _arg(t, dtype, device, n=None, name="argument"):
 
 def _cache(k_cache, v_cache):
     from . import tl_paged_cache
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+    shape, st = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape or st != v_cache.stride():
         raise ValueError("k_cache and v_cache must be [n_blocks, n_kv_heads, block_size, head_dim] of one layout")
-    if k_cache.dtype != v_cache.dtype or k_cache.device != v_cache.device or not k_cache.is_cuda:
+    if k_cache.dtype is not v_cache.dtype or k_cache.device != v_cache.device or not k_cache.is_cuda:
         raise ValueError("k_cache and v_cache must be CUDA tensors of one type and device")
-    n, kv, bs, hd = k_cache.shape
-    st = k_cache.stride()
+    n, kv, bs, hd = shape
     if st[1:] != (bs * hd, hd, 1):
         raise ValueError("the pages of a cache must be contiguous")
-    return tl_paged_cache(k=k_cache.data_ptr(), v=v_cache.data_ptr(), n_blocks=n, n_kv_heads=kv, block_size=bs,
-                          head_dim=hd, block_stride=max(st[0], kv * bs * hd) if n == 1 else st[0],
-                          dtype=_dtype(k_cache))
+    return tl_paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), n, kv, bs, hd,
+                          max(st[0], kv * bs * hd) if n == 1 else st[0], _dtype(k_cache))
 
 
 def paged_plan(block_table, cached, new_tokens, free_blocks, block_size: int, n_tokens: int):
@@ -247,15 +259,16 @@ def paged_plan(block_table, cached, new_tokens, free_blocks, block_size: int, n_
         raise ValueError("ops take CUDA tensors")
     if n_tokens < 0 or block_size < 0:
         raise ValueError("n_tokens and block_size must not be negative")
-    t, c, f = (_arg(block_table, i32, dev, name="block_table"), _arg(cached, i32, dev, n_req, "cached"),
+    t, c, f = (_arg(block_table, i32, dev, None, "block_table"), _arg(cached, i32, dev, n_req, "cached"),
                _arg(new_tokens, i32, dev, n_req, "new_tokens"))
-    fr = _arg(free_blocks, i32, dev, name="free_blocks")
-    out = torch.empty(2 * n_req + 1 + 2 * n_tokens + 2, dtype=i32, device=dev)
-    q_start, seq_lens, positions, slots, counts = parts = out.split([n_req + 1, n_req, n_tokens, n_tokens, 2])
-    with _On(dev) as s:
-        check(lib().tl_paged_plan(t, q_start.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-                                  counts.data_ptr(), c, f, fr, free_blocks.numel(), n_req, width, block_size, n_tokens, s))
-    return parts
+    fr = _arg(free_blocks, i32, dev, None, "free_blocks")
+    sizes = (n_req + 1, n_req, n_tokens, n_tokens, 2)
+    out = torch.empty(2 * n_req + 2 * n_tokens + 3, dtype=i32, device=dev)
+    a = out.data_ptr()
+    _launch(dev, lib().tl_paged_plan,
+            (t, a, a + 4 * (n_req + 1), a + 4 * (2 * n_req + 1), a + 4 * (2 * n_req + 1 + n_tokens),
+             a + 4 * (2 * n_req + 1 + 2 * n_tokens), c, f, fr, free_blocks.numel(), n_req, width, block_size, n_tokens))
+    return out.split_with_sizes(sizes)
 
 
 def qk_norm_rope(q_out, k_cache, v_cache, qkv, positions, slots, cos, sin, q_weight=None, k_weight=None,
@@ -281,13 +294,12 @@ def qk_norm_rope(q_out, k_cache, v_cache, qkv, positions, slots, cos, sin, q_wei
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise ValueError("cos and sin must be [n_pos, rot_dim / 2]")
     stride = qkv.stride(0) if n > 1 else qkv.shape[1]
-    with _On(dev) as s:
-        check(lib().tl_qk_norm_rope(
-            _arg(q_out, q_out.dtype, dev, name="q_out"), ctypes.byref(c), qkv.data_ptr(), _dtype(qkv), stride,
-            _arg(positions, torch.int32, dev, n, "positions"), _arg(slots, torch.int32, dev, n, "slots"),
-            _arg(cos, f32, dev, name="cos"), _arg(sin, f32, dev, name="sin"), cos.shape[0], 2 * cos.shape[1],
-            None if q_weight is None else _arg(q_weight, f32, dev, hd, "q_weight"),
-            None if k_weight is None else _arg(k_weight, f32, dev, hd, "k_weight"), float(eps), n, heads, s))
+    _launch(dev, lib().tl_qk_norm_rope,
+            (_arg(q_out, q_out.dtype, dev, None, "q_out"), ctypes.byref(c), qkv.data_ptr(), _dtype(qkv), stride,
+             _arg(positions, torch.int32, dev, n, "positions"), _arg(slots, torch.int32, dev, n, "slots"),
+             _arg(cos, f32, dev, None, "cos"), _arg(sin, f32, dev, None, "sin"), cos.shape[0], 2 * cos.shape[1],
+             None if q_weight is None else _arg(q_weight, f32, dev, hd, "q_weight"),
+             None if k_weight is None else _arg(k_weight, f32, dev, hd, "k_weight"), eps, n, heads))
 
 
 def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, scale=None, window: int = 0) -> None:
@@ -313,16 +325,24 @@ def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, sc
     if block_table.dim() != 2 or window < 0:
         raise ValueError("block_table must be [n_seq, max_blocks] and window not negative")
     n_seq, width = block_table.shape
-    args = (_arg(block_table, i32, dev, name="block_table"), width, _arg(q_start, i32, dev, n_seq + 1, "q_start"),
-            _arg(seq_lens, i32, dev, n_seq, "seq_lens"), n_seq, n, heads)
-    need = ctypes.c_size_t()
-    L = lib()
-    check(L.tl_paged_attention_workspace(ctypes.byref(c), n, heads, n_seq, width, ctypes.byref(need)))
-    with _On(dev) as s:
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        check(L.tl_paged_attention(
-            _arg(out, out.dtype, dev, name="out"), q.data_ptr(), q.stride(0) if n > 1 else heads * hd, ctypes.byref(c),
-            *args, hd ** -0.5 if scale is None else float(scale), int(window), ws.data_ptr(), need.value, s))
+    L, cache = lib(), ctypes.byref(c)
+    key = (c.dtype, hd, c.n_kv_heads, heads, n, n_seq)
+    need = _WORKSPACE.get(key)
+    if need is None:
+        size = ctypes.c_size_t()
+        check(L.tl_paged_attention_workspace(cache, n, heads, n_seq, width, ctypes.byref(size)))
+        if len(_WORKSPACE) >= 4096:
+            _WORKSPACE.clear()
+        need = _WORKSPACE[key] = size.value
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _launch(dev, L.tl_paged_attention,
+            (_arg(out, out.dtype, dev, None, "out"), q.data_ptr(), q.stride(0) if n > 1 else heads * hd, cache,
+             _arg(block_table, i32, dev, None, "block_table"), width, _arg(q_start, i32, dev, n_seq + 1, "q_start"),
+             _arg(seq_lens, i32, dev, n_seq, "seq_lens"), n_seq, n, heads, hd ** -0.5 if scale is None else scale, window,
+             ws.data_ptr(), need))
+
+
+_WORKSPACE = {}  # the workspace's size by type, heads and numbers of rows and sequences
 
 
 def sample_rows(logits, r, temperature, top_k=None, top_p=None, min_p=None):
@@ -342,8 +362,7 @@ def sample_rows(logits, r, temperature, top_k=None, top_p=None, min_p=None):
             None if top_k is None else _arg(top_k, torch.int32, dev, rows, "top_k"),
             None if top_p is None else _arg(top_p, f32, dev, rows, "top_p"),
             None if min_p is None else _arg(min_p, f32, dev, rows, "min_p"))
-    with _On(dev) as s:
-        out = torch.empty(rows, dtype=torch.int32, device=dev)
-        check(lib().tl_sample_rows(out.data_ptr(), logits.data_ptr(), _dtype(logits),
-                                   logits.stride(0) if rows > 1 else n, rows, n, *ptrs, s))
+    out = torch.empty(rows, dtype=torch.int32, device=dev)
+    _launch(dev, lib().tl_sample_rows, (out.data_ptr(), logits.data_ptr(), _dtype(logits),
+                                        logits.stride(0) if rows > 1 else n, rows, n, *ptrs))
     return out
