@@ -86,12 +86,15 @@ struct Shape {
     static constexpr size_t SMEM = 1024 + static_cast<size_t>(kWarps) * NST * 2 * SIDE + kWarps * JOIN * 4 + 512;
 };
 
-// Steps of KS keys, tiles of R rows.  A tile without keys counts one step, so that its zeros get written.
+// Steps of KS keys, tiles of R rows.  Beginning and ending a tile takes about as long as kTileCost steps, which count
+// as steps before its first key, so that a batch of short sequences is shared as evenly as one of long ones.  A
+// tile without keys counts one step more, so that its zeros get written.
 template <int R_, int KS>
 struct SplitPlan {
     static constexpr int R = R_;
+    static constexpr int kTileCost = 12;
     static __device__ __forceinline__ int steps(const Tile& t) {
-        return t.hi <= t.lo ? 1 : (t.hi - 1) / KS - t.lo / KS + 1;
+        return kTileCost + (t.hi <= t.lo ? 1 : (t.hi - 1) / KS - t.lo / KS + 1);
     }
 };
 
@@ -472,13 +475,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     using P = SplitPlan<R, KS>;
     Cursor c;
-    // at least one step a warp, so that a small call is not cut into crumbs
-    const int per = find_share<P, kWarps>(a, c, ws, kWarps);
+    // at least one step a warp beside the tile's cost, so that a small call is not cut into crumbs
+    const int per = find_share<P, kWarps>(a, c, ws, kWarps + P::kTileCost);
     if (per == 0) return;
 
     // producer: a second cursor that runs up to NST steps ahead; ids of this warp's next 32 steps in the lanes
     Cursor pc = c;
-    int ps = pc.s + warp, pid_at = 32, pid0 = -1, pid1 = -1;
+    auto first_step = [&](const Cursor& x) { return max(0, x.s - P::kTileCost) + warp; };
+    int ps = first_step(pc), pid_at = 32, pid0 = -1, pid1 = -1;
     bool more = true;
     int put_st = 0, got_st = 0, ahead = 0;
     uint32_t got_parity = 0;
@@ -494,12 +498,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (bool go = true; go; go = next_tile<P>(a, c), first_tile = false) {
         bool begun = false;
 #pragma unroll 1
-        for (int s = c.s + warp;; s += kWarps) {
+        for (int s = first_step(c);; s += kWarps) {
 #pragma unroll 1
             while (more && ahead < NST) {  // one step into the ring
-                if (ps >= pc.end) {
+                if (ps >= pc.end - P::kTileCost) {
                     more = next_tile<P>(a, pc);
-                    ps = pc.s + warp;
+                    ps = first_step(pc);
                     pid_at = 32;
                     continue;
                 }
@@ -538,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 core.begin(a, c, lane);
                 begun = true;
             }
-            if (s >= c.end) break;
+            if (s >= c.end - P::kTileCost) break;
             dead |= !spin(&bars[got_st], (got_parity >> got_st) & 1);
             got_parity ^= 1u << got_st;
             StepInfo si;
@@ -619,47 +623,94 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of the tile that block blockIdx.x began: part i > 0 is the first tile of block blockIdx.x + i.
+// Two warps a row (one for its even parts, one for the odd); lane = 4 or 2 dims.
 template <typename T, int HD, int R>
-__global__ void __launch_bounds__(kThreads) k_attend_join(const __grid_constant__ AttendArgs a, const Head* heads, const float* parts) {
+__global__ void __launch_bounds__(kThreads) k_attend_join(const __grid_constant__ AttendArgs a, const Head* heads,
+                                                          const float* parts) {
+    constexpr int D = HD / 32;
+    __shared__ float half[kWarps / 2][32 * D + 2];
     pdl_wait();
     const Head h = heads[blockIdx.x];
     if (h.parts == 0) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, odd = warp & 1;
     Cursor c;
     c.g = h.g;
     c.t = tile_of(a, h.b, h.rt, R);
     constexpr size_t rec = static_cast<size_t>(R) * (HD + 4);
     const float* p0 = parts + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
     const float* p1 = parts + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;  // parts 1 .. are 2 * rec apart
-    for (int row = warp; row < c.t.nrows; row += kWarps) {
-        float M = -INFINITY, bad = 0.f;
-        for (int i = lane; i < h.parts; i += 32) {
-            const float* p = (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4);
-            M = fmaxf(M, p[0]);
-            bad = fmaxf(bad, p[2]);
-        }
-        M = warp_max(M);
-        bad = warp_max(bad);
-        int tok, hh;
-        row_of(a, c, row, tok, hh);
-        if (bad > 0.f) {
-            attend_row<T, HD>(a, h.b, tok, hh, lane);
-            continue;
-        }
-        float L = 0.f, acc[HD / 32];
+    auto part = [&](int i, int row) { return (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4); };
+#pragma unroll 1
+    for (int row0 = 0; row0 < c.t.nrows; row0 += kWarps / 2) {
+        const int row = row0 + (warp >> 1);
+        float M = -INFINITY, bad = 0.f, L = 0.f, acc[D];
 #pragma unroll
-        for (int d = 0; d < HD / 32; d++) acc[d] = 0.f;
-#pragma unroll 4
-        for (int i = 0; i < h.parts; i++) {
-            const float* p = (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4);
-            const float f = M == -INFINITY ? 1.f : ex2(p[0] - M);
-            L += p[1] * f;
+        for (int d = 0; d < D; d++) acc[d] = 0.f;
+        if (row < c.t.nrows) {
+#pragma unroll 1
+            for (int i0 = odd; i0 < h.parts; i0 += 16) {  // 8 parts at a time
+                float m[8], l[8], v[8][D], mx = M;
 #pragma unroll
-            for (int d = 0; d < HD / 32; d++) acc[d] += p[4 + lane + 32 * d] * f;
+                for (int k = 0; k < 8; k++) {
+                    const int i = i0 + 2 * k;
+                    m[k] = -INFINITY;
+                    l[k] = 0.f;
+#pragma unroll
+                    for (int d = 0; d < D; d++) v[k][d] = 0.f;
+                    if (i < h.parts) {
+                        const float* p = part(i, row);
+                        const float4 q = *reinterpret_cast<const float4*>(p);
+                        m[k] = q.x;
+                        l[k] = q.y;
+                        bad = fmaxf(bad, q.z);
+#pragma unroll
+                        for (int d = 0; d < D; d++) v[k][d] = p[4 + lane + 32 * d];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) mx = fmaxf(mx, m[k]);
+                const float f0 = mx == -INFINITY ? 1.f : ex2(M - mx);
+                L *= f0;
+#pragma unroll
+                for (int d = 0; d < D; d++) acc[d] *= f0;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float f = mx == -INFINITY ? 1.f : ex2(m[k] - mx);
+                    L += l[k] * f;
+#pragma unroll
+                    for (int d = 0; d < D; d++) acc[d] += v[k][d] * f;
+                }
+                M = mx;
+            }
         }
-        T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD;
+        if (odd) {
+            float* x = half[warp >> 1];
+            if (lane == 0) {
+                x[0] = M;
+                x[1] = bad > 0.f ? NAN : L;  // (NaN: to be done over)
+            }
 #pragma unroll
-        for (int d = 0; d < HD / 32; d++) out[lane + 32 * d] = from_f32<T>(L != 0.f ? acc[d] / L : 0.f);
+            for (int d = 0; d < D; d++) x[2 + lane + 32 * d] = acc[d];
+        }
+        __syncthreads();
+        if (!odd && row < c.t.nrows) {
+            const float* x = half[warp >> 1];
+            int tok, hh;
+            row_of(a, c, row, tok, hh);
+            const float mx = fmaxf(M, x[0]), f0 = mx == -INFINITY ? 1.f : ex2(M - mx), f1 = mx == -INFINITY ? 1.f : ex2(x[0] - mx);
+            if (bad > 0.f || x[1] != x[1]) {
+                attend_row<T, HD>(a, h.b, tok, hh, lane);
+            } else {
+                const float sum = L * f0 + x[1] * f1;
+                T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD;
+#pragma unroll
+                for (int d = 0; d < D; d++) {
+                    const float o = acc[d] * f0 + x[2 + lane + 32 * d] * f1;
+                    out[lane + 32 * d] = from_f32<T>(sum != 0.f ? o / sum : 0.f);
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 

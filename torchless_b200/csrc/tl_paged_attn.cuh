@@ -131,41 +131,47 @@ __device__ __forceinline__ bool next_tile(const AttendArgs& a, Cursor& c) {
     return true;
 }
 
-// Exclusive running sum over the block's NW warps; `total` gets the sum.
+// Exclusive running sum over the block's NW warps; `total` gets the sum.  (Loops are not unrolled in what a block
+// does once: every instruction's first execution waits for its code.)
 template <int NW>
-__device__ __forceinline__ long long scan_block(long long v, long long* ws, long long& total) {
+__device__ __noinline__ long long scan_block(long long v, long long* ws, long long& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(FULL, x, o);
-        if (lane >= o) x += y;
+    long long mine = v, base = 0, sum = 0;
+#pragma unroll 1
+    for (int turn = 0; turn < 2; turn++) {  // over the lanes, then over the warps
+        long long c = mine;
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(FULL, c, o);
+            if (lane >= o) c += y;
+        }
+        if (turn == 0) {
+            base = c - mine;
+            __syncthreads();
+            if (lane == 31) ws[warp] = c;
+            __syncthreads();
+            mine = lane < NW ? ws[lane] : 0;
+        } else {
+            sum = c;
+        }
     }
-    __syncthreads();
-    if (lane == 31) ws[warp] = x;
-    __syncthreads();
-    long long before = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < NW; w++) {
-        if (w < warp) before += ws[w];
-        sum += ws[w];
-    }
-    total = sum;
-    return x - v + before;
+    total = __shfl_sync(FULL, sum, 31);
+    const long long up = __shfl_sync(FULL, sum, warp ? warp - 1 : 0);
+    return base + (warp ? up : 0);
 }
 
-// Steps of sequence b's tiles rt0, rt0 + stride, ... of one kv head.
 template <class Plan>
 __device__ __noinline__ long long steps_of_sequence(const AttendArgs& a, int b, int rt0, int stride) {
     if (b >= a.n_seq) return 0;
     int first, n;
     rows_of(a, b, first, n);
     long long u = 0;
+#pragma unroll 1
     for (int rt = rt0; rt * Plan::R < n * a.group; rt += stride) u += Plan::steps(tile_of(a, b, rt, Plan::R));
     return u;
 }
 __device__ __forceinline__ long long warp_sum_ll(long long v) {
-#pragma unroll
+#pragma unroll 1
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
     return v;
 }
@@ -236,7 +242,7 @@ __device__ __forceinline__ int find_share(const AttendArgs& a, Cursor& c, long l
         const int rt = c.rt + lane;
         const long long s = rt * Plan::R < n * a.group ? static_cast<long long>(Plan::steps(tile_of(a, c.b, rt, Plan::R))) * a.KV : 0;
         long long x = s;
-#pragma unroll
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
             const long long y = __shfl_up_sync(FULL, x, o);
             if (lane >= o) x += y;
