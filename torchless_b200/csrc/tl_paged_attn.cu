@@ -79,7 +79,7 @@ __device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity) {
 // Keys per step, stages per warp, and the bytes of one side of a stage.
 template <typename T, int HD>
 struct Shape {
-    static constexpr int KS = std::is_same<T, float>::value ? 8 : 16;
+    static constexpr int KS = std::is_same<T, float>::value ? 8 : HD == 64 ? 32 : 16;
     static constexpr int SIDE = KS * HD * static_cast<int>(sizeof(T));
     static constexpr int NST = SIDE >= 4096 ? 3 : 5;
     static constexpr int JOIN = 8 * (HD + 4);  // floats of one warp's 8 rows: {max, sum, flag, -, values}
@@ -100,7 +100,7 @@ struct SplitPlan {
 
 // ---- arithmetic of one warp -------------------------------------------------
 
-// One step's bounds: keys [key0, key0 + KS), page halves that exist (bit 0: first 8 keys, bit 1: the rest).
+// One step: keys [key0, key0 + KS); bit k of valid: the page of its keys 8 k .. exists.
 struct StepInfo {
     int key0;
     uint32_t valid;
@@ -149,7 +149,7 @@ __device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo, __nv_
 }
 // 16 rows on the matrix instruction: lane l holds rows l / 4 and l / 4 + 8.
 template <typename T, int HD, int R>
-struct Core {
+struct Core {  // (its stages: see Shape)
     static_assert(R == 16, "the instruction's height");
     static constexpr int NO = HD / 8;
     uint32_t q[HD / 16][4];
@@ -195,49 +195,86 @@ struct Core {
 
     __device__ void step(const AttendArgs& a, const Cursor& c, StepInfo si, const uint8_t* sk, const uint8_t* sv,
                          int lane) {
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        constexpr int KS = Shape<T, HD>::KS, G = KS / 16, NT = KS / 8;
         const uint32_t kb = su32(sk), vb = su32(sv);
-        {
-            const int key = (lane >> 4) * 8 + (lane & 7), c0 = (lane >> 3) & 1;
+        uint32_t kr[G][HD / 16][4], vr[G][HD / 16][4];
+        const int kk = (lane >> 4) * 8 + (lane & 7), kc0 = (lane >> 3) & 1;
 #pragma unroll
-            for (int k = 0; k < HD / 16; k++) {
-                uint32_t r[4];
-                ldsm4(r, kb + at(key, 2 * k + c0));
-                mma16<T>(s[0], q[k], r[0], r[1]);
-                mma16<T>(s[1], q[k], r[2], r[3]);
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++) ldsm4(kr[g][k], kb + at(16 * g + kk, 2 * k + kc0));
+        // the scores in two chains of sums, and the values on their way while they are worked on
+        float s[NT][4], s2[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[n][e] = s2[n][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < HD / 16; k += 2)
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                mma16<T>(s[2 * g], q[k], kr[g][k][0], kr[g][k][1]);
+                mma16<T>(s[2 * g + 1], q[k], kr[g][k][2], kr[g][k][3]);
+                mma16<T>(s2[2 * g], q[k + 1], kr[g][k + 1][0], kr[g][k + 1][1]);
+                mma16<T>(s2[2 * g + 1], q[k + 1], kr[g][k + 1][2], kr[g][k + 1][3]);
             }
-        }
+        const int vkey = ((lane >> 3) & 1) * 8 + (lane & 7), vc = lane >> 4;
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) ldsm4t(vr[g][j], vb + at(16 * g + vkey, 2 * j + vc));
         const float sl = a.scale * 1.4426950408889634f;  // log2 units
         // every row attends to every key of an inner step
-        const bool edge = si.valid != 3u || si.key0 < c.t.lo_last || si.key0 > c.t.hi_first - 16;
+        const bool edge = si.valid != (1u << NT) - 1 || si.key0 < c.t.lo_last || si.key0 > c.t.hi_first - KS;
         const int kc = si.key0 + 2 * (lane & 3);
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                s[n][e] *= sl;
-                if (edge) {
+            for (int e = 0; e < 4; e++) s[n][e] = (s[n][e] + s2[n][e]) * sl;
+        if (edge) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
                     const int key = kc + 8 * n + (e & 1), i = e >> 1;
                     if (!(key >= lo[i] && key < hi[i] && ((si.valid >> n) & 1))) s[n][e] = -INFINITY;
                 }
+            // keys that no row attends to must not reach the products (0 x NaN)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                uint32_t keep = ~0u;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int key = kc + 8 * n + e;
+                    if (!(key >= c.t.lo && key < c.t.hi && ((si.valid >> n) & 1))) keep &= e ? 0xffffu : 0xffff0000u;
+                }
+#pragma unroll
+                for (int j = 0; j < HD / 16; j++) {
+                    vr[n / 2][j][n & 1] &= keep;
+                    vr[n / 2][j][2 + (n & 1)] &= keep;
+                }
             }
+        }
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            float mx = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+            float mx = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+#pragma unroll
+            for (int n = 1; n < NT; n++) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
             mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
             const float mn = fmaxf(m[i], mx);
             const float base = mn == -INFINITY ? 0.f : mn;
             f[i] = ex2(m[i] - base);
             m[i] = mn;
+            float sum = 0.f;
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+            for (int n = 0; n < NT; n++) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) s[n][2 * i + e] = ex2(s[n][2 * i + e] - base);
-            l[i] = l[i] * f[i] + ((s[0][2 * i] + s[0][2 * i + 1]) + (s[1][2 * i] + s[1][2 * i + 1]));
+                sum += s[n][2 * i] + s[n][2 * i + 1];
+            }
+            l[i] = l[i] * f[i] + sum;
         }
         if (__any_sync(FULL, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
@@ -248,35 +285,22 @@ struct Core {
                 o[n][3] *= f[1];
             }
         }
-        uint32_t ph[4], pl[4];
-        ph[0] = split2(s[0][0], s[0][1], pl[0], static_cast<T*>(nullptr));
-        ph[1] = split2(s[0][2], s[0][3], pl[1], static_cast<T*>(nullptr));
-        ph[2] = split2(s[1][0], s[1][1], pl[2], static_cast<T*>(nullptr));
-        ph[3] = split2(s[1][2], s[1][3], pl[3], static_cast<T*>(nullptr));
-        // keys that no row attends to must not reach the products (0 x NaN)
-        uint32_t keep[2] = {~0u, ~0u};
-        if (edge) {
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+        for (int g = 0; g < G; g++) {
+            uint32_t ph[4], pl[4];
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int key = kc + 8 * n + e;
-                    if (!(key >= c.t.lo && key < c.t.hi && ((si.valid >> n) & 1))) keep[n] &= e ? 0xffffu : 0xffff0000u;
-                }
-        }
-        const int vkey = ((lane >> 3) & 1) * 8 + (lane & 7), vc = lane >> 4;
+            for (int e = 0; e < 4; e++)
+                ph[e] = split2(s[2 * g + e / 2][2 * (e & 1)], s[2 * g + e / 2][2 * (e & 1) + 1], pl[e], static_cast<T*>(nullptr));
 #pragma unroll
-        for (int j = 0; j < HD / 16; j++) {
-            uint32_t r[4];
-            ldsm4t(r, vb + at(vkey, 2 * j + vc));
-            if (edge) {
-#pragma unroll
-                for (int u = 0; u < 4; u++) r[u] &= keep[u & 1];
+            for (int j = 0; j < HD / 16; j++) {
+                mma16<T>(o[2 * j], ph, vr[g][j][0], vr[g][j][1]);
+                mma16<T>(o[2 * j + 1], ph, vr[g][j][2], vr[g][j][3]);
             }
-            mma16<T>(o[2 * j], ph, r[0], r[1]);
-            mma16<T>(o[2 * j + 1], ph, r[2], r[3]);
-            mma16<T>(o[2 * j], pl, r[0], r[1]);
-            mma16<T>(o[2 * j + 1], pl, r[2], r[3]);
+#pragma unroll
+            for (int j = 0; j < HD / 16; j++) {
+                mma16<T>(o[2 * j], pl, vr[g][j][0], vr[g][j][1]);
+                mma16<T>(o[2 * j + 1], pl, vr[g][j][2], vr[g][j][3]);
+            }
         }
     }
 
@@ -482,11 +506,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // producer: a second cursor that runs up to NST steps ahead; ids of this warp's next 32 steps in the lanes
     Cursor pc = c;
     auto first_step = [&](const Cursor& x) { return max(0, x.s - P::kTileCost) + warp; };
-    int ps = first_step(pc), pid_at = 32, pid0 = -1, pid1 = -1;
+    constexpr int NT = KS / 8;          // most pages of a step
+    const int rows = min(KS, 1 << a.shift);  // rows of a copy
+    int ps = first_step(pc), pid_at = 32, pid[NT];
     bool more = true;
     int put_st = 0, got_st = 0, ahead = 0;
     uint32_t got_parity = 0;
-    uint32_t valid_bits = 0;  // 2 bits for each stage
+    uint32_t valid_bits = 0;  // NT bits for each stage
     int stage_key[NST];
 #pragma unroll
     for (int i = 0; i < NST; i++) stage_key[i] = 0;
@@ -510,29 +536,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (pid_at == 32) {
                     const int blk = (pc.t.lo / KS + ps) + kWarps * lane;  // below 2^31 / KS + 256
                     const int key = blk < kMaxLen / KS ? blk * KS : -1;
-                    pid0 = page_of(a, pc.b, key);
-                    pid1 = (KS == 16 && a.shift == 3) ? page_of(a, pc.b, key < 0 ? -1 : key + 8) : pid0;
+#pragma unroll
+                    for (int k = 0; k < NT; k++)
+                        pid[k] = k == 0 || 8 * k % rows == 0 ? page_of(a, pc.b, key < 0 ? -1 : key + 8 * k) : pid[k - 1];
                     pid_at = 0;
                 }
-                const int id0 = __shfl_sync(FULL, pid0, pid_at), id1 = __shfl_sync(FULL, pid1, pid_at);
-                pid_at++;
                 const int key0 = (pc.t.lo / KS + ps) * KS;
-                const uint32_t v = (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u);
-                valid_bits = (valid_bits & ~(3u << (2 * put_st))) | (v << (2 * put_st));
+                int id[NT];
+                uint32_t v = 0;
+#pragma unroll
+                for (int k = 0; k < NT; k++) {
+                    id[k] = __shfl_sync(FULL, pid[k], pid_at);
+                    v |= (id[k] >= 0 ? 1u : 0u) << k;
+                }
+                pid_at++;
+                valid_bits = (valid_bits & ~(((1u << NT) - 1) << (NT * put_st))) | (v << (NT * put_st));
 #pragma unroll
                 for (int i = 0; i < NST; i++)
                     if (i == put_st) stage_key[i] = key0;
                 if (lane == 0) {
                     uint8_t* k = ring + put_st * 2 * S::SIDE;
-                    uint8_t* vv = k + S::SIDE;
-                    const int row = (pc.g << a.shift) + (key0 & ((1 << a.shift) - 1));
                     bar_expect_tx(&bars[put_st], 2 * S::SIDE);
-                    tma_page(k, &map_k, row, id0, &bars[put_st]);
-                    tma_page(vv, &map_v, row, id0, &bars[put_st]);
-                    if (KS == 16 && a.shift == 3) {
-                        tma_page(k + S::SIDE / 2, &map_k, pc.g << 3, id1, &bars[put_st]);
-                        tma_page(vv + S::SIDE / 2, &map_v, pc.g << 3, id1, &bars[put_st]);
-                    }
+#pragma unroll
+                    for (int x = 0; x < NT; x++)
+                        if (8 * x % rows == 0) {
+                            const int row = (pc.g << a.shift) + ((key0 + 8 * x) & ((1 << a.shift) - 1));
+                            tma_page(k + x * (S::SIDE / NT), &map_k, row, id[x], &bars[put_st]);
+                            tma_page(k + S::SIDE + x * (S::SIDE / NT), &map_v, row, id[x], &bars[put_st]);
+                        }
                 }
                 put_st = put_st + 1 == NST ? 0 : put_st + 1;
                 ahead++;
@@ -546,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             dead |= !spin(&bars[got_st], (got_parity >> got_st) & 1);
             got_parity ^= 1u << got_st;
             StepInfo si;
-            si.valid = (valid_bits >> (2 * got_st)) & 3u;
+            si.valid = (valid_bits >> (NT * got_st)) & ((1u << NT) - 1);
             si.key0 = 0;
 #pragma unroll
             for (int i = 0; i < NST; i++)
