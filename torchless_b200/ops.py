@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 
-from . import check, lib
+from . import check, lib, tl_paged_cache
 
 
 def _ptr(t) -> int:
@@ -165,77 +165,67 @@ def quantize_i8(x, group: int = 64):
 # host, so a step can be captured in a CUDA graph.
 
 
-class _On:
-    """Makes a device current for a call where it is not."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        import torch
-        self.before = torch.cuda.current_device()
-        torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        import torch
-        torch.cuda.set_device(self.before)
+_torch = None   # torch, from the first call on
+_DTYPES = {}    # the cache's types by torch's
 
 
-def _launch(device, f, args) -> None:
-    """f(*args, current stream of `device`), with that device current."""
+def _load():
+    global _torch
     import torch
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
+    _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    _torch = torch
+    return torch
+
+
+def _launch(index, f, *args) -> None:
+    """f(*args, current stream of device `index`), with that device current."""
+    C = _torch._C
+    stream = C._cuda_getCurrentRawStream(index)
+    before = C._cuda_getDevice()
+    if before == index:
         st = f(*args, stream)
     else:
-        with _On(index):
+        _torch.cuda.set_device(index)
+        try:
             st = f(*args, stream)
+        finally:
+            _torch.cuda.set_device(before)
     if st:
         check(st)
 
 
-_DTYPES = None
-
-
 def _dtype(t) -> int:
-    global _DTYPES
-    if _DTYPES is None:
-        import torch
-        _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
     try:
         return _DTYPES[t.dtype]
     except KeyError:
         raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}") from None
 
 
-def _arg(t, dtype, device, n, name):
-    """A contiguous tensor of `dtype` on `device` with n elements (None: any): its address."""
+def _arg(t, dtype, index, n, name):
+    """A contiguous tensor of `dtype` on device `index` with n elements (None: any): its address."""
+    if t.dtype is dtype and t.get_device() == index and t.is_contiguous() and (n is None or t.numel() == n):
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not cuda:{index}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if n is not None and t.numel() != n:
-        raise ValueError(f"{name} has {t.numel()} elements, not {n}")
-    return t.data_ptr()
+    raise ValueError(f"{name} has {t.numel()} elements, not {n}")
 
 
 def _cache(k_cache, v_cache):
-    from . import tl_paged_cache
-    shape, st = k_cache.shape, k_cache.stride()
+    """The pages as the library's structure, and their device."""
+    shape, st, index = k_cache.shape, k_cache.stride(), k_cache.get_device()
     if len(shape) != 4 or shape != v_cache.shape or st != v_cache.stride():
         raise ValueError("k_cache and v_cache must be [n_blocks, n_kv_heads, block_size, head_dim] of one layout")
-    if k_cache.dtype is not v_cache.dtype or k_cache.device != v_cache.device or not k_cache.is_cuda:
+    if index < 0 or v_cache.get_device() != index or k_cache.dtype is not v_cache.dtype:
         raise ValueError("k_cache and v_cache must be CUDA tensors of one type and device")
     n, kv, bs, hd = shape
-    if st[1:] != (bs * hd, hd, 1):
+    if st[1] != bs * hd or st[2] != hd or st[3] != 1:
         raise ValueError("the pages of a cache must be contiguous")
     return tl_paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), n, kv, bs, hd,
-                          max(st[0], kv * bs * hd) if n == 1 else st[0], _dtype(k_cache))
+                          st[0] if n > 1 else max(st[0], kv * bs * hd), _dtype(k_cache)), index
 
 
 def paged_plan(block_table, cached, new_tokens, free_blocks, block_size: int, n_tokens: int):
@@ -250,25 +240,26 @@ def paged_plan(block_table, cached, new_tokens, free_blocks, block_size: int, n_
     slots [n_tokens], counts [2])``; position and slot are -1 in rows behind
     the last token, the slot of a token without a page is -1, and counts are
     the pages taken and the pages missing."""
-    import torch
+    torch = _torch or _load()
     if block_table.dim() != 2:
         raise ValueError("block_table must be [n_req, max_blocks]")
     n_req, width = block_table.shape
-    dev, i32 = block_table.device, torch.int32
-    if not block_table.is_cuda:
+    index, i32 = block_table.get_device(), torch.int32
+    if index < 0:
         raise ValueError("ops take CUDA tensors")
     if n_tokens < 0 or block_size < 0:
         raise ValueError("n_tokens and block_size must not be negative")
-    t, c, f = (_arg(block_table, i32, dev, None, "block_table"), _arg(cached, i32, dev, n_req, "cached"),
-               _arg(new_tokens, i32, dev, n_req, "new_tokens"))
-    fr = _arg(free_blocks, i32, dev, None, "free_blocks")
-    sizes = (n_req + 1, n_req, n_tokens, n_tokens, 2)
-    out = torch.empty(2 * n_req + 2 * n_tokens + 3, dtype=i32, device=dev)
-    a = out.data_ptr()
-    _launch(dev, lib().tl_paged_plan,
-            (t, a, a + 4 * (n_req + 1), a + 4 * (2 * n_req + 1), a + 4 * (2 * n_req + 1 + n_tokens),
-             a + 4 * (2 * n_req + 1 + 2 * n_tokens), c, f, fr, free_blocks.numel(), n_req, width, block_size, n_tokens))
-    return out.split_with_sizes(sizes)
+    table, before, new, free = (
+        _arg(block_table, i32, index, None, "block_table"), _arg(cached, i32, index, n_req, "cached"),
+        _arg(new_tokens, i32, index, n_req, "new_tokens"), _arg(free_blocks, i32, index, None, "free_blocks"))
+    out = torch.empty(2 * n_req + 2 * n_tokens + 3, dtype=i32, device=block_table.device)
+    q_start = out.data_ptr()
+    seq_lens = q_start + 4 * (n_req + 1)
+    positions = seq_lens + 4 * n_req
+    slots = positions + 4 * n_tokens
+    _launch(index, lib().tl_paged_plan, table, q_start, seq_lens, positions, slots, slots + 4 * n_tokens, before, new, free,
+            free_blocks.numel(), n_req, width, block_size, n_tokens)
+    return out.split_with_sizes((n_req + 1, n_req, n_tokens, n_tokens, 2))
 
 
 def qk_norm_rope(q_out, k_cache, v_cache, qkv, positions, slots, cos, sin, q_weight=None, k_weight=None,
@@ -281,25 +272,29 @@ def qk_norm_rope(q_out, k_cache, v_cache, qkv, positions, slots, cos, sin, q_wei
     ``positions`` / ``slots`` as paged_plan gives them, ``cos`` / ``sin``
     float32 [n_pos, rot_dim / 2].  Rows with a position outside the tables are
     left alone; rows without a page get their q only."""
-    import torch
-    c = _cache(k_cache, v_cache)
-    dev, f32 = k_cache.device, torch.float32
-    if q_out.dim() != 3 or q_out.shape[2] != c.head_dim or q_out.dtype != k_cache.dtype:
+    torch = _torch or _load()
+    c, index = _cache(k_cache, v_cache)
+    i32, f32 = torch.int32, torch.float32
+    if q_out.dim() != 3 or q_out.dtype is not k_cache.dtype:
         raise ValueError("q_out must be [n_tokens, n_heads, head_dim] in the cache's type")
     n, heads, hd = q_out.shape
-    if qkv.dim() != 2 or qkv.shape != (n, (heads + 2 * c.n_kv_heads) * hd) or (n and qkv.stride(1) != 1):
+    if hd != c.head_dim:
+        raise ValueError("q_out must be [n_tokens, n_heads, head_dim] in the cache's type")
+    if qkv.shape != (n, (heads + 2 * c.n_kv_heads) * hd):
         raise ValueError("qkv must be [n_tokens, (n_heads + 2 n_kv_heads) * head_dim]")
-    if qkv.device != dev:
-        raise ValueError(f"qkv is on {qkv.device}, not {dev}")
+    stride, one = qkv.stride()
+    if n and one != 1:
+        raise ValueError("the heads of a token must be contiguous in qkv")
+    if qkv.get_device() != index:
+        raise ValueError(f"qkv is on {qkv.device}, not cuda:{index}")
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise ValueError("cos and sin must be [n_pos, rot_dim / 2]")
-    stride = qkv.stride(0) if n > 1 else qkv.shape[1]
-    _launch(dev, lib().tl_qk_norm_rope,
-            (_arg(q_out, q_out.dtype, dev, None, "q_out"), ctypes.byref(c), qkv.data_ptr(), _dtype(qkv), stride,
-             _arg(positions, torch.int32, dev, n, "positions"), _arg(slots, torch.int32, dev, n, "slots"),
-             _arg(cos, f32, dev, None, "cos"), _arg(sin, f32, dev, None, "sin"), cos.shape[0], 2 * cos.shape[1],
-             None if q_weight is None else _arg(q_weight, f32, dev, hd, "q_weight"),
-             None if k_weight is None else _arg(k_weight, f32, dev, hd, "k_weight"), eps, n, heads))
+    n_pos, half = cos.shape
+    _launch(index, lib().tl_qk_norm_rope, _arg(q_out, q_out.dtype, index, None, "q_out"), ctypes.byref(c), qkv.data_ptr(),
+            _dtype(qkv), stride if n > 1 else (heads + 2 * c.n_kv_heads) * hd, _arg(positions, i32, index, n, "positions"),
+            _arg(slots, i32, index, n, "slots"), _arg(cos, f32, index, None, "cos"), _arg(sin, f32, index, None, "sin"),
+            n_pos, 2 * half, None if q_weight is None else _arg(q_weight, f32, index, hd, "q_weight"),
+            None if k_weight is None else _arg(k_weight, f32, index, hd, "k_weight"), eps, n, heads)
 
 
 def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, scale=None, window: int = 0) -> None:
@@ -311,17 +306,19 @@ def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, sc
     defaults to 1 / sqrt(head_dim); ``window`` > 0 attends to that many last
     positions.  A query that attends to nothing gets zeros; rows of no sequence
     are left as they were."""
-    import torch
-    c = _cache(k_cache, v_cache)
-    dev, i32 = k_cache.device, torch.int32
-    if q.dim() != 3 or q.shape[2] != c.head_dim or q.dtype != k_cache.dtype or q.shape != out.shape \
-            or out.dtype != q.dtype:
+    torch = _torch or _load()
+    c, index = _cache(k_cache, v_cache)
+    i32, dtype = torch.int32, q.dtype
+    if q.dim() != 3 or dtype is not k_cache.dtype or q.shape != out.shape:
         raise ValueError("q and out must be [n_tokens, n_heads, head_dim] in the cache's type")
     n, heads, hd = q.shape
-    if n and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != hd)):
+    stride, of_head, one = q.stride()
+    if hd != c.head_dim or out.dtype is not dtype:
+        raise ValueError("q and out must be [n_tokens, n_heads, head_dim] in the cache's type")
+    if n and (one != 1 or (heads > 1 and of_head != hd)):
         raise ValueError("the heads of a token must be contiguous in q")
-    if q.device != dev:
-        raise ValueError(f"q is on {q.device}, not {dev}")
+    if q.get_device() != index:
+        raise ValueError(f"q is on {q.device}, not cuda:{index}")
     if block_table.dim() != 2 or window < 0:
         raise ValueError("block_table must be [n_seq, max_blocks] and window not negative")
     n_seq, width = block_table.shape
@@ -334,12 +331,11 @@ def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, sc
         if len(_WORKSPACE) >= 4096:
             _WORKSPACE.clear()
         need = _WORKSPACE[key] = size.value
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _launch(dev, L.tl_paged_attention,
-            (_arg(out, out.dtype, dev, None, "out"), q.data_ptr(), q.stride(0) if n > 1 else heads * hd, cache,
-             _arg(block_table, i32, dev, None, "block_table"), width, _arg(q_start, i32, dev, n_seq + 1, "q_start"),
-             _arg(seq_lens, i32, dev, n_seq, "seq_lens"), n_seq, n, heads, hd ** -0.5 if scale is None else scale, window,
-             ws.data_ptr(), need))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch(index, L.tl_paged_attention, _arg(out, dtype, index, None, "out"), q.data_ptr(),
+            stride if n > 1 else heads * hd, cache, _arg(block_table, i32, index, None, "block_table"), width,
+            _arg(q_start, i32, index, n_seq + 1, "q_start"), _arg(seq_lens, i32, index, n_seq, "seq_lens"), n_seq, n, heads,
+            hd ** -0.5 if scale is None else scale, window, ws.data_ptr(), need)
 
 
 _WORKSPACE = {}  # the workspace's size by type, heads and numbers of rows and sequences
@@ -351,18 +347,21 @@ def sample_rows(logits, r, temperature, top_k=None, top_p=None, min_p=None):
     ``r`` in [0, 1), ``temperature`` (<= 0: sample_max), and optionally
     ``top_k`` (int32; <= 0: off), ``top_p`` (>= 1: off) and ``min_p`` (<= 0:
     off), applied in that order.  Returns the indexes, an int32 tensor [n_rows]."""
-    import torch
-    if logits.dim() != 2 or (logits.shape[0] and logits.stride(1) != 1 and logits.shape[1] > 1):
+    torch = _torch or _load()
+    if logits.dim() != 2:
         raise ValueError("logits must be [n_rows, n] with contiguous rows")
-    if not logits.is_cuda:
-        raise ValueError("ops take CUDA tensors")
     rows, n = logits.shape
-    dev, f32 = logits.device, torch.float32
-    ptrs = (_arg(r, f32, dev, rows, "r"), _arg(temperature, f32, dev, rows, "temperature"),
-            None if top_k is None else _arg(top_k, torch.int32, dev, rows, "top_k"),
-            None if top_p is None else _arg(top_p, f32, dev, rows, "top_p"),
-            None if min_p is None else _arg(min_p, f32, dev, rows, "min_p"))
-    out = torch.empty(rows, dtype=torch.int32, device=dev)
-    _launch(dev, lib().tl_sample_rows, (out.data_ptr(), logits.data_ptr(), _dtype(logits),
-                                        logits.stride(0) if rows > 1 else n, rows, n, *ptrs))
+    stride, one = logits.stride()
+    if rows and n > 1 and one != 1:
+        raise ValueError("logits must be [n_rows, n] with contiguous rows")
+    index, f32, i32 = logits.get_device(), torch.float32, torch.int32
+    if index < 0:
+        raise ValueError("ops take CUDA tensors")
+    draws, temps = _arg(r, f32, index, rows, "r"), _arg(temperature, f32, index, rows, "temperature")
+    k = None if top_k is None else _arg(top_k, i32, index, rows, "top_k")
+    p = None if top_p is None else _arg(top_p, f32, index, rows, "top_p")
+    m = None if min_p is None else _arg(min_p, f32, index, rows, "min_p")
+    out = torch.empty(rows, dtype=i32, device=logits.device)
+    _launch(index, lib().tl_sample_rows, out.data_ptr(), logits.data_ptr(), _dtype(logits), stride if rows > 1 else n, rows, n,
+            draws, temps, k, p, m)
     return out
