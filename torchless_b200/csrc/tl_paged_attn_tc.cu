@@ -91,6 +91,40 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(y));
     return y != 0;
 }
+// Four products of 16 keys (or dims) each.  Addresses in tensor memory, the instruction descriptor and the upper
+// halves of the operand descriptors are constants, so that what an instruction takes from registers is the lower
+// half of one or two descriptors: moving all of them cost more time than the products.
+template <uint32_t D, uint32_t ID, uint32_t HI>
+__device__ __forceinline__ void mma4_ss(uint32_t a, uint32_t b, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %2, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 da, {%0, %5};\n\tmov.b64 db, {%1, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%3], da, db, %4, p;\n\t"
+        "add.u32 x, %0, 2;\n\tadd.u32 y, %1, 2;\n\tmov.b64 da, {x, %5};\n\tmov.b64 db, {y, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%3], da, db, %4, q;\n\t"
+        "add.u32 x, %0, 4;\n\tadd.u32 y, %1, 4;\n\tmov.b64 da, {x, %5};\n\tmov.b64 db, {y, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%3], da, db, %4, q;\n\t"
+        "add.u32 x, %0, 6;\n\tadd.u32 y, %1, 6;\n\tmov.b64 da, {x, %5};\n\tmov.b64 db, {y, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%3], da, db, %4, q;\n\t}" ::"r"(a),
+        "r"(b), "r"(acc), "r"(D), "r"(ID), "r"(HI));
+}
+template <uint32_t D, uint32_t A, uint32_t ID, uint32_t HI>
+__device__ __forceinline__ void mma4_ts(uint32_t b, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 y;\n\t.reg .b64 db;\n\t"
+        "setp.ne.b32 p, %1, 0;\n\tsetp.eq.b32 q, 0, 0;\n\t"
+        "mov.b64 db, {%0, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%2], [%5], db, %3, p;\n\t"
+        "add.u32 y, %0, 128;\n\tmov.b64 db, {y, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%2], [%6], db, %3, q;\n\t"
+        "add.u32 y, %0, 256;\n\tmov.b64 db, {y, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%2], [%7], db, %3, q;\n\t"
+        "add.u32 y, %0, 384;\n\tmov.b64 db, {y, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%2], [%8], db, %3, q;\n\t}" ::"r"(b),
+        "r"(acc), "r"(D), "r"(ID), "r"(HI), "r"(A), "r"(A + 8), "r"(A + 16), "r"(A + 24));
+}
+
 __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
     return bar_spin_ab(b, parity, abort_flag);
 }
@@ -223,8 +257,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(FULL, *tmem_slot, 0);
-    const uint32_t tS = tmem, tO = tmem + 256;  // S_i at + 128 i, O_i at + 128 i
+    // All 512 columns are this block's, so they begin at 0.  S_i at 128 i, O_i at 256 + 128 i.
+    constexpr uint32_t tmem = 0, tS = 0, kTO = 256, tO = kTO;
+    if (*tmem_slot != tmem) *abort_flag = 1;
 
     auto fail = [&] { *abort_flag = 1; };
     // waits poll: the hand-offs here are short and frequent
@@ -267,74 +302,100 @@ __global__ void __launch_bounds__(kThreads, 1)
         // every copy issued lands before the block ends
         for (uint32_t k = n > NST ? n - NST : 0; k < n; k++) bar_wait(&full[k % NST], (k / NST) & 1);
     } else if (warp == 9) {
-        // ---- MMA: the whole warp keeps step, so that addresses and descriptors stay in uniform registers;
-        // one elected lane issues ----
-        constexpr uint32_t id_s = idesc<T>(kKB, false), id_o = idesc<T>(HD, true);
-        const uint64_t dq = sdesc_k128(su32(sQ)), dk = sdesc_k128(su32(ring)), dv = sdesc_n128(su32(ring), S::PANEL);
-        constexpr uint32_t STEP = S::STAGE >> 4, PSTEP = S::PANEL >> 4;
-        uint32_t n0 = 0;              // loads before this tile
-        uint32_t nq = 0, np = 0;      // phases of the streams' barriers
-        auto wait_all = [&](uint64_t* b, uint32_t parity) { return __all_sync(FULL, wait(b, parity)); };
-        bool ok = true;
+        if (elect_one()) {
+            // ---- MMA: one thread for both streams, so that they stay half a step apart and do not take the
+            // exponentials at the same time.  It has to be quick between its waits: what it queues in the matrix
+            // unit lasts for two or three products. ----
+            constexpr uint32_t id_s = idesc<T>(kKB, false), id_o = idesc<T>(HD, true);
+            constexpr uint32_t kHi = (1024 >> 4) | (1u << 14) | (2u << 29);  // stride offset, version, SWIZZLE_128B
+            constexpr uint32_t STEP = S::STAGE >> 4, PSTEP = S::PANEL >> 4;
+            const uint32_t lq = static_cast<uint32_t>(sdesc_k128(su32(sQ))), lk = static_cast<uint32_t>(sdesc_k128(su32(ring))),
+                           lv = static_cast<uint32_t>(sdesc_n128(su32(ring), S::PANEL));
+            uint32_t n0 = 0;                         // loads before this tile
+            uint32_t nq[2] = {0, 0}, np[2] = {0, 0}; // phases of q_full and p_full
+            bool ok = true;
 #pragma unroll 1
-        for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
-            const Part p = part_of(a, c);
-            const int stride = p.stride();
-            // begin: the first scores of both streams; then values and next scores, in turn
-#pragma unroll 1
-            for (int j = p.jb - stride; ok && j < p.je; j += stride)
-#pragma unroll 1
+            for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
+                const Part p = part_of(a, c);
+                const uint32_t step = 2 * p.stride();
+                // the stages and phases of each stream's next K and V
+                uint32_t ks[2], kp[2], vs[2], vp[2];
+                int nb[2];  // key tiles of the streams
+#pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const int ji = p.two ? j : j + i;
-                    const bool start = j < p.jb;
-                    if (!p.active(i) || ji >= p.end(i)) continue;
-                    if (start) {
-                        if (!(ok = wait_all(&q_full[i], (nq >> i) & 1))) break;
-                        nq ^= 1u << i;
-                    } else {  // O_i (+)= P_i V_j
-                        const uint32_t n = n0 + 2 * (ji - p.jb) + 1, st = n % NST;
-                        if (!(ok = wait_all(&full[st], (n / NST) & 1))) break;
-                        const uint64_t db = dv + st * STEP;
-                        const uint32_t first = ji != p.begin(i);
-#pragma unroll
-                        for (int hf = 0; hf < 2; hf++) {
-                            if (!(ok = wait_all(&p_full[2 * i + hf], (np >> i) & 1))) break;
-                            tc_fence_after();
-                            if (elect_one()) {
-#pragma unroll
-                                for (int k = 4 * hf; k < 4 * hf + 4; k++)
-                                    umma_f16_ts(tO + 128 * i, tS + 128 * i + 8 * k, db + 128 * k, id_o, k == 0 ? first : 1u);
-                                if (hf && (!p.two || i == 1)) umma_commit(&empty[st]);  // V_j is read
-                            }
-                        }
-                        if (!ok) break;
-                        np ^= 1u << i;
-                    }
-                    const int jn = start ? p.begin(i) : ji + stride;
-                    if (jn < p.end(i)) {  // S_i = Q_i K_j^T
-                        const uint32_t n = n0 + 2 * (jn - p.jb), st = n % NST;
-                        if (!(ok = wait_all(&full[st], (n / NST) & 1))) break;
-                        tc_fence_after();
-                        const uint64_t da = dq + i * STEP, db = dk + st * STEP;
-                        if (elect_one()) {
-#pragma unroll
-                            for (int d = 0; d < S::PANELS; d++)
-#pragma unroll
-                                for (int k = 0; k < 4; k++)
-                                    umma_f16(tS + 128 * i, da + d * PSTEP + 2 * k, db + d * PSTEP + 2 * k, id_s, (d | k) != 0);
-                            umma_commit(&s_full[i]);
-                            if (!p.two || i == 1) umma_commit(&empty[st]);  // K_j is read (stream 1 is its last reader)
-                        }
-                    } else if (elect_one()) {
-                        umma_commit(&o_full[i]);
-                    }
+                    const uint32_t k = n0 + 2 * (p.begin(i) - p.jb);
+                    ks[i] = k % NST;
+                    kp[i] = (k / NST) & 1;
+                    vs[i] = (k + 1) % NST;
+                    vp[i] = ((k + 1) / NST) & 1;
+                    nb[i] = max(0, p.two ? p.end(i) - p.jb : (p.je - p.jb + 1 - i) / 2);
                 }
-            n0 += 2 * (p.je - p.jb);
+                auto advance = [&](uint32_t& st, uint32_t& ph) {
+                    st += step;
+                    if (st >= NST) {
+                        st -= NST;
+                        ph ^= 1;
+                    }
+                };
+                const bool both = p.two;  // stream 0 has waited for what stream 1 reads; stream 1 frees it
+                auto scores = [&](auto stream, bool known) -> bool {  // S_i = Q_i K^T
+                    constexpr int i = decltype(stream)::value;
+                    if (!known && !wait(&full[ks[i]], kp[i])) return false;
+                    tc_fence_after();
+                    const uint32_t x = lq + i * STEP, y = lk + ks[i] * STEP;
+#pragma unroll
+                    for (int d = 0; d < S::PANELS; d++) mma4_ss<128 * i, id_s, kHi>(x + d * PSTEP, y + d * PSTEP, d);
+                    umma_commit(&s_full[i]);
+                    if (!both || i == 1) umma_commit(&empty[ks[i]]);
+                    advance(ks[i], kp[i]);
+                    return true;
+                };
+                auto values = [&](auto stream, bool known, uint32_t acc) -> bool {  // O_i (+)= P_i V
+                    constexpr int i = decltype(stream)::value;
+                    if (!known && !wait(&full[vs[i]], vp[i])) return false;
+                    const uint32_t y = lv + vs[i] * STEP;
+                    if (!wait(&p_full[2 * i], np[i])) return false;
+                    tc_fence_after();
+                    mma4_ts<kTO + 128 * i, 128 * i, id_o, kHi>(y, acc);
+                    if (!wait(&p_full[2 * i + 1], np[i])) return false;
+                    tc_fence_after();
+                    mma4_ts<kTO + 128 * i, 128 * i + 32, id_o, kHi>(y + 512, 1);
+                    np[i] ^= 1;
+                    if (!both || i == 1) umma_commit(&empty[vs[i]]);
+                    advance(vs[i], vp[i]);
+                    return true;
+                };
+                auto begin = [&](auto stream) {
+                    constexpr int i = decltype(stream)::value;
+                    if (!ok || nb[i] == 0) return;
+                    ok = wait(&q_full[i], nq[i]);
+                    nq[i] ^= 1;
+                    ok = ok && scores(stream, both && i == 1 && nb[0] > 0);
+                };
+                auto turn = [&](auto stream, int j) {
+                    constexpr int i = decltype(stream)::value;
+                    if (!ok || j >= nb[i]) return;
+                    ok = values(stream, both && i == 1 && j < nb[0], j != 0);
+                    if (!ok) return;
+                    if (j + 1 < nb[i]) ok = scores(stream, both && i == 1 && j + 1 < nb[0]);
+                    else umma_commit(&o_full[i]);
+                };
+                constexpr std::integral_constant<int, 0> s0{};
+                constexpr std::integral_constant<int, 1> s1{};
+                begin(s0);
+                begin(s1);
+                const int nt = max(nb[0], nb[1]);
+#pragma unroll 1
+                for (int j = 0; ok && j < nt; j++) {
+                    turn(s0, j);
+                    turn(s1, j);
+                }
+                n0 += 2 * (p.je - p.jb);
+            }
+            if (!ok) fail();
+            umma_commit(drain);  // completes once every MMA issued above has
+            bar_wait(drain, 0);
         }
-        if (!ok) fail();
-        __syncwarp();
-        if (elect_one()) umma_commit(drain);  // completes once every MMA issued above has
-        bar_wait(drain, 0);
     } else {
         // ---- softmax and epilogue: thread = row r of stream i ----
         const int i = warp >> 2, r = (warp & 3) * 32 + lane;
@@ -422,19 +483,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_wait_st();
                     }
                     // the scores are read twice, 32 columns at a time: 128 of them do not fit beside the rest
-                    float mx[2] = {-INFINITY, -INFINITY};
-                    {
-                        uint32_t u[2][32];
-                        tmem_ld32_async(ts, u[0]);
+                    // The maximum, a quarter at a time, the first quarter last: it stays in registers for the weights.
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    uint32_t u[2][32];
+                    tmem_ld32_async(ts + 32, u[0]);
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            tmem_wait_ld();
-                            if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[(q + 1) & 1]);
+                    for (int x = 0; x < 4; x++) {
+                        tmem_wait_ld();
+                        if (x < 3) tmem_ld32_async(ts + 32 * ((x + 2) & 3), u[(x + 1) & 1]);
 #pragma unroll
-                            for (int e = 0; e < 32; e += 2)
-                                mx[(e / 2) & 1] = max3(mx[(e / 2) & 1], __uint_as_float(u[q & 1][e]), __uint_as_float(u[q & 1][e + 1]));
-                        }
+                        for (int e = 0; e < 32; e += 2)
+                            mx[(e / 2) & 3] = max3(mx[(e / 2) & 3], __uint_as_float(u[x & 1][e]), __uint_as_float(u[x & 1][e + 1]));
                     }
+                    mx[0] = fmaxf(mx[0], mx[1]);
+                    mx[1] = fmaxf(mx[2], mx[3]);
                     const float top = fmaxf(mx[0], mx[1]) * sl;
                     float f = 1.f;
                     if (top > m + kRescale || (m == -INFINITY && top > -INFINITY)) {
@@ -471,34 +533,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         fence_proxy_async();
                     }
-                    float sum[2] = {0.f, 0.f};
-                    {
-                        uint32_t u[2][32];
-                        tmem_ld32_async(ts, u[0]);
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    auto arrive = [&](int half) {  // half of the weights: the products of their keys may begin
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(&p_full[2 * i + half]);
+                    };
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            tmem_wait_ld();
-                            if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[(q + 1) & 1]);
-                            const uint32_t (&v)[32] = u[q & 1];
-                            uint32_t w[16];
+                    for (int q = 0; q < 4; q++) {
+                        if (q) tmem_wait_ld();
+                        if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[q & 1]);
+                        const uint32_t (&v)[32] = u[(q + 1) & 1];
+                        uint32_t w[16];
 #pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const float x = ex2(fmaf(__uint_as_float(v[2 * e]), sl, base));
-                                const float y = ex2(fmaf(__uint_as_float(v[2 * e + 1]), sl, base));
-                                sum[0] += x;
-                                sum[1] += y;
-                                w[e] = pack2(x, y, static_cast<T*>(nullptr));
-                            }
-                            tmem_st16_async(ts + 16 * q, w);  // over scores that have been read
-                            if (q & 1) {  // half of the weights: the products of their keys may begin
-                                tmem_wait_st();
-                                tc_fence_before();
-                                __syncwarp();
-                                if (lane == 0) bar_arrive(&p_full[2 * i + q / 2]);
-                            }
+                        for (int e = 0; e < 16; e++) {
+                            const float x = ex2(fmaf(__uint_as_float(v[2 * e]), sl, base));
+                            const float y = ex2(fmaf(__uint_as_float(v[2 * e + 1]), sl, base));
+                            sum[(2 * e) & 3] += x;
+                            sum[(2 * e + 1) & 3] += y;
+                            w[e] = pack2(x, y, static_cast<T*>(nullptr));
                         }
+                        if (q == 2) arrive(0);  // (stored a quarter ago: no waiting)
+                        tmem_st16_async(ts + 16 * q, w);  // over scores that have been read
                     }
-                    l += sum[0] + sum[1];
+                    arrive(1);
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 }
             }
             Cursor nc = c;
