@@ -7,7 +7,7 @@
 // rows of one kv head at a time, as two streams of 128 rows that share every
 // K / V tile:
 //   S_i[128 x 128] = Q_i K^T      tcgen05.mma, tensor memory
-//   P_i            = 2^(S_i scale - m_i)   one thread a row, 16-bit, over S_i
+//   P_i            = 2^(S_i scale - m_i)   two threads a row, 16-bit, over S_i
 //   O_i[128 x hd] += P_i V        tcgen05.mma, P_i from tensor memory
 // While the threads of one stream take exponentials, the matrix unit works for
 // the other.  A tile of at most 128 rows (the tail of a chunk, a single token
@@ -20,7 +20,9 @@
 //     the final O / l is exact all the same.
 //   - Persistent blocks with equal shares of the key tiles (tl_paged_attn.cuh);
 //     a row tile that two blocks share is joined by a second kernel.
-// Warps: 0-3 stream 0, 4-7 stream 1 (softmax, epilogue), 8 TMA, 9 MMA.
+// Warps: 0-7 stream 0, 8-15 stream 1 (softmax and epilogue: a row's first 64 keys and first columns by warps 0-3
+// of a stream, the rest by 4-7, which agree on the row's maximum through shared memory), 16 TMA, 17 MMA, 18 and 19
+// Q of stream 0 and 1: the next tile's, as soon as the last scores of this one are done.
 // Every mbarrier wait is bounded (~2 s): on expiry the roles stop, copies and
 // MMAs in flight drain, tensor memory is freed.
 #include <math.h>
@@ -37,7 +39,7 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 256, kHalf = 128, kKB = 128;
-constexpr int kWarps = 10, kThreads = kWarps * 32;
+constexpr int kWarps = 20, kThreads = kWarps * 32;
 constexpr float kRescale = 8.f;  // log2 units
 
 // One step: 256 rows x 128 keys, or (tiles of at most 128 rows) 128 rows x 256 keys.  Beginning and ending a
@@ -60,8 +62,8 @@ struct Shape {
     static constexpr int PANEL = kKB * 128;       // bytes of 64 columns of 128 rows
     static constexpr int STAGE = PANELS * PANEL;  // K or V of 128 keys
     static constexpr int NST = HD == 128 ? 5 : 10;
-    static constexpr size_t SMEM = 2 * static_cast<size_t>(STAGE) + static_cast<size_t>(NST) * STAGE + 256 +
-                                   2 * 2 * kHalf * 4 + 128;
+    static constexpr size_t SMEM = 2 * static_cast<size_t>(STAGE) + static_cast<size_t>(NST) * STAGE + 512 +
+                                   4 * kHalf * 4 + 16;
 };
 
 // K-major operand: rows of 64 columns (128 bytes), SWIZZLE_128B: sdesc_k128.
@@ -129,6 +131,17 @@ __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile in
     return bar_spin_ab(b, parity, abort_flag);
 }
 
+// All threads of a stream meet; whether `good` holds for all of them.
+__device__ __forceinline__ bool stream_sync(int i, bool good) {
+    uint32_t y;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(y)
+        : "r"(static_cast<uint32_t>(good)), "r"(1 + i)
+        : "memory");
+    return y != 0;
+}
+
 // The larger of three.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -153,6 +166,13 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st16_async(uint32_t taddr, const uint32_t* v) {
@@ -216,13 +236,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* empty = full + NST;
     uint64_t* s_full = empty + NST;  // [2] S_i written (and every MMA before it done)
     uint64_t* p_full = s_full + 2;   // [2][2] halves of P_i (64 keys) written: 4 warps
-    uint64_t* q_full = p_full + 4;   // [2] Q_i written: 4 warps
+    uint64_t* q_full = p_full + 4;   // [2] Q_i written
     uint64_t* o_full = q_full + 2;   // [2] the stream's last product done
-    uint64_t* xbar = o_full + 2;     // both streams' 8 warps
+    uint64_t* xbar = o_full + 2;     // both streams' 16 warps
     uint64_t* drain = xbar + 1;
-    static_assert((2 * 10 + 12) * 8 <= 256, "barriers");
-    float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + 256);  // [2][128] max, [2][128] sum
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xch + 4 * kHalf);
+    uint64_t* q_free = drain + 1;    // [2] the tile's last scores of stream i done
+    static_assert((2 * 10 + 14) * 8 <= 512, "barriers");
+    uint8_t* xch = reinterpret_cast<uint8_t*>(full) + 512;  // what the halves and streams of a row exchange
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xch + 2048);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     long long* ws = reinterpret_cast<long long*>(ring);  // the scan runs before the ring is used
 
@@ -241,15 +262,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(&s_full[i], 1);
             bar_init(&p_full[2 * i], 4);
             bar_init(&p_full[2 * i + 1], 4);
-            bar_init(&q_full[i], 4);
+            bar_init(&q_full[i], 1);
+            bar_init(&q_free[i], 1);
             bar_init(&o_full[i], 1);
         }
-        bar_init(xbar, 8);
+        bar_init(xbar, 16);
         bar_init(drain, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -265,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // waits poll: the hand-offs here are short and frequent
     auto wait = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || wait_slow(b, parity, abort_flag); };
 
-    if (warp == 8) {
+    if (warp == 16) {
         // ---- TMA: K_j, V_j of each key tile; lane = one page's rows of one panel ----
         const int rows = min(kKB, 1 << a.shift);  // rows of a copy
         const int pages = kKB / rows;
@@ -301,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) fail();
         // every copy issued lands before the block ends
         for (uint32_t k = n > NST ? n - NST : 0; k < n; k++) bar_wait(&full[k % NST], (k / NST) & 1);
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         if (elect_one()) {
             // ---- MMA: one thread for both streams, so that they stay half a step apart and do not take the
             // exponentials at the same time.  It has to be quick between its waits: what it queues in the matrix
@@ -338,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 };
                 const bool both = p.two;  // stream 0 has waited for what stream 1 reads; stream 1 frees it
-                auto scores = [&](auto stream, bool known) -> bool {  // S_i = Q_i K^T
+                auto scores = [&](auto stream, bool known, bool last) -> bool {  // S_i = Q_i K^T
                     constexpr int i = decltype(stream)::value;
                     if (!known && !wait(&full[ks[i]], kp[i])) return false;
                     tc_fence_after();
@@ -346,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int d = 0; d < S::PANELS; d++) mma4_ss<128 * i, id_s, kHi>(x + d * PSTEP, y + d * PSTEP, d);
                     umma_commit(&s_full[i]);
+                    if (last) umma_commit(&q_free[i]);
                     if (!both || i == 1) umma_commit(&empty[ks[i]]);
                     advance(ks[i], kp[i]);
                     return true;
@@ -359,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mma4_ts<kTO + 128 * i, 128 * i, id_o, kHi>(y, acc);
                     if (!wait(&p_full[2 * i + 1], np[i])) return false;
                     tc_fence_after();
-                    mma4_ts<kTO + 128 * i, 128 * i + 32, id_o, kHi>(y + 512, 1);
+                    mma4_ts<kTO + 128 * i, 128 * i + 64, id_o, kHi>(y + 512, 1);
                     np[i] ^= 1;
                     if (!both || i == 1) umma_commit(&empty[vs[i]]);
                     advance(vs[i], vp[i]);
@@ -370,14 +393,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok || nb[i] == 0) return;
                     ok = wait(&q_full[i], nq[i]);
                     nq[i] ^= 1;
-                    ok = ok && scores(stream, both && i == 1 && nb[0] > 0);
+                    ok = ok && scores(stream, both && i == 1 && nb[0] > 0, nb[i] == 1);
                 };
                 auto turn = [&](auto stream, int j) {
                     constexpr int i = decltype(stream)::value;
                     if (!ok || j >= nb[i]) return;
                     ok = values(stream, both && i == 1 && j < nb[0], j != 0);
                     if (!ok) return;
-                    if (j + 1 < nb[i]) ok = scores(stream, both && i == 1 && j + 1 < nb[0]);
+                    if (j + 1 < nb[i]) ok = scores(stream, both && i == 1 && j + 1 < nb[0], j + 2 == nb[i]);
                     else umma_commit(&o_full[i]);
                 };
                 constexpr std::integral_constant<int, 0> s0{};
@@ -396,35 +419,58 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit(drain);  // completes once every MMA issued above has
             bar_wait(drain, 0);
         }
+    } else if (warp >= 18) {
+        // ---- Q rows of stream i into the swizzled K-major panels: a row is CH pieces of 16 bytes, one a lane ----
+        const int i = warp - 18;
+        constexpr int CH = HD / 8, RPI = 32 / CH;
+        const int d = lane % CH;
+        uint8_t* dst = sQ + i * S::STAGE + (d / 8) * S::PANEL;
+        uint32_t loaded = 0;
+        bool ok = true;
+#pragma unroll 1
+        for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
+            const Part p = part_of(a, c);
+            if (!p.active(i)) continue;
+            if (loaded && !__all_sync(FULL, wait(&q_free[i], (loaded - 1) & 1))) {
+                ok = false;
+                break;
+            }
+            const int row0 = p.two ? i * kHalf : 0;
+#pragma unroll 1
+            for (int rr = lane / CH; rr < kHalf; rr += RPI) {
+                int tok, h;
+                row_of(a, c, row0 + rr, tok, h);
+                const T* src = static_cast<const T*>(a.q) + static_cast<size_t>(tok) * a.q_stride + static_cast<size_t>(h) * HD + 8 * d;
+                const uint32_t bytes = row0 + rr < c.t.nrows ? 16u : 0u;  // (a row that does not exist: zeros)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(su32(dst + sw128(rr, d & 7))), "l"(src), "r"(bytes)
+                             : "memory");
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&q_full[i]);
+            loaded++;
+        }
+        if (!ok) fail();
     } else {
-        // ---- softmax and epilogue: thread = row r of stream i ----
-        const int i = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tS + 128 * i + lane_off, to = tO + 128 * i + lane_off;
+        // ---- softmax and epilogue: thread = half hf of row r of stream i.  A thread whose wait fails goes on
+        // through the loops' barriers, doing no work, so that the others find it there ----
+        const int i = warp >> 3, hf = (warp >> 2) & 1, quad = (warp & 3) * 32, r = quad + lane;
+        const uint32_t lane_off = static_cast<uint32_t>(quad) << 16;
+        const uint32_t ts = tS + 128 * i + 64 * hf + lane_off, to = tO + 128 * i + lane_off;
         const float scale = a.scale * 1.4426950408889634f;  // log2 units
         const float sl = fabsf(scale);
+        // [stream][half][row]: the maxima of a block (read before its weights, which the next block's scores wait
+        // for: one buffer is enough), at a tile's end the sums
+        float* xl = reinterpret_cast<float*>(xch);
         uint32_t n0 = 0, ns = 0, no = 0, nx = 0;
         bool ok = true, first_tile = true, go = true;
-        // a tile's Q rows are fetched before the epilogue of the tile before: 16 bytes a lane, whole rows
-        constexpr int CH = HD / 8, RPI = 32 / CH, QL = 32 / RPI;  // pieces of a row, rows a load, loads
-        uint4 qv[QL];
-        auto fetch_q = [&](const Cursor& t) {
-            const bool two = t.t.nrows > kHalf;
-            const int rw = two ? i * kHalf + r : r;
-            int tk, hh;
-            row_of(a, t, rw, tk, hh);
-            const unsigned long long mine = rw < t.t.nrows ? static_cast<unsigned long long>(tk) * a.q_stride +
-                                                                 static_cast<unsigned long long>(hh) * HD : ~0ull;
-#pragma unroll
-            for (int q = 0; q < QL; q++) {
-                const unsigned long long at = __shfl_sync(FULL, mine, q * RPI + lane / CH);
-                qv[q] = at != ~0ull ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at)[lane % CH]
-                                    : make_uint4(0, 0, 0, 0);
-            }
+        auto give_up = [&] {
+            ok = false;
+            fail();
         };
-        fetch_q(c);
 #pragma unroll 1
-        while (ok && go) {
+        for (; go; go = next_tile<ChunkPlan>(a, c), first_tile = false) {
             const Part p = part_of(a, c);
             const int row = p.two ? i * kHalf + r : r;  // of the tile
             const bool in = row < c.t.nrows;
@@ -435,69 +481,58 @@ __global__ void __launch_bounds__(kThreads, 1)
             attended(a, c.t.p0 + (tok - c.t.first), lo, hi);
             float m = -INFINITY, l = 0.f;
             if (act) {
-                // this warp's 32 Q rows into the swizzled K-major panels
-#pragma unroll
-                for (int q = 0; q < QL; q++) {
-                    const int rr = q * RPI + lane / CH, d = lane % CH;
-                    *reinterpret_cast<uint4*>(sQ + i * S::STAGE + (d / 8) * S::PANEL + sw128((warp & 3) * 32 + rr, d & 7)) = qv[q];
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&q_full[i]);
-                auto page_at = [&](int j) { return lane < kKB / 8 ? page_of(a, c.b, (p.kb0 + j) * kKB + 8 * lane) : 0; };
-                int pid_next = page_at(p.begin(i));
                 const int stride = p.stride();
-                for (int j = p.begin(i); j < p.end(i); j += stride) {
-                    const int key0 = (p.kb0 + j) * kKB;
+                auto page_at = [&](int j) { return lane < 8 ? page_of(a, c.b, (p.kb0 + j) * kKB + 64 * hf + 8 * lane) : 0; };
+                int pid_next = page_at(p.begin(i));
+#pragma unroll 1
+                for (int j = p.begin(i); j < p.end(i); j += stride, ns++) {
+                    const int key0 = (p.kb0 + j) * kKB + 64 * hf;  // of this half
                     const int pid = pid_next;
                     pid_next = j + stride < p.end(i) ? page_at(j + stride) : 0;
                     // every lane waits; the outcome is warp-uniform (tensor-memory access is warp-wide)
-                    if (!__all_sync(FULL, wait(&s_full[i], ns & 1))) {
-                        ok = false;
-                        break;
-                    }
-                    ns++;
-                    tc_fence_after();
-                    const uint32_t pages = __ballot_sync(FULL, pid >= 0);  // bit k: keys 8 k .. 8 k + 7 exist
-                    const bool edge = !__all_sync(FULL, !in || (key0 >= lo && key0 <= hi - kKB)) || pages != FULL;
-                    // Masked columns, and the sign of a negative scale, go into the scores in tensor memory first;
-                    // only the border tiles of a row need that, and the loops below stay short.
-                    if (edge || scale < 0.f) {
-                        const uint32_t sign = scale < 0.f ? 0x80000000u : 0u;
+                    bool good = ok && __all_sync(FULL, wait(&s_full[i], ns & 1));
+                    if (ok && !good) give_up();
+                    uint32_t u[32];
+                    float mx[2] = {-INFINITY, -INFINITY};
+                    if (good) {
+                        tc_fence_after();
+                        const uint32_t pages = __ballot_sync(FULL, pid >= 0);  // bit k: keys 8 k .. 8 k + 7 exist
+                        // Masked columns, and the sign of a negative scale, go into the scores in tensor memory first;
+                        // only the border tiles of a row need that, and the loops below stay short.
+                        if (!__all_sync(FULL, !in || (key0 >= lo && key0 <= hi - 64)) || pages != FULL || scale < 0.f) {
+                            const uint32_t sign = scale < 0.f ? 0x80000000u : 0u;
 #pragma unroll 1
-                        for (int q = 0; q < 4; q++) {
-                            const int k0 = key0 + 32 * q;
-                            const int x0 = max(0, min(32, lo - k0)), x1 = max(0, min(32, hi - k0));
-                            uint32_t keep = x1 > x0 ? (x1 == 32 ? ~0u : (1u << x1) - 1) & ~(x0 == 32 ? ~0u : (1u << x0) - 1) : 0u;
-                            const uint32_t pq = pages >> (4 * q);
-                            keep &= ((pq & 1) ? 0xffu : 0u) | ((pq & 2) ? 0xff00u : 0u) | ((pq & 4) ? 0xff0000u : 0u) |
-                                    ((pq & 8) ? 0xff000000u : 0u);
-                            uint32_t u[32];
+                            for (int q = 0; q < 2; q++) {
+                                const int k0 = key0 + 32 * q;
+                                const int x0 = max(0, min(32, lo - k0)), x1 = max(0, min(32, hi - k0));
+                                uint32_t keep = x1 > x0 ? (x1 == 32 ? ~0u : (1u << x1) - 1) & ~(x0 == 32 ? ~0u : (1u << x0) - 1) : 0u;
+                                const uint32_t pq = pages >> (4 * q);
+                                keep &= ((pq & 1) ? 0xffu : 0u) | ((pq & 2) ? 0xff00u : 0u) | ((pq & 4) ? 0xff0000u : 0u) |
+                                        ((pq & 8) ? 0xff000000u : 0u);
+                                tmem_ld32_async(ts + 32 * q, u);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; e++) u[e] = ((keep >> e) & 1) ? u[e] ^ sign : 0xff800000u;
+                                tmem_st16_async(ts + 32 * q, u);
+                                tmem_st16_async(ts + 32 * q + 16, u + 16);
+                            }
+                            tmem_wait_st();
+                        }
+                        // the maximum, the first 32 columns last: they stay in registers for the weights
+#pragma unroll
+                        for (int q = 1; q >= 0; q--) {
                             tmem_ld32_async(ts + 32 * q, u);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; e++) u[e] = ((keep >> e) & 1) ? u[e] ^ sign : 0xff800000u;
-                            tmem_st16_async(ts + 32 * q, u);
-                            tmem_st16_async(ts + 32 * q + 16, u + 16);
+                            for (int e = 0; e < 32; e += 2)
+                                mx[(e / 2) & 1] = max3(mx[(e / 2) & 1], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
                         }
-                        tmem_wait_st();
                     }
-                    // the scores are read twice, 32 columns at a time: 128 of them do not fit beside the rest
-                    // The maximum, a quarter at a time, the first quarter last: it stays in registers for the weights.
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    uint32_t u[2][32];
-                    tmem_ld32_async(ts + 32, u[0]);
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        tmem_wait_ld();
-                        if (x < 3) tmem_ld32_async(ts + 32 * ((x + 2) & 3), u[(x + 1) & 1]);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2)
-                            mx[(e / 2) & 3] = max3(mx[(e / 2) & 3], __uint_as_float(u[x & 1][e]), __uint_as_float(u[x & 1][e + 1]));
-                    }
-                    mx[0] = fmaxf(mx[0], mx[1]);
-                    mx[1] = fmaxf(mx[2], mx[3]);
-                    const float top = fmaxf(mx[0], mx[1]) * sl;
+                    const float own = fmaxf(mx[0], mx[1]) * sl;
+                    xl[(2 * i + hf) * 128 + r] = own;
+                    good = stream_sync(i, good);
+                    if (!good) continue;
+                    const float top = fmaxf(own, xl[(2 * i + (hf ^ 1)) * 128 + r]);
                     float f = 1.f;
                     if (top > m + kRescale || (m == -INFINITY && top > -INFINITY)) {
                         if (m != -INFINITY) f = ex2(m - top);
@@ -506,167 +541,147 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (__any_sync(FULL, f != 1.f)) {  // S of this tile is done, so the products before it are
                         l *= f;
 #pragma unroll 1
-                        for (int q = 0; q < HD / 32; q++) {
-                            float o[32];
-                            tmem_ld32(to + 32 * q, o);
+                        for (int q = 0; q < HD / 32; q++) {  // this half's columns
+                            uint32_t o[16];
+                            const uint32_t ta = to + hf * (HD / 2) + 16 * q;
+                            tmem_ld16_async(ta, o);
+                            tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] *= f;
-                            tmem_st32(to + 32 * q, o);
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16_async(ta, o);
                         }
+                        tmem_wait_st();
+                        tc_fence_before();
+                        // the first half's weights start the products: not before the other half's columns are scaled
+                        asm volatile("bar.sync %0, 64;" ::"r"(3 + 4 * i + (warp & 3)) : "memory");
                     }
                     // masked scores and rows that see nothing: 2^(-inf) = 0
                     const float base = m == -INFINITY ? 0.f : -m;
-                    if (key0 < c.t.lo || key0 > c.t.hi - kKB) {
+                    if (key0 < c.t.lo || key0 > c.t.hi - 64) {
                         // rows of V that no query attends to may hold anything: no 0 x NaN.  (Both streams
                         // write the same zeros; each before its own product.)
                         const uint32_t n = n0 + 2 * (j - p.jb) + 1, st = n % NST;
-                        if (!__all_sync(FULL, wait(&full[st], (n / NST) & 1))) {
-                            ok = false;
-                            break;
-                        }
-                        const int key = key0 + r;
+                        if (!__all_sync(FULL, wait(&full[st], (n / NST) & 1))) give_up();
+                        const int key = key0 + (r & 63), vr = 64 * hf + (r & 63);
                         if (key < c.t.lo || key >= c.t.hi) {
-#pragma unroll
-                            for (int d = 0; d < HD / 8; d++)
-                                *reinterpret_cast<uint4*>(ring + st * S::STAGE + (d / 8) * S::PANEL + sw128(r, d & 7)) =
+#pragma unroll 1
+                            for (int d = r >> 6; d < HD / 8; d += 2)
+                                *reinterpret_cast<uint4*>(ring + st * S::STAGE + (d / 8) * S::PANEL + sw128(vr, d & 7)) =
                                     make_uint4(0, 0, 0, 0);
                         }
                         fence_proxy_async();
                     }
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    auto arrive = [&](int half) {  // half of the weights: the products of their keys may begin
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(&p_full[2 * i + half]);
-                    };
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
+                    for (int q = 0; q < 2; q++) {
                         if (q) tmem_wait_ld();
-                        if (q < 3) tmem_ld32_async(ts + 32 * (q + 1), u[q & 1]);
-                        const uint32_t (&v)[32] = u[(q + 1) & 1];
                         uint32_t w[16];
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            const float x = ex2(fmaf(__uint_as_float(v[2 * e]), sl, base));
-                            const float y = ex2(fmaf(__uint_as_float(v[2 * e + 1]), sl, base));
+                            const float x = ex2(fmaf(__uint_as_float(u[2 * e]), sl, base));
+                            const float y = ex2(fmaf(__uint_as_float(u[2 * e + 1]), sl, base));
                             sum[(2 * e) & 3] += x;
                             sum[(2 * e + 1) & 3] += y;
                             w[e] = pack2(x, y, static_cast<T*>(nullptr));
                         }
-                        if (q == 2) arrive(0);  // (stored a quarter ago: no waiting)
+                        if (q == 0) tmem_ld32_async(ts + 32, u);
                         tmem_st16_async(ts + 16 * q, w);  // over scores that have been read
                     }
-                    arrive(1);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&p_full[2 * i + hf]);
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 }
             }
-            Cursor nc = c;
-            go = next_tile<ChunkPlan>(a, nc);
-            if (go) fetch_q(nc);
             if (act) {
-                if (ok && !__all_sync(FULL, wait(&o_full[i], no & 1))) ok = false;
+                if (ok && !__all_sync(FULL, wait(&o_full[i], no & 1))) give_up();
                 no++;
                 tc_fence_after();
             }
             n0 += 2 * (p.je - p.jb);
-            // ---- epilogue: this thread's columns [c0, c1) of the row's sum over the streams ----
-            float w0 = 1.f, w1 = 0.f, mt = m, lt = l;
-            const bool fold = !p.two && p.active(1);  // two streams of keys: add them
+            // ---- epilogue: this thread's columns of the row's sum over the halves and, if both have keys of the
+            // same rows, over the streams ----
+            const bool fold = !p.two && p.active(1);
+            stream_sync(i, true);  // the maxima have been read
+            xl[(2 * i + hf) * 128 + r] = l;
+            const bool good = stream_sync(i, ok);
+            float w0 = 1.f, w1 = 0.f, mt = m, lt = xl[2 * i * 128 + r] + xl[(2 * i + 1) * 128 + r];
             if (fold) {
-                xch[i * kHalf + r] = m;
-                xch[(2 + i) * kHalf + r] = l;
+                stream_sync(i, true);
+                xl[(2 * i + hf) * 128 + r] = hf ? lt : m;
                 __syncwarp();
                 if (lane == 0) bar_arrive(xbar);
-                if (!__all_sync(FULL, wait(xbar, nx & 1))) ok = false;
+                if (good && !__all_sync(FULL, wait(xbar, nx & 1))) give_up();
                 nx++;
-                const float m0 = xch[r], m1 = xch[kHalf + r];
+                const float m0 = xl[r], m1 = xl[256 + r];
                 mt = fmaxf(m0, m1);
                 w0 = mt == -INFINITY ? 1.f : ex2(m0 - mt);
                 w1 = mt == -INFINITY ? 1.f : ex2(m1 - mt);
-                lt = xch[2 * kHalf + r] * w0 + xch[3 * kHalf + r] * w1;
+                lt = xl[128 + r] * w0 + xl[384 + r] * w1;
                 tc_fence_after();
             }
-            if (!ok) break;
             const bool whole = c.s == 0 && c.end == c.steps;
-            const bool writer = p.two || fold || i == 0;
-            const int q0 = fold ? i * (HD / 64) : 0, q1 = fold ? (i + 1) * (HD / 64) : HD / 32;  // 32-column groups
+            const bool writer = good && (p.two || fold || i == 0);
+            const int c0 = fold ? (2 * i + hf) * (HD / 4) : hf * (HD / 2), c1 = c0 + (fold ? HD / 4 : HD / 2);  // columns
             float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * kRows * (HD + 4);
             if (writer) {
                 const float inv = lt != 0.f ? 1.f / lt : 0.f;
                 float z = lt * 0.f;  // NaN once a value is not finite
                 const bool t0 = fold || act;
                 const uint32_t ta = fold ? tO + lane_off : to;
-                uint8_t* stage_out = sQ + i * S::STAGE;
 #pragma unroll 1
-                for (int q = q0; q < q1; q++) {
-                    float o[32];
+                for (int col = c0; col < c1; col += 16) {
+                    uint32_t o[16];
                     if (t0) {
-                        tmem_ld32(ta + 32 * q, o);
+                        tmem_ld16_async(ta + col, o);
+                        tmem_wait_ld();
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = 0.f;
+                        for (int e = 0; e < 16; e++) o[e] = 0u;
                     }
                     if (fold) {
-                        float o1[32];
-                        tmem_ld32(tO + 128 + lane_off + 32 * q, o1);
+                        uint32_t o1[16];
+                        tmem_ld16_async(tO + 128 + lane_off + col, o1);
+                        tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = o[e] * w0 + o1[e] * w1;
+                        for (int e = 0; e < 16; e++)
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * w0 + __uint_as_float(o1[e]) * w1);
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) z = fmaf(o[e], 0.f, z);
-                    if (whole) {  // into this stream's Q tile, which every product has read
+                    for (int e = 0; e < 16; e++) z = fmaf(__uint_as_float(o[e]), 0.f, z);
+                    if (!in) continue;
+                    if (whole) {  // 32 bytes of this row
+                        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + h) * HD + col);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
+                        for (int e = 0; e < 2; e++) {
                             uint4 v;
                             uint32_t* vw = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
                             for (int k = 0; k < 4; k++)
-                                vw[k] = pack2(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv, static_cast<T*>(nullptr));
-                            *reinterpret_cast<uint4*>(stage_out + (q / 2) * S::PANEL + sw128(r, (4 * q + e) & 7)) = v;
+                                vw[k] = pack2(__uint_as_float(o[8 * e + 2 * k]) * inv, __uint_as_float(o[8 * e + 2 * k + 1]) * inv,
+                                              static_cast<T*>(nullptr));
+                            dst[e] = v;
                         }
-                    } else if (in) {  // [4-column group][row], so that a warp's stores are whole lines
-                        float4* dst = reinterpret_cast<float4*>(part) + kRows;
+                    } else {  // [4-column group][row], so that a warp's stores are whole lines
+                        uint4* dst = reinterpret_cast<uint4*>(part) + kRows;
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            dst[static_cast<size_t>(8 * q + e) * kRows + row] =
-                                make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        for (int e = 0; e < 4; e++)
+                            dst[static_cast<size_t>(col / 4 + e) * kRows + row] =
+                                make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
                 }
                 // not finite: a value that this row must not see may have met it as 0 x infinity (see tl_paged_attn.cu)
                 const bool redo = in && z != z;
                 if (whole) {
-                    // whole lines of the rows of this warp, 16 bytes a lane
-                    __syncwarp();
-                    const unsigned long long mine =
-                        in ? (static_cast<unsigned long long>(tok) * a.H + h) * HD + 32 * q0 : ~0ull;
-                    auto copy_out = [&](auto pieces) {
-                        constexpr int nch = decltype(pieces)::value;  // 16-byte pieces of a row
-#pragma unroll 4
-                        for (int k = 0; k < nch; k++) {
-                            const int rr = (32 / nch) * k + lane / nch, d = 4 * q0 + lane % nch;
-                            const unsigned long long at = __shfl_sync(FULL, mine, rr);
-                            const uint4 v = *reinterpret_cast<const uint4*>(stage_out + (d / 8) * S::PANEL +
-                                                                            sw128((warp & 3) * 32 + rr, d & 7));
-                            if (at != ~0ull) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + 8 * (lane % nch)) = v;
-                        }
-                    };
-                    if (fold) copy_out(std::integral_constant<int, HD / 16>());
-                    else copy_out(std::integral_constant<int, HD / 8>());
                     __syncwarp();
                     for (unsigned bad = __ballot_sync(FULL, redo); bad; bad &= bad - 1) {
                         const int src = __ffs(bad) - 1;
                         __syncwarp();
                         attend_row<T, HD>(a, c.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, h, src), lane);
                     }
-                } else if (in) {
-                    float* hd = part + 4 * row;  // {max, sum, redo, redo of the other columns}
-                    if (!fold || i == 0) {
-                        hd[0] = mt;
-                        hd[1] = lt;
-                        hd[2] = redo ? 1.f : 0.f;
-                    }
-                    if (!fold || i == 1) hd[3] = redo ? 1.f : 0.f;
+                } else if (in && hf == 0 && (!fold || i == 0)) {
+                    *reinterpret_cast<float2*>(part + 4 * row) = make_float2(mt, lt);
                 }
             }
             if (!whole && c.s == 0 && threadIdx.x == 0) {  // this block begins the tile: it says who has the rest
@@ -678,21 +693,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 hd.g = c.g;
                 heads[blockIdx.x] = hd;
             }
-            if (fold) {  // both have read the accumulators: the next tile may overwrite them
+            // Before the next tile's weights, which let products overwrite them: both halves, and (fold) both streams,
+            // have read the accumulators.
+            if (fold) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(xbar);
-                if (!__all_sync(FULL, wait(xbar, nx & 1))) ok = false;
+                if (good && !__all_sync(FULL, wait(xbar, nx & 1))) give_up();
                 nx++;
             }
-            c = nc;
-            first_tile = false;
+            tc_fence_before();
+            stream_sync(i, true);
         }
-        if (!ok) fail();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 17) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
@@ -717,13 +733,11 @@ __global__ void __launch_bounds__(256) k_attend_chunk_join(const __grid_constant
     const float4* p0 = reinterpret_cast<const float4*>(parts) + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
     const float4* p1 = reinterpret_cast<const float4*>(parts) + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;
     auto part = [&](int i) { return i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec; };
-    float M = -INFINITY, bad = 0.f;
+    __shared__ unsigned bad_rows;
+    if (threadIdx.x == 0) bad_rows = 0;
+    float M = -INFINITY;
     if (in)
-        for (int i = 0; i < h.parts; i++) {
-            const float4 s = part(i)[row];
-            M = fmaxf(M, s.x);
-            bad += s.z + s.w;
-        }
+        for (int i = 0; i < h.parts; i++) M = fmaxf(M, part(i)[row].x);
     float L = 0.f;
     float4 acc[G];
 #pragma unroll
@@ -731,7 +745,7 @@ __global__ void __launch_bounds__(256) k_attend_chunk_join(const __grid_constant
     if (in)
         for (int i = 0; i < h.parts; i++) {
             const float4* p = part(i);
-            const float4 s = p[row];
+            const float2 s = *reinterpret_cast<const float2*>(p + row);
             const float f = M == -INFINITY ? 1.f : ex2(s.x - M);
             L += s.y * f;
 #pragma unroll
@@ -745,8 +759,15 @@ __global__ void __launch_bounds__(256) k_attend_chunk_join(const __grid_constant
         }
     int tok, hh;
     row_of(a, c, row, tok, hh);
-    const unsigned again = __ballot_sync(FULL, in && bad > 0.f);
-    if (in && !(bad > 0.f)) {
+    float z = L * 0.f;  // NaN once a value is not finite: the row is done over
+#pragma unroll
+    for (int g = 0; g < G; g++) z = fmaf(acc[g].x, 0.f, fmaf(acc[g].y, 0.f, fmaf(acc[g].z, 0.f, fmaf(acc[g].w, 0.f, z))));
+    const unsigned mine = __ballot_sync(FULL, in && z != z);
+    __syncthreads();
+    if (lane == 0 && mine) atomicOr(&bad_rows, mine);
+    __syncthreads();
+    const unsigned again = bad_rows;
+    if (in && !((again >> lane) & 1)) {
         const float inv = L != 0.f ? 1.f / L : 0.f;
         uint2* dst = reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD) + warp * G;
 #pragma unroll
