@@ -715,71 +715,87 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the parts of the tile that block blockIdx.x began (part i > 0: the first tile of block blockIdx.x + i).
-// Block y takes 32 rows: lane = row, warp = one 8th of the columns.
+// Block y takes 32 rows.  Reading, lane = row and warp = one 8th of the columns, as the parts lie; writing, a warp a
+// row, through shared memory.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) k_attend_chunk_join(const __grid_constant__ AttendArgs a, const Head* heads, const float* parts) {
+    constexpr int G = HD / 4 / 8;  // 4-column groups of a warp
+    __shared__ float4 rows[32][HD / 4 + 1];
+    __shared__ unsigned bad_rows;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) bad_rows = 0;
     pdl_wait();
     const Head h = heads[blockIdx.x];
     if (h.parts == 0) return;
     Cursor c;
     c.g = h.g;
     c.t = tile_of(a, h.b, h.rt, kRows);
-    if (static_cast<int>(blockIdx.y) * 32 >= c.t.nrows) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.y * 32 + lane;
+    const int row0 = blockIdx.y * 32, row = row0 + lane;
+    if (row0 >= c.t.nrows) return;
     const bool in = row < c.t.nrows;
     constexpr size_t rec = static_cast<size_t>(kRows) * (HD / 4 + 1);  // float4s of a part
-    constexpr int G = HD / 4 / 8;                                      // 4-column groups of a warp
     const float4* p0 = reinterpret_cast<const float4*>(parts) + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
     const float4* p1 = reinterpret_cast<const float4*>(parts) + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;
-    auto part = [&](int i) { return i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec; };
-    __shared__ unsigned bad_rows;
-    if (threadIdx.x == 0) bad_rows = 0;
-    float M = -INFINITY;
-    if (in)
-        for (int i = 0; i < h.parts; i++) M = fmaxf(M, part(i)[row].x);
-    float L = 0.f;
+    float M = -INFINITY, L = 0.f;
     float4 acc[G];
 #pragma unroll
     for (int g = 0; g < G; g++) acc[g] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (in)
-        for (int i = 0; i < h.parts; i++) {
-            const float4* p = part(i);
-            const float2 s = *reinterpret_cast<const float2*>(p + row);
-            const float f = M == -INFINITY ? 1.f : ex2(s.x - M);
-            L += s.y * f;
+    if (in) {
+#pragma unroll 1
+        for (int i0 = 0; i0 < h.parts; i0 += 2) {  // two parts' loads at a time
+            float2 s[2];
+            float4 v[2][G];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int i = i0 + k;
+                if (i < h.parts) {
+                    const float4* p = i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec;
+                    s[k] = *reinterpret_cast<const float2*>(p + row);
+#pragma unroll
+                    for (int g = 0; g < G; g++) v[k][g] = p[static_cast<size_t>(1 + warp * G + g) * kRows + row];
+                } else {
+                    s[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                    for (int g = 0; g < G; g++) v[k][g] = make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+            const float mx = fmaxf(M, fmaxf(s[0].x, s[1].x));
+            const float f = mx == -INFINITY ? 1.f : ex2(M - mx), f0 = mx == -INFINITY ? 1.f : ex2(s[0].x - mx),
+                        f1 = mx == -INFINITY ? 1.f : ex2(s[1].x - mx);
+            M = mx;
+            L = L * f + s[0].y * f0 + s[1].y * f1;
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                const float4 v = p[static_cast<size_t>(1 + warp * G + g) * kRows + row];
-                acc[g].x += v.x * f;
-                acc[g].y += v.y * f;
-                acc[g].z += v.z * f;
-                acc[g].w += v.w * f;
+                acc[g].x = acc[g].x * f + v[0][g].x * f0 + v[1][g].x * f1;
+                acc[g].y = acc[g].y * f + v[0][g].y * f0 + v[1][g].y * f1;
+                acc[g].z = acc[g].z * f + v[0][g].z * f0 + v[1][g].z * f1;
+                acc[g].w = acc[g].w * f + v[0][g].w * f0 + v[1][g].w * f1;
             }
         }
-    int tok, hh;
-    row_of(a, c, row, tok, hh);
+    }
     float z = L * 0.f;  // NaN once a value is not finite: the row is done over
+    const float inv = L != 0.f ? 1.f / L : 0.f;
 #pragma unroll
-    for (int g = 0; g < G; g++) z = fmaf(acc[g].x, 0.f, fmaf(acc[g].y, 0.f, fmaf(acc[g].z, 0.f, fmaf(acc[g].w, 0.f, z))));
+    for (int g = 0; g < G; g++) {
+        z = fmaf(acc[g].x, 0.f, fmaf(acc[g].y, 0.f, fmaf(acc[g].z, 0.f, fmaf(acc[g].w, 0.f, z))));
+        rows[lane][warp * G + g] = make_float4(acc[g].x * inv, acc[g].y * inv, acc[g].z * inv, acc[g].w * inv);
+    }
     const unsigned mine = __ballot_sync(FULL, in && z != z);
     __syncthreads();
     if (lane == 0 && mine) atomicOr(&bad_rows, mine);
     __syncthreads();
-    const unsigned again = bad_rows;
-    if (in && !((again >> lane) & 1)) {
-        const float inv = L != 0.f ? 1.f / L : 0.f;
-        uint2* dst = reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD) + warp * G;
-#pragma unroll
-        for (int g = 0; g < G; g++)
-            dst[g] = make_uint2(pack2(acc[g].x * inv, acc[g].y * inv, static_cast<T*>(nullptr)),
-                                pack2(acc[g].z * inv, acc[g].w * inv, static_cast<T*>(nullptr)));
-    }
-    if (warp == 0)
-        for (unsigned b = again; b; b &= b - 1) {
-            const int src = __ffs(b) - 1;
-            attend_row<T, HD>(a, h.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, hh, src), lane);
+#pragma unroll 1
+    for (int rr = warp; rr < 32 && row0 + rr < c.t.nrows; rr += 8) {
+        int tok, hh;
+        row_of(a, c, row0 + rr, tok, hh);
+        if ((bad_rows >> rr) & 1) {
+            attend_row<T, HD>(a, h.b, tok, hh, lane);
+        } else if (lane < HD / 4) {
+            const float4 v = rows[rr][lane];
+            reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD)[lane] =
+                make_uint2(pack2(v.x, v.y, static_cast<T*>(nullptr)), pack2(v.z, v.w, static_cast<T*>(nullptr)));
         }
+    }
 }
 
 template <typename T, int HD>
