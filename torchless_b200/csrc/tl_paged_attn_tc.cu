@@ -131,6 +131,10 @@ __device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile in
     return bar_spin_ab(b, parity, abort_flag);
 }
 
+__device__ __noinline__ bool doze_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+    return bar_wait_ab(b, parity, abort_flag);
+}
+
 // All threads of a stream meet; whether `good` holds for all of them.
 __device__ __forceinline__ bool stream_sync(int i, bool good) {
     uint32_t y;
@@ -286,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto fail = [&] { *abort_flag = 1; };
     // waits poll: the hand-offs here are short and frequent
     auto wait = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || wait_slow(b, parity, abort_flag); };
+    auto doze = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || doze_slow(b, parity, abort_flag); };
 
     if (warp == 16) {
         // ---- TMA: K_j, V_j of each key tile; lane = one page's rows of one panel ----
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int kv = 0; kv < 2; kv++) {
                     const uint32_t st = n % NST;
-                    if (!__all_sync(FULL, n < NST || wait(&empty[st], (n / NST - 1) & 1))) {
+                    if (!__all_sync(FULL, n < NST || doze(&empty[st], (n / NST - 1) & 1))) {
                         ok = false;
                         break;
                     }
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (bool go = true; ok && go; go = next_tile<ChunkPlan>(a, c)) {
             const Part p = part_of(a, c);
             if (!p.active(i)) continue;
-            if (loaded && !__all_sync(FULL, wait(&q_free[i], (loaded - 1) & 1))) {
+            if (loaded && !__all_sync(FULL, doze(&q_free[i], (loaded - 1) & 1))) {
                 ok = false;
                 break;
             }
@@ -490,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int pid = pid_next;
                     pid_next = j + stride < p.end(i) ? page_at(j + stride) : 0;
                     // every lane waits; the outcome is warp-uniform (tensor-memory access is warp-wide)
-                    bool good = ok && __all_sync(FULL, wait(&s_full[i], ns & 1));
+                    bool good = ok && __all_sync(FULL, doze(&s_full[i], ns & 1));
                     if (ok && !good) give_up();
                     uint32_t u[32];
                     float mx[2] = {-INFINITY, -INFINITY};
@@ -595,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (act) {
-                if (ok && !__all_sync(FULL, wait(&o_full[i], no & 1))) give_up();
+                if (ok && !__all_sync(FULL, doze(&o_full[i], no & 1))) give_up();
                 no++;
                 tc_fence_after();
             }
