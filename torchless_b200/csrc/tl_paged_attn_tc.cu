@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool both = p.two;  // stream 0 has waited for what stream 1 reads; stream 1 frees it
                 auto scores = [&](auto stream, bool known, bool last) -> bool {  // S_i = Q_i K^T
                     constexpr int i = decltype(stream)::value;
-                    if (!known && !wait(&full[ks[i]], kp[i])) return false;
+                    if (!known && !doze(&full[ks[i]], kp[i])) return false;
                     tc_fence_after();
                     const uint32_t x = lq + i * STEP, y = lk + ks[i] * STEP;
 #pragma unroll
@@ -380,12 +380,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 auto values = [&](auto stream, bool known, uint32_t acc) -> bool {  // O_i (+)= P_i V
                     constexpr int i = decltype(stream)::value;
-                    if (!known && !wait(&full[vs[i]], vp[i])) return false;
+                    if (!known && !doze(&full[vs[i]], vp[i])) return false;
                     const uint32_t y = lv + vs[i] * STEP;
-                    if (!wait(&p_full[2 * i], np[i])) return false;
+                    if (!doze(&p_full[2 * i], np[i])) return false;
                     tc_fence_after();
                     mma4_ts<kTO + 128 * i, 128 * i, id_o, kHi>(y, acc);
-                    if (!wait(&p_full[2 * i + 1], np[i])) return false;
+                    if (!doze(&p_full[2 * i + 1], np[i])) return false;
                     tc_fence_after();
                     mma4_ts<kTO + 128 * i, 128 * i + 64, id_o, kHi>(y + 512, 1);
                     np[i] ^= 1;
