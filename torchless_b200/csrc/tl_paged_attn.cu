@@ -653,98 +653,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Joins the parts of the tile that block blockIdx.x began: part i > 0 is the first tile of block blockIdx.x + i.
-// Two warps a row (one for its even parts, one for the odd); lane = 4 or 2 dims.
-template <typename T, int HD, int R>
-__global__ void __launch_bounds__(kThreads) k_attend_join(const __grid_constant__ AttendArgs a, const Head* heads,
-                                                          const float* parts) {
-    constexpr int D = HD / 32;
-    __shared__ float half[kWarps / 2][32 * D + 2];
-    pdl_wait();
-    const Head h = heads[blockIdx.x];
-    if (h.parts == 0) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, odd = warp & 1;
-    Cursor c;
-    c.g = h.g;
-    c.t = tile_of(a, h.b, h.rt, R);
-    constexpr size_t rec = static_cast<size_t>(R) * (HD + 4);
-    const float* p0 = parts + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
-    const float* p1 = parts + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;  // parts 1 .. are 2 * rec apart
-    auto part = [&](int i, int row) { return (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4); };
-#pragma unroll 1
-    for (int row0 = 0; row0 < c.t.nrows; row0 += kWarps / 2) {
-        const int row = row0 + (warp >> 1);
-        float M = -INFINITY, bad = 0.f, L = 0.f, acc[D];
-#pragma unroll
-        for (int d = 0; d < D; d++) acc[d] = 0.f;
-        if (row < c.t.nrows) {
-#pragma unroll 1
-            for (int i0 = odd; i0 < h.parts; i0 += 16) {  // 8 parts at a time
-                float m[8], l[8], v[8][D], mx = M;
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const int i = i0 + 2 * k;
-                    m[k] = -INFINITY;
-                    l[k] = 0.f;
-#pragma unroll
-                    for (int d = 0; d < D; d++) v[k][d] = 0.f;
-                    if (i < h.parts) {
-                        const float* p = part(i, row);
-                        const float4 q = *reinterpret_cast<const float4*>(p);
-                        m[k] = q.x;
-                        l[k] = q.y;
-                        bad = fmaxf(bad, q.z);
-#pragma unroll
-                        for (int d = 0; d < D; d++) v[k][d] = p[4 + lane + 32 * d];
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 8; k++) mx = fmaxf(mx, m[k]);
-                const float f0 = mx == -INFINITY ? 1.f : ex2(M - mx);
-                L *= f0;
-#pragma unroll
-                for (int d = 0; d < D; d++) acc[d] *= f0;
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float f = mx == -INFINITY ? 1.f : ex2(m[k] - mx);
-                    L += l[k] * f;
-#pragma unroll
-                    for (int d = 0; d < D; d++) acc[d] += v[k][d] * f;
-                }
-                M = mx;
-            }
-        }
-        if (odd) {
-            float* x = half[warp >> 1];
-            if (lane == 0) {
-                x[0] = M;
-                x[1] = bad > 0.f ? NAN : L;  // (NaN: to be done over)
-            }
-#pragma unroll
-            for (int d = 0; d < D; d++) x[2 + lane + 32 * d] = acc[d];
-        }
-        __syncthreads();
-        if (!odd && row < c.t.nrows) {
-            const float* x = half[warp >> 1];
-            int tok, hh;
-            row_of(a, c, row, tok, hh);
-            const float mx = fmaxf(M, x[0]), f0 = mx == -INFINITY ? 1.f : ex2(M - mx), f1 = mx == -INFINITY ? 1.f : ex2(x[0] - mx);
-            if (bad > 0.f || x[1] != x[1]) {
-                attend_row<T, HD>(a, h.b, tok, hh, lane);
-            } else {
-                const float sum = L * f0 + x[1] * f1;
-                T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD;
-#pragma unroll
-                for (int d = 0; d < D; d++) {
-                    const float o = acc[d] * f0 + x[2 + lane + 32 * d] * f1;
-                    out[lane + 32 * d] = from_f32<T>(sum != 0.f ? o / sum : 0.f);
-                }
-            }
-        }
-        __syncthreads();
-    }
-}
-
 template <typename T, int HD, int R>
 tl_status run_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
     using S = Shape<T, HD>;
@@ -761,25 +669,15 @@ tl_status run_split(const AttendArgs& a, const tl_paged_cache* c, void* workspac
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeadBytes);
     k_attend_split<T, HD, R><<<grid, kThreads, S::SMEM, s>>>(mk, mv, a, heads, parts);
     TL_TRY(check_launch("paged_attention"));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_attend_join<T, HD, R>, a, static_cast<const Head*>(heads),
-                                   static_cast<const float*>(parts)));
-    return TL_OK;
+    return launch_join<T, HD, R>(a, heads, parts, grid, 1, s);
 }
 
 template <int HD>
 tl_status run_split_hd(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
     if (c->dtype == TL_F16) return run_split<__half, HD, 16>(a, c, workspace, s);
     if (c->dtype == TL_BF16) return run_split<__nv_bfloat16, HD, 16>(a, c, workspace, s);
-    // fp32: rows are paid for one by one, so no more of them than a decode step has
+    // fp32: rows are paid for one by one, so no more of them than a decode step has (64 x 4096 keys: 4 rows 339 us,
+    // as 16 882 us; 8 rows 244 us, as 16 454 us)
     const long long rows = static_cast<long long>(a.n_tokens) * a.group;
     if (a.group <= 4 && rows <= 4ll * a.n_seq) return run_split<float, HD, 4>(a, c, workspace, s);
     if (a.group <= 8 && rows <= 8ll * a.n_seq) return run_split<float, HD, 8>(a, c, workspace, s);
@@ -803,9 +701,12 @@ using namespace tl;
 using namespace tl::paged;
 
 namespace {
-// Rows per sequence and kv head, on average, from which the 256-row tiles pay.
+// Rows per sequence and kv head, on average, from which the kernels for chunks pay: this file's kernel reads all keys
+// once for every 16 rows, theirs for every 256 (fp32: 64).  32 heads, 8 kv heads, hd 128, 64 x 4096 keys, bf16 / fp32:
+// 16 rows 180 / 905 us here and 205 / 1630 us there, 20 rows 343 / 1763 and 212 / 1631; 16 x 1000 keys: 16 rows
+// 30 / 85 and 28 / 130, 20 rows 43 / 139 and 28 / 130.
 bool many_rows(const tl_paged_cache* c, size_t n_tokens, size_t n_heads, size_t n_seq) {
-    return c->dtype != TL_F32 && n_tokens * (n_heads / c->n_kv_heads) > 16 * n_seq;
+    return n_tokens * (n_heads / c->n_kv_heads) > 16 * n_seq;
 }
 }  // namespace
 
@@ -820,7 +721,9 @@ tl_status tl_paged_attention_workspace(const tl_paged_cache* cache, size_t n_tok
                n_heads, cache->n_kv_heads);
     (void)max_blocks;
     const int hd = static_cast<int>(cache->head_dim);
-    *bytes = many_rows(cache, n_tokens, n_heads, n_seq) ? chunk_workspace(hd) : split_workspace(hd);
+    *bytes = !many_rows(cache, n_tokens, n_heads, n_seq) ? split_workspace(hd)
+             : cache->dtype == TL_F32                    ? chunk_f32_workspace(hd)
+                                                         : chunk_workspace(hd);
     return TL_OK;
 }
 
@@ -868,8 +771,9 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.cap = static_cast<int>(std::min<size_t>(max_blocks << a.shift, kMaxLen));
     a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
     a.scale = scale == 0.f ? 1e-30f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
-    return many_rows(cache, n_tokens, n_heads, n_seq) ? attend_chunk(a, cache, workspace, as_stream(stream))
-                                                      : attend_split(a, cache, workspace, as_stream(stream));
+    if (!many_rows(cache, n_tokens, n_heads, n_seq)) return attend_split(a, cache, workspace, as_stream(stream));
+    return cache->dtype == TL_F32 ? attend_chunk_f32(a, cache, workspace, as_stream(stream))
+                                  : attend_chunk(a, cache, workspace, as_stream(stream));
 }
 
 }  // extern "C"

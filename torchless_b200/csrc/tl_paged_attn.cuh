@@ -320,16 +320,127 @@ __device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h
     for (int d = 0; d < D; d++) op[d] = from_f32<T>(l != 0.f ? acc[d] / l : 0.f);
 }
 
+constexpr int kJoinWarps = 8;
+// Joins the parts (fp32 rows of hd + 4: maximum, sum, whether to do it over, -, values) of the tile that block blockIdx.x began: part i > 0 is the first tile of block blockIdx.x + i.
+// Two warps a row (one for its
+// even parts, one for the odd); lane = 4 or 2 dims; the rows are spread over gridDim.y blocks.
+template <typename T, int HD, int R>
+__global__ void __launch_bounds__(kJoinWarps * 32) k_attend_join(const __grid_constant__ AttendArgs a, const Head* heads,
+                                                          const float* parts) {
+    constexpr int D = HD / 32;
+    __shared__ float half[kJoinWarps / 2][32 * D + 2];
+    pdl_wait();
+    const Head h = heads[blockIdx.x];
+    if (h.parts == 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, odd = warp & 1;
+    Cursor c;
+    c.g = h.g;
+    c.t = tile_of(a, h.b, h.rt, R);
+    constexpr size_t rec = static_cast<size_t>(R) * (HD + 4);
+    const float* p0 = parts + (static_cast<size_t>(blockIdx.x) * 2 + h.slot) * rec;
+    const float* p1 = parts + (static_cast<size_t>(blockIdx.x) + 1) * 2 * rec;  // parts 1 .. are 2 * rec apart
+    auto part = [&](int i, int row) { return (i == 0 ? p0 : p1 + static_cast<size_t>(i - 1) * 2 * rec) + row * (HD + 4); };
+#pragma unroll 1
+    for (int row0 = blockIdx.y * (kJoinWarps / 2); row0 < c.t.nrows; row0 += gridDim.y * (kJoinWarps / 2)) {
+        const int row = row0 + (warp >> 1);
+        float M = -INFINITY, bad = 0.f, L = 0.f, acc[D];
+#pragma unroll
+        for (int d = 0; d < D; d++) acc[d] = 0.f;
+        if (row < c.t.nrows) {
+#pragma unroll 1
+            for (int i0 = odd; i0 < h.parts; i0 += 16) {  // 8 parts at a time
+                float m[8], l[8], v[8][D], mx = M;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int i = i0 + 2 * k;
+                    m[k] = -INFINITY;
+                    l[k] = 0.f;
+#pragma unroll
+                    for (int d = 0; d < D; d++) v[k][d] = 0.f;
+                    if (i < h.parts) {
+                        const float* p = part(i, row);
+                        const float4 q = *reinterpret_cast<const float4*>(p);
+                        m[k] = q.x;
+                        l[k] = q.y;
+                        bad = fmaxf(bad, q.z);
+#pragma unroll
+                        for (int d = 0; d < D; d++) v[k][d] = p[4 + lane + 32 * d];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) mx = fmaxf(mx, m[k]);
+                const float f0 = mx == -INFINITY ? 1.f : ex2(M - mx);
+                L *= f0;
+#pragma unroll
+                for (int d = 0; d < D; d++) acc[d] *= f0;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float f = mx == -INFINITY ? 1.f : ex2(m[k] - mx);
+                    L += l[k] * f;
+#pragma unroll
+                    for (int d = 0; d < D; d++) acc[d] += v[k][d] * f;
+                }
+                M = mx;
+            }
+        }
+        if (odd) {
+            float* x = half[warp >> 1];
+            if (lane == 0) {
+                x[0] = M;
+                x[1] = bad > 0.f ? NAN : L;  // (NaN: to be done over)
+            }
+#pragma unroll
+            for (int d = 0; d < D; d++) x[2 + lane + 32 * d] = acc[d];
+        }
+        __syncthreads();
+        if (!odd && row < c.t.nrows) {
+            const float* x = half[warp >> 1];
+            int tok, hh;
+            row_of(a, c, row, tok, hh);
+            const float mx = fmaxf(M, x[0]), f0 = mx == -INFINITY ? 1.f : ex2(M - mx), f1 = mx == -INFINITY ? 1.f : ex2(x[0] - mx);
+            if (bad > 0.f || x[1] != x[1]) {
+                attend_row<T, HD>(a, h.b, tok, hh, lane);
+            } else {
+                const float sum = L * f0 + x[1] * f1;
+                T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD;
+#pragma unroll
+                for (int d = 0; d < D; d++) {
+                    const float o = acc[d] * f0 + x[2 + lane + 32 * d] * f1;
+                    out[lane + 32 * d] = from_f32<T>(sum != 0.f ? o / sum : 0.f);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int HD, int R>
+tl_status launch_join(const AttendArgs& a, const Head* heads, const float* parts, int blocks, int slices, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks, slices);
+    cfg.blockDim = dim3(kJoinWarps * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    TL_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_attend_join<T, HD, R>, a, heads, parts));
+    return TL_OK;
+}
+
 // Map of one side (K or V) of the pages: {64 or hd columns, rows of all kv heads, column
 // panels, pages}; a box is `rows` rows of `panels` panels of one page, zero where the page does not
 // exist.  16-bit types: panels of 64 columns, SWIZZLE_128B; fp32: one panel, no swizzle.
 tl_status encode_pages(CUtensorMap* map, const void* base, const tl_paged_cache* c, int rows, int panels);
 
-// Few query rows per sequence (tl_paged_attn.cu), and many (tl_paged_attn_tc.cu; not fp32).
+// Few query rows per sequence (tl_paged_attn.cu), and many (tl_paged_attn_tc.cu; fp32: tl_paged_attn_f32.cu).
 size_t split_workspace(int hd);
 tl_status attend_split(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s);
 size_t chunk_workspace(int hd);
 tl_status attend_chunk(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s);
+size_t chunk_f32_workspace(int hd);
+tl_status attend_chunk_f32(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace tl
