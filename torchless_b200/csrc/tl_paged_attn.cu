@@ -92,7 +92,7 @@ struct Shape {
 template <int R_, int KS>
 struct SplitPlan {
     static constexpr int R = R_;
-    static constexpr int kTileCost = 12;
+    static constexpr int kTileCost = 24;
     static __device__ __forceinline__ int steps(const Tile& t) {
         return kTileCost + (t.hi <= t.lo ? 1 : (t.hi - 1) / KS - t.lo / KS + 1);
     }
