@@ -250,7 +250,7 @@ TL_API tl_status tl_paged_plan(int32_t* block_table, int32_t* q_start, int32_t* 
  *   slots    as tl_paged_plan gives them
  * A row whose position is not in [0, n_pos) belongs to no sequence: nothing is
  * written for it.  A row whose slot names no page of the cache gets its q, and
- * no cache write.  Two rows with one slot leave either's k and v there.
+ * no cache write.  Two rows with one slot leave values of both there.
  * Arithmetic is fp32, rounded once.  rot_dim is a multiple of 16 up to
  * head_dim; pointers and row_stride are aligned to 16 bytes; q_out does not
  * overlap qkv. */

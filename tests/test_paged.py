@@ -54,6 +54,12 @@ def test_attention_refusals():
     assert call(n_seq=0) == 0
 
 
+def test_scales_that_pass_fp32_are_refused():
+    L, c = lib(), cache()
+    for scale in (3.0e38, -3.0e38):
+        assert L.tl_paged_attention(A, A, 256, ctypes.byref(c), A, 1, A, A, 1, 1, 4, scale, 0, A, 1 << 30, None) == INVALID
+
+
 def test_rope_refusals():
     L, c = lib(), cache()
 

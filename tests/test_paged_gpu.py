@@ -556,3 +556,144 @@ def test_another_stream_and_repeated_calls_agree():
             outs.append(out)
     torch.cuda.synchronize()
     assert all(torch.equal(outs[0], x) for x in outs[1:])
+
+
+# ---------------------------------------------------------------- more of attention
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_seq", [257, 700])
+@pytest.mark.parametrize("most", [1, 12])
+def test_more_sequences_than_a_block_has_threads(dtype, n_seq, most):
+    """Decode steps (most = 1) and short chunks, some without tokens."""
+    rng = np.random.default_rng(n_seq + most)
+    new = rng.integers(0, most + 1, n_seq)
+    lens = new + rng.integers(0, 30, n_seq)
+    run_attend(lens.tolist(), new.tolist(), 4, 1, 64, 8, dtype, seed=most)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_row_tiles_than_a_warp_has_lanes(dtype):
+    run_attend([1200, 3], [1100, 1], 8, 1, 64, 64, dtype)
+    run_attend([300] + [5] * 59, [130] + [1] * 59, 4, 1, 64, 16, dtype)  # few rows a sequence on average
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,KV", [(24, 1), (100, 1), (14, 2)])
+def test_groups_of_odd_sizes(dtype, H, KV):
+    run_attend([77, 5, 300], [1, 1, 1], H, KV, 64, 16, dtype)
+    run_attend([77, 5, 300], [13, 5, 2], H, KV, 128, 32, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [[1, 1], [90, 33]])
+def test_signs_and_sizes_of_the_scale(dtype, new):
+    """A negative scale, a tiny one, and 0 with scores that are far from 1: all weights alike."""
+    run_attend([90, 333], new, 8, 2, 128, 16, dtype, scale=-0.2)
+    run_attend([90, 333], new, 8, 2, 64, 16, dtype, scale=1e-38)
+    run_attend([90, 333], new, 8, 2, 64, 16, dtype, scale=0.0, kscale=1e4 if dtype == "f16" else 1e33)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [[1, 1, 1], [80, 20, 33]])
+@pytest.mark.parametrize("window", [5, 40])
+def test_missing_pages_under_a_window(dtype, new, window):
+    q, kc, vc, table, q_start, ln = attend_case([200, 64, 90], new, 8, 2, 64, 8, dtype)
+    table[0, 23:25], table[0, 15], table[1, 7], table[2, 3:12] = -1, kc.shape[0], -2 ** 31, -1
+    out = torch.full(q.shape, 3.0, device="cuda", dtype=q.dtype)
+    ops().paged_attention(out, q, kc, vc, i32(table), i32(q_start), i32(ln), None, window)
+    check_attend(out, q, kc, vc, table, q_start, ln, dtype, window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_offsets_past_32_bits(dtype):
+    """Pages 2^25 elements apart: the last ones lie more than 2^31 elements behind the first.  K and V are
+    written there by qk_norm_rope and read by both kinds of attention."""
+    KV, hd, bs, n_blocks, stride, H = 1, 64, 8, 68, 1 << 25, 4
+    big = torch.zeros(2 * n_blocks * stride, device="cuda", dtype=DT[dtype])
+    kc, vc = (big[i * n_blocks * stride:][:n_blocks * stride].view(n_blocks, stride)[:, :KV * bs * hd].view(n_blocks, KV, bs, hd)
+              for i in (0, 1))
+    n = 540
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn(n, (H + 2 * KV) * hd, generator=g, device="cuda")
+    pos = torch.arange(n, device="cuda", dtype=torch.int32)
+    table = torch.arange(n_blocks, device="cuda", dtype=torch.int32)[None]
+    cos, sin = torch.ones(n, 32, device="cuda"), torch.zeros(n, 32, device="cuda")
+    q = torch.empty(n, H, hd, device="cuda", dtype=DT[dtype])
+    ops().qk_norm_rope(q, kc, vc, qkv, pos, pos, cos, sin)
+    assert torch.equal(kc.reshape(-1, hd)[:n], qkv[:, H * hd:(H + 1) * hd].to(DT[dtype]))
+    assert torch.equal(vc.reshape(-1, hd)[:n], qkv[:, (H + 1) * hd:].to(DT[dtype]))
+    small = kc.contiguous(), vc.contiguous()
+    for rows in (1, 200):
+        qq, args = q[n - rows:], (table, i32([0, rows]), i32([n]))
+        a, b = torch.empty_like(qq), torch.empty_like(qq)
+        ops().paged_attention(a, qq, kc, vc, *args)
+        ops().paged_attention(b, qq, *small, *args)
+        assert torch.equal(a, b)
+        check_attend(a, qq, *small, np.arange(n_blocks)[None], np.array([0, rows]), np.array([n]), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_streams_at_once(dtype):
+    """Steps of two batches in two streams, each call with a workspace of its own, give what they give alone."""
+    cases = [attend_case([900, 90, 14], [1, 1, 1], 8, 2, 128, 16, dtype, seed=1),
+             attend_case([700, 260], [300, 60], 8, 2, 128, 16, dtype, seed=2)]
+    args = [(i32(t), i32(s), i32(n)) for _, _, _, t, s, n in cases]
+    want = []
+    for (q, kc, vc, *_), a in zip(cases, args):
+        want.append(torch.empty(q.shape, device="cuda", dtype=q.dtype))
+        ops().paged_attention(want[-1], q, kc, vc, *a)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(20):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                q, kc, vc = cases[k][:3]
+                outs[k].append(torch.empty(q.shape, device="cuda", dtype=q.dtype))
+                ops().paged_attention(outs[k][-1], q, kc, vc, *args[k])
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(x, want[k]) for x in outs[k])
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("tokens", [1, 64])
+def test_workspaces_that_do_not_do_are_refused(dtype, tokens):
+    import ctypes
+    from torchless_b200 import lib, tl_paged_cache
+    L = lib()
+    kc = torch.zeros(4, 1, 16, 64, device="cuda", dtype=[torch.float32, torch.float16][dtype])
+    q = torch.zeros(tokens, 4, 64, device="cuda", dtype=kc.dtype)
+    out = torch.full_like(q, 3.0)
+    table, start, lens = i32([[0, 1, 2, 3]]), i32([0, tokens]), i32([64])
+    c = tl_paged_cache(kc.data_ptr(), kc.data_ptr(), 4, 1, 16, 64, 16 * 64, dtype)
+    need = ctypes.c_size_t()
+    assert L.tl_paged_attention_workspace(ctypes.byref(c), tokens, 4, 1, 4, ctypes.byref(need)) == 0
+    ws = torch.zeros(need.value + 16, device="cuda", dtype=torch.uint8)
+
+    def call(p, size):
+        return L.tl_paged_attention(out.data_ptr(), q.data_ptr(), 256, ctypes.byref(c), table.data_ptr(), 4,
+                                    start.data_ptr(), lens.data_ptr(), 1, tokens, 4, 0.1, 0, p, size, None)
+    assert call(None, need.value) and call(ws.data_ptr(), need.value - 1) and call(ws.data_ptr() + 8, need.value)
+    torch.cuda.synchronize()
+    assert (out == 3).all()
+    assert call(ws.data_ptr(), need.value) == 0
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+
+
+def test_two_tokens_with_one_slot():
+    """The slot holds numbers of the two; nothing else changes."""
+    q_out, kc, vc, _, qkv, pos, slots, cos, sin, wq, wk = rope_case(30, 4, 2, 64, 16, 64, "f32", "f32", "none")
+    slots[9] = slots[4]
+    before = [f64(t) for t in (q_out, kc, vc)]
+    ops().qk_norm_rope(q_out, kc, vc, qkv, pos, slots, cos, sin)
+    got = []
+    for drop in (4, 9):  # either alone
+        kk, vv = kc.clone().fill_(7), vc.clone().fill_(7)
+        s = slots.clone()
+        s[drop] = -1
+        ops().qk_norm_rope(torch.empty_like(q_out), kk, vv, qkv, pos, s, cos, sin)
+        got.append((kk, vv))
+    for x, a, b in zip((kc, vc), got[0], got[1]):
+        assert ((x == a) | (x == b)).all()
+    assert before[1].shape == kc.shape

@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int s = first_step(c);; s += kWarps) {
 #pragma unroll 1
-            while (more && ahead < NST) {  // one step into the ring
+            while (more && !dead && ahead < NST) {  // one step into the ring
                 if (ps >= pc.end - P::kTileCost) {
                     more = next_tile<P>(a, pc);
                     ps = first_step(pc);
@@ -574,6 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 begun = true;
             }
             if (s >= c.end - P::kTileCost) break;
+            if (ahead == 0) continue;  // (a copy never came: no further ones)
             dead |= !spin(&bars[got_st], (got_parity >> got_st) & 1);
             got_parity ^= 1u << got_st;
             StepInfo si;
@@ -590,8 +591,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // A result that is not finite: a value that one row must not see may have met it as 0 x infinity,
         // or an infinite value the split weights.  Such a tile is done over row by row, which gives the
-        // formula's result to each.  (Every finite input stays far from this.)
-        const bool redo = core.finish(c.t.nrows, lane) && !dead;
+        // formula's result to each.  (Every finite input stays far from this.)  The same where a copy never came.
+        const bool redo = core.finish(c.t.nrows, lane) || dead;
         const bool whole = c.s == 0 && c.end == c.steps;
         float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * R * (HD + 4);
         const int any_redo = __syncthreads_or(redo);
@@ -599,7 +600,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int pass = 0; pass * 8 < c.t.nrows; pass++) {
             if (pass) __syncthreads();
             core.dump(join + warp * S::JOIN, pass, lane);
-            if (dead && lane < 8) join[warp * S::JOIN + lane * (HD + 4) + 1] = NAN;  // a copy never came: no answer
             __syncthreads();
             const int row = 8 * pass + warp;  // one warp a row
             if (row < c.t.nrows) {
@@ -744,7 +744,7 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
                q_stride);
     TL_REQUIRE(aligned16(out) && aligned16(q) && q_stride * dtype_size(cache->dtype) % 16 == 0,
                "tl_paged_attention: out, q and q_stride must be 16-byte aligned");
-    TL_REQUIRE(scale == scale && fabsf(scale) <= 3.0e38f, "tl_paged_attention: scale %g", static_cast<double>(scale));
+    TL_REQUIRE(scale == scale && fabsf(scale) <= 2.0e38f, "tl_paged_attention: scale %g", static_cast<double>(scale));
     size_t need = 0;
     TL_TRY(tl_paged_attention_workspace(cache, n_tokens, n_heads, n_seq, max_blocks, &need));
     TL_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need,
@@ -770,7 +770,7 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.shift = __builtin_ctzll(cache->block_size);
     a.cap = static_cast<int>(std::min<size_t>(max_blocks << a.shift, kMaxLen));
     a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
-    a.scale = scale == 0.f ? 1e-30f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
+    a.scale = scale == 0.f ? 1e-45f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
     if (!many_rows(cache, n_tokens, n_heads, n_seq)) return attend_split(a, cache, workspace, as_stream(stream));
     return cache->dtype == TL_F32 ? attend_chunk_f32(a, cache, workspace, as_stream(stream))
                                   : attend_chunk(a, cache, workspace, as_stream(stream));

@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float w0 = 1.f, w1 = 0.f, mt = m, lt = xl[2 * i * 128 + r] + xl[(2 * i + 1) * 128 + r];
             if (fold) {
                 stream_sync(i, true);
-                xl[(2 * i + hf) * 128 + r] = hf ? lt : m;
+                xl[(2 * i + hf) * 128 + r] = !good ? NAN : hf ? lt : m;
                 __syncwarp();
                 if (lane == 0) bar_arrive(xbar);
                 if (good && !__all_sync(FULL, wait(xbar, nx & 1))) give_up();
@@ -627,13 +627,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_after();
             }
             const bool whole = c.s == 0 && c.end == c.steps;
-            const bool writer = good && (p.two || fold || i == 0);
+            const bool writer = p.two || fold || i == 0;
+            // A wait that ran out: the accumulators hold nothing, and the rows are done over like those that are not finite.
+            const bool fine = good && ok;
+            if (!fine) lt = NAN;
             const int c0 = fold ? (2 * i + hf) * (HD / 4) : hf * (HD / 2), c1 = c0 + (fold ? HD / 4 : HD / 2);  // columns
             float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * kRows * (HD + 4);
             if (writer) {
                 const float inv = lt != 0.f ? 1.f / lt : 0.f;
                 float z = lt * 0.f;  // NaN once a value is not finite
-                const bool t0 = fold || act;
+                const bool t0 = fine && (fold || act);
                 const uint32_t ta = fold ? tO + lane_off : to;
 #pragma unroll 1
                 for (int col = c0; col < c1; col += 16) {
@@ -645,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 16; e++) o[e] = 0u;
                     }
-                    if (fold) {
+                    if (fold && fine) {
                         uint32_t o1[16];
                         tmem_ld16_async(tO + 128 + lane_off + col, o1);
                         tmem_wait_ld();
