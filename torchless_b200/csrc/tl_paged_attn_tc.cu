@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             const int row0 = p.two ? i * kHalf : 0;
-#pragma unroll 1
+#pragma unroll 4
             for (int rr = lane / CH; rr < kHalf; rr += RPI) {
                 int tok, h;
                 row_of(a, c, row0 + rr, tok, h);
