@@ -229,7 +229,7 @@ __device__ __forceinline__ Part part_of(const AttendArgs& a, const Cursor& c) {
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attend_chunk(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                   const __grid_constant__ AttendArgs a,
+                   const __grid_constant__ CUtensorMap map_q, const __grid_constant__ AttendArgs a,
                    Head* heads, float* parts) {
     using S = Shape<HD>;
     constexpr int NST = S::NST;
@@ -441,22 +441,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             const int row0 = p.two ? i * kHalf : 0;
-#pragma unroll 4
-            for (int rr = lane / CH; rr < kHalf; rr += RPI) {
+            loaded++;
+            if (kHalf % a.group == 0) {  // whole tokens: a box of the map each panel
+                if (lane == 0) {
+                    bar_expect_tx(&q_full[i], S::STAGE);
+                    for (int x = 0; x < S::PANELS; x++)
+                        tma_panel(sQ + i * S::STAGE + x * S::PANEL, &map_q, x, c.g * a.group, c.t.first + div_group(a, c.t.r0 + row0),
+                                  &q_full[i]);
+                }
+                __syncwarp();
+                continue;
+            }
+#pragma unroll 1
+            for (int r0 = 0; r0 < kHalf; r0 += 32) {  // a lane finds one row's place, the others get it from there
                 int tok, h;
-                row_of(a, c, row0 + rr, tok, h);
-                const T* src = static_cast<const T*>(a.q) + static_cast<size_t>(tok) * a.q_stride + static_cast<size_t>(h) * HD + 8 * d;
-                const uint32_t bytes = row0 + rr < c.t.nrows ? 16u : 0u;  // (a row that does not exist: zeros)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(su32(dst + sw128(rr, d & 7))), "l"(src), "r"(bytes)
-                             : "memory");
+                row_of(a, c, row0 + r0 + lane, tok, h);
+                const unsigned long long at = static_cast<size_t>(tok) * a.q_stride + static_cast<size_t>(h) * HD;
+#pragma unroll 2
+                for (int k = 0; k < 32; k += RPI) {
+                    const int kk = k + lane / CH, rr = r0 + kk;
+                    const T* src = static_cast<const T*>(a.q) + __shfl_sync(FULL, at, kk) + 8 * d;
+                    const uint32_t bytes = row0 + rr < c.t.nrows ? 16u : 0u;  // (a row that does not exist: zeros)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(su32(dst + sw128(rr, d & 7))), "l"(src), "r"(bytes)
+                                 : "memory");
+                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) bar_arrive(&q_full[i]);
-            loaded++;
         }
         if (!ok) fail();
+        if (loaded) bar_wait(&q_full[i], (loaded - 1) & 1);  // a copy lands before the block ends
     } else {
         // ---- softmax and epilogue: thread = half hf of row r of stream i.  A thread whose wait fails goes on
         // through the loops' barriers, doing no work, so that the others find it there ----
@@ -806,20 +822,39 @@ __global__ void __launch_bounds__(256) k_attend_chunk_join(const __grid_constant
     }
 }
 
+// Map of Q: {64 columns, panels, heads, tokens}; a box is one panel of 128 rows, which are the heads of a group for
+// 128 / group tokens.  (Where the group does not divide 128 the map is not used.)
+template <int HD>
+tl_status encode_q(CUtensorMap* map, const AttendArgs& a, tl_dtype dtype) {
+    auto fn = encode_fn();
+    if (!fn) return set_error(TL_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint32_t group = kHalf % a.group == 0 ? a.group : 1;
+    const cuuint64_t dims[4] = {64, HD / 64, static_cast<cuuint64_t>(a.H), static_cast<cuuint64_t>(a.n_tokens)};
+    const cuuint64_t strides[3] = {128, HD * 2, a.q_stride * 2};
+    const cuuint32_t box[4] = {64, 1, group, kHalf / group};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, dtype == TL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                          const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(TL_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return TL_OK;
+}
+
 template <typename T, int HD>
 tl_status run_chunk(const AttendArgs& a, const tl_paged_cache* c, void* workspace, cudaStream_t s) {
     using S = Shape<HD>;
     static_assert(S::SMEM <= 232448, "shared memory of a block");
-    CUtensorMap mk, mv;
+    CUtensorMap mk, mv, mq;
     const int rows = std::min(kKB, 1 << a.shift);
     TL_TRY(encode_pages(&mk, c->k, c, rows, 1));
     TL_TRY(encode_pages(&mv, c->v, c, rows, 1));
+    TL_TRY(encode_q<HD>(&mq, a, c->dtype));
     TL_CUDA_TRY(cudaFuncSetAttribute(k_attend_chunk<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      static_cast<int>(S::SMEM)));
     const int grid = std::min(sm_count(), kMaxBlocks);
     Head* heads = static_cast<Head*>(workspace);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeadBytes);
-    k_attend_chunk<T, HD><<<grid, kThreads, S::SMEM, s>>>(mk, mv, a, heads, parts);
+    k_attend_chunk<T, HD><<<grid, kThreads, S::SMEM, s>>>(mk, mv, mq, a, heads, parts);
     TL_TRY(check_launch("paged_attention"));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid, kRows / 32);
