@@ -106,28 +106,26 @@ struct Cursor {
     Tile t;
 };
 
-template <class Plan>
-__device__ __forceinline__ void enter(const AttendArgs& a, Cursor& c) {
-    c.t = tile_of(a, c.b, c.rt, Plan::R);
-    c.steps = Plan::steps(c.t);
-    c.end = min(c.steps, c.s + c.left);
-}
 // To the next tile that has rows; false when the block's share is done.
 template <class Plan>
 __device__ __forceinline__ bool next_tile(const AttendArgs& a, Cursor& c) {
     c.left -= c.end - c.s;
     if (c.left <= 0) return false;
     c.s = 0;
-    if (++c.g == a.KV) {
-        c.g = 0;
-        c.rt++;
-        while (c.rt * Plan::R >= c.t.n * a.group) {  // sequences without rows have no steps
-            if (++c.b >= a.n_seq) return false;
-            c.rt = 0;
-            rows_of(a, c.b, c.t.first, c.t.n);
-        }
+    if (++c.g < a.KV) {  // the same rows of the next kv head
+        c.end = min(c.steps, c.left);
+        return true;
     }
-    enter<Plan>(a, c);
+    c.g = 0;
+    c.rt++;
+    while (c.rt * Plan::R >= c.t.n * a.group) {  // sequences without rows have no steps
+        if (++c.b >= a.n_seq) return false;
+        c.rt = 0;
+        rows_of(a, c.b, c.t.first, c.t.n);
+    }
+    c.t = tile_of(a, c.b, c.rt, Plan::R);
+    c.steps = Plan::steps(c.t);
+    c.end = min(c.steps, c.left);
     return true;
 }
 
