@@ -299,7 +299,7 @@ tl_status run_chunk_f32(const AttendArgs& a, void* workspace, cudaStream_t s) {
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeadBytes);
     k_attend_chunk_f32<HD><<<grid, kThreads, S::SMEM, s>>>(a, heads, parts);
     TL_TRY(check_launch("paged_attention"));
-    return launch_join<float, HD, kRows>(a, heads, parts, grid, kRows / 16, s);
+    return launch_join<float, HD, kRows>(a, heads, parts, grid, kRows / 8, s);
 }
 
 }  // namespace
