@@ -21,6 +21,10 @@
 //   - At a tile's end the warps join (max, sum, accumulator) in shared memory;
 //     a tile that continues in another block leaves its part in the workspace,
 //     and a second small kernel joins the parts in order.
+// 32 heads, 8 kv heads, hd 128, one token a sequence: 64 x 4096 keys bf16 178 us (6.0 TB/s of 6.55 that a copy reaches),
+// fp32 329 us (6.5 TB/s), 64 ragged lengths of at most 4096 fp16 70 us (5.3 TB/s); 1 x 8192 bf16 15.4 us, where finding
+// the shares (2.7 us), the first copies, the join and the launches count more than the 5.1 us of reading.  A tile
+// costs about 3 us beside its keys: 200 x 300 keys 73 us (3.4 TB/s).
 #include <math.h>
 
 #include <algorithm>
@@ -87,8 +91,9 @@ struct Shape {
 };
 
 // Steps of KS keys, tiles of R rows.  Beginning and ending a tile takes about as long as kTileCost steps, which count
-// as steps before its first key, so that a batch of short sequences is shared as evenly as one of long ones.  A
-// tile without keys counts one step more, so that its zeros get written.
+// as steps before its first key, so that a batch of short sequences is shared as evenly as one of long ones (64 ragged
+// lengths of at most 4096: 12 steps 78.8 us, 16 73.7, 24 69.9, 32 69.9, 48 74.4 us; where all are alike it makes no
+// difference).  A tile without keys counts one step more, so that its zeros get written.
 template <int R_, int KS>
 struct SplitPlan {
     static constexpr int R = R_;
@@ -149,7 +154,7 @@ __device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo, __nv_
 }
 // 16 rows on the matrix instruction: lane l holds rows l / 4 and l / 4 + 8.
 template <typename T, int HD, int R>
-struct Core {  // (its stages: see Shape)
+struct Core {
     static_assert(R == 16, "the instruction's height");
     static constexpr int NO = HD / 8;
     uint32_t q[HD / 16][4];

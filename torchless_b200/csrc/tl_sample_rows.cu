@@ -281,7 +281,10 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
 //                 in which the running sum crosses.
 // A block per row.  An instruction that is executed once costs some 35 cycles (its line of code comes from L2), so
 // for one row the length of the path counts as much as the work on it; with many rows the 64-bit arithmetic of the
-// rows that keep thousands of logits does.
+// rows that keep thousands of logits does.  32000 logits of fp32, 1 row / 256 rows: top-k below 257 with top-p and
+// min-p 13 / 30 us, no cut 20 / 43 us, top-p alone 31 / 74 us, mixed rows 70 us (0.5 TB/s); by radix selection 156 /
+// 343, 76 / 156, 465 / 1142 us.  With the row read again from L2 in place of shared memory 14 / 37, 23 / 53, 35 / 88 us.
+// 512 threads a row, two rows an SM, are no faster.
 constexpr int kSmallK = 256, kBins = 2048, kList = 4096, kSeg = 4 * kThreads, kMaxSegs = 64;
 constexpr int kWarps = kThreads / 32;
 constexpr float kDepth = 20.f;  // the bins reach to weights of e^-20
