@@ -232,8 +232,8 @@ typedef struct tl_paged_cache {
  *   slots[n_tokens]     page id * block_size + offset in the page; -1 for a
  *       token without a page
  *   counts[2]           ids taken from free_blocks; ids missing
- * Rows behind the last request get position and slot -1.  n_req = 0 or
- * n_tokens = 0 are allowed.  n_req * max_blocks and n_tokens must stay below 2^31. */
+ * Rows behind the last request get position and slot -1.  No output overlaps
+ * an input or another output.  n_req = 0 or n_tokens = 0 are allowed.  n_req * max_blocks and n_tokens must stay below 2^31. */
 TL_API tl_status tl_paged_plan(int32_t* block_table, int32_t* q_start, int32_t* seq_lens, int32_t* positions,
                                int32_t* slots, int32_t* counts, const int32_t* cached, const int32_t* new_tokens,
                                const int32_t* free_blocks, size_t n_free, size_t n_req, size_t max_blocks,

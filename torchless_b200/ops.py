@@ -323,11 +323,12 @@ def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, sc
         raise ValueError("block_table must be [n_seq, max_blocks] and window not negative")
     n_seq, width = block_table.shape
     L, cache = lib(), ctypes.byref(c)
-    key = (c.dtype, hd, c.n_kv_heads, heads, n, n_seq)
+    key = (index, c.dtype, hd, c.n_kv_heads, heads, n, n_seq)
     need = _WORKSPACE.get(key)
     if need is None:
         size = ctypes.c_size_t()
-        check(L.tl_paged_attention_workspace(cache, n, heads, n_seq, width, ctypes.byref(size)))
+        with torch.cuda.device(index):
+            check(L.tl_paged_attention_workspace(cache, n, heads, n_seq, width, ctypes.byref(size)))
         if len(_WORKSPACE) >= 4096:
             _WORKSPACE.clear()
         need = _WORKSPACE[key] = size.value
@@ -338,7 +339,7 @@ def paged_attention(out, q, k_cache, v_cache, block_table, q_start, seq_lens, sc
             hd ** -0.5 if scale is None else scale, window, ws.data_ptr(), need)
 
 
-_WORKSPACE = {}  # the workspace's size by type, heads and numbers of rows and sequences
+_WORKSPACE = {}  # the workspace's size by device, type, heads and numbers of rows and sequences
 
 
 def sample_rows(logits, r, temperature, top_k=None, top_p=None, min_p=None):
