@@ -441,6 +441,20 @@ def test_sample_strided_rows():
     assert ops().sample_rows(x[:0], f32([]), f32([])).numel() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n", [(700, 257), (310, 1500), (160, 30000)])
+def test_sample_more_rows_than_run_at_once(dtype, rows, n):
+    """Greedy rows, short lists, cuts by top-p and none, side by side: every row gets its answer."""
+    rng = np.random.default_rng(rows)
+    x = rng.standard_normal((rows, n)) * 2
+    kind = rng.integers(0, 4, rows)
+    T = np.where(kind == 0, 0.0, rng.uniform(0.4, 1.3, rows)).astype(np.float32)
+    k = np.where(kind == 1, rng.integers(1, 300, rows), 0)
+    p = np.where(kind == 2, rng.uniform(0.3, 0.99, rows), 1.0).astype(np.float32)
+    run_sample(x, rng.random(rows, np.float32), T, k, p, None, dtype)
+    run_sample(x, rng.random(rows, np.float32), T, None, p, None, dtype)
+
+
 # ---------------------------------------------------------------- together
 
 def step_state(dtype, seed):

@@ -22,6 +22,7 @@ struct SampleRowsArgs {
     const float *r, *temperature, *top_p, *min_p;
     const int32_t* top_k;
     int segs;  // segments of kSeg logits
+    int rows;  // the grid is as large, or twice (see tl_sample_rows)
 };
 
 // Order-preserving key of a logit: larger logit, larger key; -0 and +0 the same.
@@ -282,7 +283,7 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
 // A block per row.  An instruction that is executed once costs some 35 cycles (its line of code comes from L2), so
 // for one row the length of the path counts as much as the work on it; with many rows the 64-bit arithmetic of the
 // rows that keep thousands of logits does.  32000 logits of fp32, 1 row / 256 rows: top-k below 257 with top-p and
-// min-p 13 / 30 us, no cut 20 / 43 us, top-p alone 31 / 74 us, mixed rows 70 us (0.5 TB/s); by radix selection 156 /
+// min-p 13 / 31 us, no cut 20 / 43 us, top-p alone 31 / 74 us, mixed rows 54 us (0.6 TB/s); by radix selection 156 /
 // 343, 76 / 156, 465 / 1142 us.  With the row read again from L2 in place of shared memory 14 / 37, 23 / 53, 35 / 88 us.
 // 512 threads a row, two rows an SM, are no faster.
 constexpr int kSmallK = 256, kBins = 2048, kList = 4096, kSeg = 4 * kThreads, kMaxSegs = 64;
@@ -748,10 +749,13 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleRowsArgs a) {
     uint32_t* hist = reinterpret_cast<uint32_t*>(list + kList);            // kBins
     unsigned long long* cells = reinterpret_cast<unsigned long long*>(hist + kBins);
     float* v = reinterpret_cast<float*>(cells + a.segs * kWarps);          // SMEM: the row
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool again = blockIdx.x >= static_cast<unsigned>(a.rows);  // the second half of a grid of twice the rows
+    const int row = blockIdx.x - (again ? a.rows : 0), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T* x = static_cast<const T*>(a.logits) + static_cast<size_t>(row) * a.row_stride;
     const int n = a.n;
     const float temp = a.temperature[row];
+    const int k = a.top_k ? a.top_k[row] : 0;
+    if (gridDim.x > static_cast<unsigned>(a.rows) && (!(temp > 0.f) || (k > 0 && k < n && k <= kSmallK)) != again) return;
     if (!(temp > 0.f)) {
         const uint32_t best = first_max<T>(x, n, sc);
         if (tid == 0) a.out[row] = best;
@@ -808,7 +812,6 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleRowsArgs a) {
     uint32_t answer = static_cast<uint32_t>(n - 1);
     if (bk < 0xff800000u && bk > key_of(-INFINITY)) {  // neither NaN nor +inf, and something above -inf
         const float top = logit_of(bk);
-        const int k = a.top_k ? a.top_k[row] : 0;
         const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f, r = a.r[row];
         const Scale ws{widen(top), 46.16624130844683 / static_cast<double>(temp), pow2};  // 32 / ln 2
         const Row R{v, x, n, pad, a.segs, top, ws.c, kBins / (kDepth * temp), cells};
@@ -842,9 +845,13 @@ extern "C" tl_status tl_sample_rows(uint32_t* out, const void* logits, tl_dtype 
     const int segs = static_cast<int>((n + 3 + kSeg - 1) / kSeg);
     const size_t base = kList * 8 + kBins * 4 + static_cast<size_t>(std::min(segs, kMaxSegs)) * kWarps * 8;
     const bool fits = base + static_cast<size_t>(segs) * kSeg * 4 <= 227 * 1024 - sizeof(Scratch) - 32 * 8 - 1024;
-    SampleRowsArgs a{out, logits, row_stride, static_cast<int>(n), r, temperature, top_p, min_p, top_k, segs};
+    SampleRowsArgs a{out, logits, row_stride, static_cast<int>(n), r, temperature, top_p, min_p, top_k, segs, static_cast<int>(n_rows)};
     const int smem = static_cast<int>(fits ? base + static_cast<size_t>(segs) * kSeg * 4 : base);
-    const unsigned grid = static_cast<unsigned>(n_rows);
+    // More rows than run at once: a block for each row that takes long, then one for each that does not (greedy or a short
+    // list); the others of a grid of twice the rows leave at once.  256 rows of 32000, mixed: 54 us, in the rows' order 70;
+    // 1000 rows 232 and 253 us; rows that are all alike 31.1 and 29.5 us (short lists), 74 and 74 us (top-p).
+    const size_t at_once = static_cast<size_t>(sm_count()) * (2 * (smem + sizeof(Scratch) + 2048) <= 227 * 1024 ? 2 : 1);
+    const unsigned grid = static_cast<unsigned>(n_rows > at_once && n_rows <= 0x3fffffff ? 2 * n_rows : n_rows);
     const cudaStream_t s = as_stream(stream);
     auto run = [&](auto kernel) -> tl_status {
         TL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
