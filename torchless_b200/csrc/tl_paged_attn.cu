@@ -28,7 +28,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 #include "tl_paged_attn.cuh"
@@ -98,6 +97,7 @@ template <int R_, int KS>
 struct SplitPlan {
     static constexpr int R = R_;
     static constexpr int kTileCost = 24;
+    static constexpr bool kLookAgain = KS != 16;  // fp32, and head_dim 64
     static __device__ __forceinline__ int steps(const Tile& t) {
         return kTileCost + (t.hi <= t.lo ? 1 : (t.hi - 1) / KS - t.lo / KS + 1);
     }

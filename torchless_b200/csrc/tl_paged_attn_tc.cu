@@ -55,6 +55,7 @@ constexpr float kRescale = 8.f;  // log2 units
 struct ChunkPlan {
     static constexpr int R = kRows;
     static constexpr int kTileCost = 2;
+    static constexpr bool kLookAgain = false;
     static __device__ __forceinline__ int key_tiles(const Tile& t) {
         return t.hi <= t.lo ? 1 : (t.hi - 1) / kKB - t.lo / kKB + 1;
     }

@@ -295,7 +295,6 @@ struct Row {
     const void* x;   // the row in global memory
     int n, pad, segs;
     float top;
-    double c;        // weights are 2^((x - top) * c / 32)
     float bin_scale;
     unsigned long long* cells;  // sums of the weights of 128 positions: [segs][kWarps]
     __device__ __forceinline__ int bin(float f) const { return min(kBins - 1, static_cast<int>((top - f) * bin_scale)); }
@@ -814,7 +813,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleRowsArgs a) {
         const float top = logit_of(bk);
         const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f, r = a.r[row];
         const Scale ws{widen(top), 46.16624130844683 / static_cast<double>(temp), pow2};  // 32 / ln 2
-        const Row R{v, x, n, pad, a.segs, top, ws.c, kBins / (kDepth * temp), cells};
+        const Row R{v, x, n, pad, a.segs, top, kBins / (kDepth * temp), cells};
         answer = 0xffffffffu;
         if (a.segs <= kMaxSegs) answer = sample_row<T, SMEM>(R, ws, best, bk, lk, k, p, mp, r, list, hist, sc);
         if (answer == 0xffffffffu) {
