@@ -297,8 +297,10 @@ TL_API tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, c
  *   min_p  keeps those with w >= min_p (max has w = 1)  (<= 0 or NaN: off)
  * out[row] = the first kept index, in index order, whose running sum of kept w
  * reaches r x (sum of all kept w); r in [0, 1).  temperature <= 0 or NaN:
- * sample_max (main.cpp:10-21).  A row with a NaN or +inf logit, or with -inf
- * alone, gives n - 1 at a temperature > 0, as tl_sample_multinomial does.
+ * sample_max (main.cpp:10-21).  A logit of -inf has w = 0 at any temperature,
+ * infinity included, which gives all others w = 1.  A row with a NaN or +inf
+ * logit, or with -inf alone, gives n - 1 at a temperature > 0, as
+ * tl_sample_multinomial does.
  * Weights are fp64 rounded to multiples of 2^-40 and summed exactly, so the
  * result does not depend on the order of the sums.  logits: n values per row
  * in `dtype`, row_stride elements apart; n < 2^22.  No allocation. */

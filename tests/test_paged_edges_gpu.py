@@ -1,0 +1,54 @@
+"""Edges of the paged serving operators, against the plain 64-bit forms."""
+import math
+import os
+import subprocess
+import sys
+import threading
+
+import numpy as np
+import pytest
+
+import paged_plain as plain
+from test_paged_gpu import DT, TYPES, attend_case, check_attend, f32, f64, i32, ops, rope_case, run_sample, u
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    torch.cuda.set_device(0)
+
+
+def attend(q, kc, vc, table, q_start, lens, scale=None, window=0):
+    out = torch.full(q.shape, 3.0, device="cuda", dtype=q.dtype)
+    ops().paged_attention(out, q, kc, vc, i32(table), i32(q_start), i32(lens), scale, window)
+    return out
+
+
+# ---------------------------------------------------------------- sampling
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 3, 1001, 4093, 32001, 270001])
+def test_masked_logits_are_not_drawn_at_very_large_temperatures(dtype, n):
+    """All weights are 1 but those of -inf, which stay 0 at any temperature; rows begin off 16 bytes (odd n)."""
+    rng = np.random.default_rng(n)
+    temps = np.array([1e36, 1.3e37, 1e38, 3.4e38, np.inf], np.float32)
+    rows = 4 * len(temps)
+    x = rng.standard_normal((rows, n)).astype(np.float32)
+    x[rng.random((rows, n)) < 0.3] = -np.inf
+    x[::4] = rng.standard_normal((len(temps), n))
+    x[1::4, : n // 2] = -np.inf
+    x[:, n // 3] = 0.5
+    T = np.repeat(temps, 4)
+    t = torch.as_tensor(x).cuda().to(DT[dtype])
+    xs = t.float().cpu().numpy()
+    for k, p, m in ((0, 1.0, 0.0), (2, 1.0, 0.0), (700, 1.0, 0.5), (0, 0.37, 0.0), (900, 0.61, 1.0)):
+        for r in (0.0, 0.43, float(np.nextafter(np.float32(1), np.float32(0)))):
+            full = [np.full(rows, v, np.float32) for v in (r, p, m)]
+            got = ops().sample_rows(t, f32(full[0]), f32(T), i32(np.full(rows, k)), f32(full[1]), f32(full[2])).cpu().numpy()
+            # (x - max) / T of these rows is 0 to within 1e-35, and the quotient -inf / inf is read as -inf
+            want = [plain.sample(xs[i], r, min(T[i], np.float32(3.4e38)), k, p, m) for i in range(rows)]
+            np.testing.assert_array_equal(got, want, err_msg=str((k, p, m, r)))

@@ -1,5 +1,6 @@
 // tl_sample_rows.cu -- tl_sample_rows: temperature, top-k, top-p and min-p for
 // many rows, each with its own settings.
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -35,7 +36,8 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
 }
 
 // 32-bit to 64-bit floating point by integer operations (the conversion instruction runs at a quarter of the rate of
-// the 64-bit arithmetic).  Zero and subnormals become about 2^-127, infinity about 2^128: no weight changes by 2^-40.
+// the 64-bit arithmetic).  Zero and subnormals become about 2^-127: no weight changes by 2^-40.  Infinity becomes about
+// 2^128, which a large temperature brings near the other logits: the weight of -inf is 0 and never comes from here.
 __device__ __forceinline__ double widen(float x) {
     const uint32_t u = __float_as_uint(x);
     return __hiloint2double(static_cast<int>((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + (896u << 20))), static_cast<int>(u << 29));
@@ -58,7 +60,7 @@ struct Scale {
 
 // The weight of a logit as a multiple of 2^-40.  2^(t / 32) = 2^(k >> 5) 2^((k & 31) / 32) 2^(f / 32) with t = k + f,
 // |f| <= 1/2; the last factor by its series to the 5th power of f ln2 / 32 (what is left out is below 2^-48), all in
-// 64 bits, then rounded to a multiple of 2^-40 by adding 2^52.
+// 64 bits, then rounded to a multiple of 2^-40 by adding 2^52.  x is finite.
 __device__ __forceinline__ unsigned long long weight_of(float x, const Scale& s) {
     const double t = fmax((widen(x) - s.top) * s.c, -1400.0);  // 2^(-1400 / 32) rounds to 0
     const double magic = 6755399441055744.0;                   // 1.5 * 2^52: k in the low bits
@@ -74,6 +76,11 @@ __device__ __forceinline__ unsigned long long weight_of(float x, const Scale& s)
     q *= s.pow2[k & 31];
     const double v = __hiloint2double(__double2hiint(q) + (((k >> 5) + 40) << 20), __double2loint(q));
     return static_cast<unsigned long long>(__double_as_longlong(v + 4503599627370496.0)) & 0xfffffffffffffull;
+}
+
+// The same for any logit up to the largest: none of -inf, whatever the temperature.
+__device__ __forceinline__ unsigned long long weight_of_any(float x, const Scale& s) {
+    return x > -INFINITY ? weight_of(x, s) : 0ull;
 }
 
 __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long* red) {
@@ -144,10 +151,10 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
 #pragma unroll 1
         for (int i = tid; i < n; i += kThreads) {
             const float v = to_f32<T>(x[i]);
-            if (key_of(v) > kkey) sum += weight_of(v, ws);
+            if (key_of(v) > kkey) sum += weight_of_any(v, ws);
         }
         sum = block_sum_u64(sum, red);
-        if (kties != ~0ull) sum += kties * weight_of(logit_of(kkey), ws);
+        if (kties != ~0ull) sum += kties * weight_of_any(logit_of(kkey), ws);
         const double want = static_cast<double>(p) * static_cast<double>(sum);  // stop at the first prefix that reaches it
         uint32_t prefix = 0;
         unsigned long long above = 0;  // weight of the keys above the prefix's range
@@ -160,11 +167,11 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
                 const float v = to_f32<T>(x[i]);
                 const uint32_t u = key_of(v);
                 if (u > kkey && (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))))
-                    atomicAdd(&bins[(u >> shift) & 255], weight_of(v, ws));
+                    atomicAdd(&bins[(u >> shift) & 255], weight_of_any(v, ws));
             }
             __syncthreads();
             if (tid == 0 && kties != ~0ull && (shift == 24 || (kkey >> (shift + 8)) == (prefix >> (shift + 8))))
-                bins[(kkey >> shift) & 255] += kties * weight_of(logit_of(kkey), ws);
+                bins[(kkey >> shift) & 255] += kties * weight_of_any(logit_of(kkey), ws);
             __syncthreads();
             if (tid == 0) {
                 unsigned long long at = above;
@@ -181,7 +188,7 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
             above = sc.above;
             __syncthreads();
         }
-        const unsigned long long w = weight_of(logit_of(prefix), ws);
+        const unsigned long long w = weight_of_any(logit_of(prefix), ws);
         // ties of equal weight: as many as the sum still lacks, at least one
         unsigned long long m = 1;
         if (w > 0 && static_cast<double>(above) < want) {
@@ -218,7 +225,7 @@ __device__ __noinline__ uint32_t sample_by_radix(const T* x, int n, int k, float
         bool in = u > key;
         if (u == key) in = rank++ < ties;
         if (!in) return 0;
-        const unsigned long long w = weight_of(v, ws);
+        const unsigned long long w = weight_of_any(v, ws);
         return mp > 0.f && u != bk && static_cast<double>(w) < static_cast<double>(mp) * kOne ? 0 : w;
     };
     unsigned long long mine = 0, rank = before;
@@ -483,8 +490,8 @@ __device__ __forceinline__ unsigned long long kept_weights(const Row& R, const S
                                                            unsigned long long (&w)[4]) {
     float f[4];
     four<T, SMEM>(R, s, f);
-    const float cut_x = cut ? logit_at(cut) : -INFINITY;
-    const int cut_i = static_cast<int>(index_of(cut));
+    const float cut_x = cut ? logit_at(cut) : -INFINITY;  // (no cut: above -inf, which the padding holds too)
+    const int cut_i = cut ? static_cast<int>(index_of(cut)) : INT_MIN;
     unsigned long long sum = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -689,7 +696,7 @@ __device__ __forceinline__ uint32_t sample_row(const Row& R, const Scale& ws, ui
             __syncthreads();
             // exact: the weights above those bins, by cells, and of everything; the list of the bins between
             const float cut_x = cut ? logit_at(cut) : -INFINITY;
-            const int cut_i = static_cast<int>(index_of(cut));
+            const int cut_i = cut ? static_cast<int>(index_of(cut)) : INT_MIN;
             unsigned long long over = 0, sum = 0, over_all, sum_all;
             const int m = collect<T, SMEM>(
                 R, list, &sc.sel[3],
