@@ -52,3 +52,30 @@ def test_masked_logits_are_not_drawn_at_very_large_temperatures(dtype, n):
             # (x - max) / T of these rows is 0 to within 1e-35, and the quotient -inf / inf is read as -inf
             want = [plain.sample(xs[i], r, min(T[i], np.float32(3.4e38)), k, p, m) for i in range(rows)]
             np.testing.assert_array_equal(got, want, err_msg=str((k, p, m, r)))
+
+
+def test_sample_from_several_threads():
+    """Rows of two sizes, which take unlike amounts of shared memory, from host threads at once."""
+    from torchless_b200 import lib
+    rng = np.random.default_rng(1)
+    jobs, bad = [], []
+    for n in (777, 32000):
+        x = rng.standard_normal((1, n)).astype(np.float32)
+        r, T = rng.random(1).astype(np.float32), np.full(1, 0.9, np.float32)
+        jobs.append((torch.as_tensor(x).cuda(), f32(r), f32(T), plain.sample(x[0], r[0], T[0])))
+
+    def work(x, r, T, want):
+        side, out, L = torch.cuda.Stream(), i32([-1]), lib()
+        n, args = x.shape[1], (r.data_ptr(), T.data_ptr(), None, None, None, side.cuda_stream)
+        torch.cuda.synchronize()
+        status = [L.tl_sample_rows(out.data_ptr(), x.data_ptr(), 0, n, 1, n, *args) for _ in range(4000)]
+        side.synchronize()
+        if any(status) or out.item() != want:
+            bad.append((n, sum(map(bool, status)), out.item(), want))
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -850,7 +850,8 @@ extern "C" tl_status tl_sample_rows(uint32_t* out, const void* logits, tl_dtype 
     // up to 3 positions before the first logit align it; a segment more than shared memory holds: read from L2
     const int segs = static_cast<int>((n + 3 + kSeg - 1) / kSeg);
     const size_t base = kList * 8 + kBins * 4 + static_cast<size_t>(std::min(segs, kMaxSegs)) * kWarps * 8;
-    const bool fits = base + static_cast<size_t>(segs) * kSeg * 4 <= 227 * 1024 - sizeof(Scratch) - 32 * 8 - 1024;
+    constexpr size_t most = 227 * 1024 - sizeof(Scratch) - 32 * 8 - 1024;
+    const bool fits = base + static_cast<size_t>(segs) * kSeg * 4 <= most;
     SampleRowsArgs a{out, logits, row_stride, static_cast<int>(n), r, temperature, top_p, min_p, top_k, segs, static_cast<int>(n_rows)};
     const int smem = static_cast<int>(fits ? base + static_cast<size_t>(segs) * kSeg * 4 : base);
     // More rows than run at once: a block for each row that takes long, then one for each that does not (greedy or a short
@@ -860,7 +861,8 @@ extern "C" tl_status tl_sample_rows(uint32_t* out, const void* logits, tl_dtype 
     const unsigned grid = static_cast<unsigned>(n_rows > at_once && n_rows <= 0x3fffffff ? 2 * n_rows : n_rows);
     const cudaStream_t s = as_stream(stream);
     auto run = [&](auto kernel) -> tl_status {
-        TL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        // (the limit is the kernel's, not the launch's: another thread may be about to launch a longer row)
+        TL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
         kernel<<<grid, kThreads, smem, s>>>(a);
         return TL_OK;
     };
