@@ -294,7 +294,8 @@ TL_API tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, c
  *   top_k  keeps the first k of the order        (k <= 0 or >= n: off)
  *   top_p  keeps its shortest prefix whose sum reaches top_p x the sum of what
  *          top_k left (at least one)             (>= 1 or NaN: off)
- *   min_p  keeps those with w >= min_p (max has w = 1)  (<= 0 or NaN: off)
+ *   min_p  keeps those with w >= min_p (max has w = 1), the first of the order
+ *          alone if there is none              (<= 0 or NaN: off)
  * out[row] = the first kept index, in index order, whose running sum of kept w
  * reaches r x (sum of all kept w); r in [0, 1).  temperature <= 0 or NaN:
  * sample_max (main.cpp:10-21).  A logit of -inf has w = 0 at any temperature,

@@ -79,3 +79,14 @@ def test_sample_from_several_threads():
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("n", [7, 1500, 32000, 270000])
+def test_min_p_above_one_keeps_the_first_of_the_order(n):
+    """No weight reaches it: one logit is kept all the same, the largest with the lowest index."""
+    rng = np.random.default_rng(n)
+    x = rng.integers(0, 4, (4, n)).astype(np.float32)
+    r, T = np.array([0.0, 0.3, 0.7, 0.99], np.float32), np.full(4, 0.8, np.float32)
+    m = np.array([1.0001, 2.0, np.inf, 1.0], np.float32)
+    for k, p in ((None, None), ([3] * 4, None), ([n // 2] * 4, [0.9] * 4), (None, [0.5] * 4)):
+        run_sample(x, r, T, k, p, m)

@@ -818,7 +818,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_rows(SampleRowsArgs a) {
     uint32_t answer = static_cast<uint32_t>(n - 1);
     if (bk < 0xff800000u && bk > key_of(-INFINITY)) {  // neither NaN nor +inf, and something above -inf
         const float top = logit_of(bk);
-        const float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f, r = a.r[row];
+        float p = a.top_p ? a.top_p[row] : 1.f, mp = a.min_p ? a.min_p[row] : 0.f;
+        const float r = a.r[row];
+        if (mp > 1.f) p = mp = 0.f;  // no weight reaches it: the first of the order, as for a top-p of 0
         const Scale ws{widen(top), 46.16624130844683 / static_cast<double>(temp), pow2};  // 32 / ln 2
         const Row R{v, x, n, pad, a.segs, top, kBins / (kDepth * temp), cells};
         answer = 0xffffffffu;

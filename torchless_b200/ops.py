@@ -347,7 +347,7 @@ def sample_rows(logits, r, temperature, top_k=None, top_p=None, min_p=None):
     float16 or bfloat16; rows may be strided) with the row's own uniform draw
     ``r`` in [0, 1), ``temperature`` (<= 0: sample_max), and optionally
     ``top_k`` (int32; <= 0: off), ``top_p`` (>= 1: off) and ``min_p`` (<= 0:
-    off), applied in that order.  Returns the indexes, an int32 tensor [n_rows]."""
+    off; > 1: the largest alone), applied in that order.  Returns the indexes, an int32 tensor [n_rows]."""
     torch = _torch or _load()
     if logits.dim() != 2:
         raise ValueError("logits must be [n_rows, n] with contiguous rows")
