@@ -274,7 +274,7 @@ TL_API tl_status tl_qk_norm_rope(void* q_out, const tl_paged_cache* cache, const
  *        [n_heads][head_dim], both in the cache's dtype, not overlapping
  *   block_table [n_seq][max_blocks]; q_start [n_seq + 1], not decreasing
  * Rows outside q_start[0] .. q_start[n_seq] stay as they were.  Scores and sums
- * are fp32; with fp16 / bf16 caches the weights of the values are rounded to
+ * are fp32 (fp64, key by key, for rows whose scores pass it); with fp16 / bf16 caches the weights of the values are rounded to
  * that type for the tensor cores.  `workspace` holds the partial results
  * of split sequences: tl_paged_attention_workspace bytes, 16-byte aligned, its
  * contents need no preparation; calls that may overlap in time need one each.

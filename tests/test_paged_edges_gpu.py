@@ -90,3 +90,24 @@ def test_min_p_above_one_keeps_the_first_of_the_order(n):
     m = np.array([1.0001, 2.0, np.inf, 1.0], np.float32)
     for k, p in ((None, None), ([3] * 4, None), ([n // 2] * 4, [0.9] * 4), (None, [0.5] * 4)):
         run_sample(x, r, T, k, p, m)
+
+
+# ---------------------------------------------------------------- attention
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [[1, 1], [90, 33]])
+@pytest.mark.parametrize("scale", [1e6, 1e7, 1e9, 3e36, 1e37, -1e37, 2e38])
+def test_scores_that_pass_fp32_through_the_scale(dtype, new, scale):
+    """Products of small whole numbers are exact, so the largest has all the weight, however large the scale (ties share
+    it).  One kv head's products are all negative."""
+    q, kc, vc, table, q_start, ln = attend_case([90, 333], new, 8, 2, 64, 16, dtype)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q.copy_(torch.randint(1, 4, q.shape, generator=g, device="cuda"))
+    k = torch.randint(-3, 4, kc.shape, generator=g, device="cuda")
+    k[:, 1] = -k[:, 1].abs() - 1
+    kc.copy_(k)
+    out = attend(q, kc, vc, table, q_start, ln, scale)
+    want, ao, _, _, _ = plain.attend(f64(q), f64(kc), f64(vc), table, q_start, ln, scale, 0)
+    # the weights of the largest are alike and exact, the sum over ties (fewer than 64) and the quotient round in 32 bits
+    tol = u(DT[dtype]) * np.abs(want) * (1 + 2.0 ** -8) + 80 * 2.0 ** -24 * ao
+    assert np.all(np.abs(f64(out) - want) <= tol)

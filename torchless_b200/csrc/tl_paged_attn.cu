@@ -596,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // A result that is not finite: a value that one row must not see may have met it as 0 x infinity,
         // or an infinite value the split weights.  Such a tile is done over row by row, which gives the
-        // formula's result to each.  (Every finite input stays far from this.)  The same where a copy never came.
+        // formula's result to each.  The same where a score passed fp32's range or a copy never came, and for a row whose
+        // weights are all 0: it attends to nothing, or all its scores lie below that range.
         const bool redo = core.finish(c.t.nrows, lane) || dead;
         const bool whole = c.s == 0 && c.end == c.steps;
         float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * R * (HD + 4);
@@ -626,12 +627,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int tok, h;
                 row_of(a, c, row, tok, h);
                 if (whole) {
-                    if (any_redo) {
+                    if (any_redo || L == 0.f) {
                         attend_row<T, HD>(a, c.b, tok, h, lane);
                     } else {
                         T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + h) * HD;
 #pragma unroll
-                        for (int d = 0; d < HD / 32; d++) out[lane + 32 * d] = from_f32<T>(L != 0.f ? acc[d] / L : 0.f);
+                        for (int d = 0; d < HD / 32; d++) out[lane + 32 * d] = from_f32<T>(acc[d] / L);
                     }
                 } else {
                     float* pr = part + row * (HD + 4);

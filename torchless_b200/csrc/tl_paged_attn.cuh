@@ -279,8 +279,9 @@ __device__ __forceinline__ void row_of(const AttendArgs& a, const Cursor& c, int
     h = c.g * a.group + fr - i * a.group;
 }
 
-// One (token, head) by one warp, straight from the pages in fp32: lane l holds
-// dims l * HD / 32 ...  Reads the attended keys only.
+// One (token, head) by one warp, straight from the pages: lane l holds dims l * HD / 32 ...  Reads the attended keys only.
+// What the kernels' fp32 cannot hold comes here (scores beyond its range, rows whose weights all vanish, values that are
+// not finite), so scores and sums are 64-bit: products of three 32-bit numbers stay in range.
 template <typename T, int HD>
 __device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h, int lane) {
     constexpr int D = HD / 32;
@@ -291,35 +292,41 @@ __device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h
     attended(a, p, lo, hi);
     const int g = div_group(a, h);
     const T* qp = static_cast<const T*>(a.q) + static_cast<size_t>(t) * a.q_stride + static_cast<size_t>(h) * HD + lane * D;
-    float q[D], acc[D];
+    float q[D];
+    double acc[D], m = -INFINITY, l = 0.0;
 #pragma unroll
     for (int d = 0; d < D; d++) {
         q[d] = to_f32<T>(qp[d]);
-        acc[d] = 0.f;
+        acc[d] = 0.0;
     }
-    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
     for (int j = lo; j < hi; j++) {
         const int id = page_of(a, b, j);
-        if (id < 0) continue;
+        if (id < 0) {  // to the last position of the page
+            j |= (1 << a.shift) - 1;
+            continue;
+        }
         const size_t at = static_cast<size_t>(id) * a.block_stride +
                           ((static_cast<size_t>(g) << a.shift) + (j & ((1 << a.shift) - 1))) * HD + lane * D;
         const T* kp = static_cast<const T*>(a.k) + at;
         const T* vp = static_cast<const T*>(a.v) + at;
-        float s = 0.f;
+        double s = 0.0;
 #pragma unroll
-        for (int d = 0; d < D; d++) s += q[d] * to_f32<T>(kp[d]);
-        s = warp_sum(s) * a.scale;
-        const float mn = fmaxf(m, s);
-        const float f = m == -INFINITY ? 1.f : expf(m - mn);
-        const float e = s == -INFINITY ? 0.f : expf(s - mn);  // NaN stays NaN
+        for (int d = 0; d < D; d++) s += static_cast<double>(q[d]) * to_f32<T>(kp[d]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
+        s *= a.scale;
+        const double mn = fmax(m, s);
+        const float f = m == -INFINITY ? 1.f : expf(static_cast<float>(m - mn));
+        const float e = s == -INFINITY ? 0.f : expf(static_cast<float>(s - mn));  // NaN stays NaN
         m = mn;
         l = l * f + e;
 #pragma unroll
-        for (int d = 0; d < D; d++) acc[d] = acc[d] * f + e * to_f32<T>(vp[d]);
+        for (int d = 0; d < D; d++) acc[d] = acc[d] * f + static_cast<double>(e) * to_f32<T>(vp[d]);
     }
     T* op = static_cast<T*>(a.out) + (static_cast<size_t>(t) * a.H + h) * HD + lane * D;
 #pragma unroll
-    for (int d = 0; d < D; d++) op[d] = from_f32<T>(l != 0.f ? acc[d] / l : 0.f);
+    for (int d = 0; d < D; d++) op[d] = from_f32<T>(static_cast<float>(l != 0.0 ? acc[d] / l : 0.0));
 }
 
 constexpr int kJoinWarps = 8;
@@ -400,15 +407,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attend_join(const __grid_co
             int tok, hh;
             row_of(a, c, row, tok, hh);
             const float mx = fmaxf(M, x[0]), f0 = mx == -INFINITY ? 1.f : ex2(M - mx), f1 = mx == -INFINITY ? 1.f : ex2(x[0] - mx);
-            if (bad > 0.f || x[1] != x[1]) {
+            const float sum = L * f0 + x[1] * f1;
+            if (bad > 0.f || x[1] != x[1] || sum == 0.f) {
                 attend_row<T, HD>(a, h.b, tok, hh, lane);
             } else {
-                const float sum = L * f0 + x[1] * f1;
                 T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD;
 #pragma unroll
                 for (int d = 0; d < D; d++) {
                     const float o = acc[d] * f0 + x[2 + lane + 32 * d] * f1;
-                    out[lane + 32 * d] = from_f32<T>(sum != 0.f ? o / sum : 0.f);
+                    out[lane + 32 * d] = from_f32<T>(o / sum);
                 }
             }
         }

@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(FULL, l[i], x);
             if (r < c.t.nrows) {
                 float4 v[NC];
-                float z = l[i] * 0.f;  // NaN once a value is not finite: the row is done over
+                // NaN once a value is not finite, or a whole row's weights are all 0: the row is done over
+                float z = whole && l[i] == 0.f ? NAN : l[i] * 0.f;
 #pragma unroll
                 for (int j = 0; j < NC; j++) {
                     const float2 x = halves(o[i][j][0]), y = halves(o[i][j][1]);
@@ -258,9 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                                    : part + r * (HD + 4) + 4;
 #pragma unroll
                 for (int j = 0; j < NC; j++) {
-                    if (whole)
-                        v[j] = l[i] != 0.f ? make_float4(v[j].x / l[i], v[j].y / l[i], v[j].z / l[i], v[j].w / l[i])
-                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (whole) v[j] = make_float4(v[j].x / l[i], v[j].y / l[i], v[j].z / l[i], v[j].w / l[i]);
                     *reinterpret_cast<float4*>(dst + 64 * j + 4 * tx) = v[j];
                 }
                 if (!whole && tx == 0) *reinterpret_cast<float2*>(dst - 4) = make_float2(m[i], l[i]);

@@ -640,6 +640,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             xl[(2 * i + hf) * 128 + r] = l;
             const bool good = stream_sync(i, ok);
             float w0 = 1.f, w1 = 0.f, mt = m, lt = xl[2 * i * 128 + r] + xl[(2 * i + 1) * 128 + r];
+            // The largest weight is 2^-0 to 2^8, but for what m was rounded by, which the exact products in the exponents
+            // bring back: scores beyond 2^24 may lose all their weights by that, and infinite ones do.
+            if ((lt > 0.f && lt < 0.5f) || m == INFINITY) lt = NAN;
             if (fold) {
                 stream_sync(i, true);
                 xl[(2 * i + hf) * 128 + r] = !good ? NAN : hf ? lt : m;
@@ -663,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * kRows * (HD + 4);
             if (writer) {
                 const float inv = lt != 0.f ? 1.f / lt : 0.f;
-                float z = lt * 0.f;  // NaN once a value is not finite
+                float z = whole && lt == 0.f ? NAN : lt * 0.f;  // NaN once a value is not finite (or nothing has weight)
                 const bool t0 = fine && (fold || act);
                 const uint32_t ta = fold ? tO + lane_off : to;
 #pragma unroll 1
@@ -707,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
                 }
-                // not finite: a value that this row must not see may have met it as 0 x infinity (see tl_paged_attn.cu)
+                // do over: a value that this row must not see may have met it as 0 x infinity (see tl_paged_attn.cu)
                 const bool redo = in && z != z;
                 if (whole) {
                     __syncwarp();
@@ -809,7 +812,7 @@ __global__ void __launch_bounds__(256) k_attend_chunk_join(const __grid_constant
             }
         }
     }
-    float z = L * 0.f;  // NaN once a value is not finite: the row is done over
+    float z = L != 0.f ? L * 0.f : NAN;  // NaN once a value is not finite, or nothing has weight: the row is done over
     const float inv = L != 0.f ? 1.f / L : 0.f;
 #pragma unroll
     for (int g = 0; g < G; g++) {
