@@ -111,3 +111,14 @@ def test_scores_that_pass_fp32_through_the_scale(dtype, new, scale):
     # the weights of the largest are alike and exact, the sum over ties (fewer than 64) and the quotient round in 32 bits
     tol = u(DT[dtype]) * np.abs(want) * (1 + 2.0 ** -8) + 80 * 2.0 ** -24 * ao
     assert np.all(np.abs(f64(out) - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,new", [([50, 200], [1, 1]), ([6000], [1]), ([140, 50], [140, 40]), ([3000, 40], [30, 20])])
+def test_values_near_the_largest_of_the_type(dtype, lens, new):
+    """A mean of finite values is finite, although their sum is not."""
+    q, kc, vc, table, q_start, ln = attend_case(lens, new, 4, 1, 64, 16, dtype)
+    vc[..., 3] = 3e38
+    vc[..., 7] = torch.where(torch.rand(vc.shape[:-1], device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) < 0.5,
+                             3e38, -3e38).to(vc.dtype)
+    check_attend(attend(q, kc, vc, table, q_start, ln), q, kc, vc, table, q_start, ln, dtype)

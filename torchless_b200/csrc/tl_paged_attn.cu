@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();  // every lane has read the stage
         }
         // A result that is not finite: a value that one row must not see may have met it as 0 x infinity,
-        // or an infinite value the split weights.  Such a tile is done over row by row, which gives the
+        // or an infinite value the split weights, or values near the type's largest add up to more.  Such a tile is done over row by row, which gives the
         // formula's result to each.  The same where a score passed fp32's range or a copy never came, and for a row whose
         // weights are all 0: it attends to nothing, or all its scores lie below that range.
         const bool redo = core.finish(c.t.nrows, lane) || dead;
@@ -624,10 +624,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int d = 0; d < HD / 32; d++) acc[d] += j[w * S::JOIN + 4 + lane + 32 * d] * f;
                 }
+                float z = L * 0.f;  // NaN once the sum over the warps is not finite
+#pragma unroll
+                for (int d = 0; d < HD / 32; d++) z = fmaf(acc[d], 0.f, z);
+                const bool over = any_redo || __any_sync(FULL, z != z);
                 int tok, h;
                 row_of(a, c, row, tok, h);
                 if (whole) {
-                    if (any_redo || L == 0.f) {
+                    if (over || L == 0.f) {
                         attend_row<T, HD>(a, c.b, tok, h, lane);
                     } else {
                         T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + h) * HD;
@@ -639,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) {
                         pr[0] = M;
                         pr[1] = L;
-                        pr[2] = any_redo ? 1.f : 0.f;
+                        pr[2] = over ? 1.f : 0.f;
                     }
 #pragma unroll
                     for (int d = 0; d < HD / 32; d++) pr[4 + lane + 32 * d] = acc[d];

@@ -408,15 +408,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_attend_join(const __grid_co
             row_of(a, c, row, tok, hh);
             const float mx = fmaxf(M, x[0]), f0 = mx == -INFINITY ? 1.f : ex2(M - mx), f1 = mx == -INFINITY ? 1.f : ex2(x[0] - mx);
             const float sum = L * f0 + x[1] * f1;
-            if (bad > 0.f || x[1] != x[1] || sum == 0.f) {
+            float o[D], z = 0.f;  // NaN once a sum is not finite
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+                o[d] = acc[d] * f0 + x[2 + lane + 32 * d] * f1;
+                z = fmaf(o[d], 0.f, z);
+            }
+            if (bad > 0.f || x[1] != x[1] || sum == 0.f || __any_sync(FULL, z != z)) {
                 attend_row<T, HD>(a, h.b, tok, hh, lane);
             } else {
                 T* out = static_cast<T*>(a.out) + (static_cast<size_t>(tok) * a.H + hh) * HD;
 #pragma unroll
-                for (int d = 0; d < D; d++) {
-                    const float o = acc[d] * f0 + x[2 + lane + 32 * d] * f1;
-                    out[lane + 32 * d] = from_f32<T>(o / sum);
-                }
+                for (int d = 0; d < D; d++) out[lane + 32 * d] = from_f32<T>(o[d] / sum);
             }
         }
         __syncthreads();
