@@ -122,3 +122,20 @@ def test_values_near_the_largest_of_the_type(dtype, lens, new):
     vc[..., 7] = torch.where(torch.rand(vc.shape[:-1], device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) < 0.5,
                              3e38, -3e38).to(vc.dtype)
     check_attend(attend(q, kc, vc, table, q_start, ln), q, kc, vc, table, q_start, ln, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,ln", [(64, 300), (30, 300), (30, 100)])
+def test_a_column_that_is_not_finite_leaves_the_other_half_alone(dtype, n, ln):
+    """As many equal row tiles as SMs, so that each block has a whole one.  The threads that hold the columns of the other
+    half do not see the infinity, and what they write must not depend on who is faster."""
+    seqs = torch.cuda.get_device_properties(0).multi_processor_count
+    q, kc, vc, table, q_start, lens = attend_case([ln] * seqs, [n] * seqs, 4, 1, 128, 16, dtype)
+    clean = attend(q, kc, vc, table, q_start, lens)
+    for b in range(seqs):
+        vc[table[b, (ln - 3) // 16], 0, (ln - 3) % 16, 5] = float("inf")
+    for _ in range(5):
+        out = attend(q, kc, vc, table, q_start, lens)
+        assert torch.equal(out[..., 64:], clean[..., 64:])
+        rows = out.view(seqs, n, 4, 128)
+        assert torch.isfinite(rows[:, : n - 3]).all() and torch.isposinf(rows[:, n - 3:, :, 5]).all()

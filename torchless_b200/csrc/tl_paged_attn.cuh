@@ -281,9 +281,10 @@ __device__ __forceinline__ void row_of(const AttendArgs& a, const Cursor& c, int
 
 // One (token, head) by one warp, straight from the pages: lane l holds dims l * HD / 32 ...  Reads the attended keys only.
 // What the kernels' fp32 cannot hold comes here (scores beyond its range, rows whose weights all vanish, values that are
-// not finite), so scores and sums are 64-bit: products of three 32-bit numbers stay in range.
+// not finite), so scores and sums are 64-bit: products of three 32-bit numbers stay in range.  Columns [c0, c1) are
+// written (multiples of HD / 32).
 template <typename T, int HD>
-__device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h, int lane) {
+__device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h, int lane, int c0 = 0, int c1 = HD) {
     constexpr int D = HD / 32;
     int first, n;
     rows_of(a, b, first, n);
@@ -324,6 +325,7 @@ __device__ __noinline__ void attend_row(const AttendArgs& a, int b, int t, int h
 #pragma unroll
         for (int d = 0; d < D; d++) acc[d] = acc[d] * f + static_cast<double>(e) * to_f32<T>(vp[d]);
     }
+    if (lane * D < c0 || lane * D >= c1) return;
     T* op = static_cast<T*>(a.out) + (static_cast<size_t>(t) * a.H + h) * HD + lane * D;
 #pragma unroll
     for (int d = 0; d < D; d++) op[d] = from_f32<T>(static_cast<float>(l != 0.0 ? acc[d] / l : 0.0));

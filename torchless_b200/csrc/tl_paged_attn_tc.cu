@@ -710,14 +710,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
                 }
-                // do over: a value that this row must not see may have met it as 0 x infinity (see tl_paged_attn.cu)
+                // do over: a value that this row must not see may have met it as 0 x infinity (see tl_paged_attn.cu).
+                // These columns only: the row's others are other warps', which may not see it and write theirs.
                 const bool redo = in && z != z;
                 if (whole) {
                     __syncwarp();
                     for (unsigned bad = __ballot_sync(FULL, redo); bad; bad &= bad - 1) {
                         const int src = __ffs(bad) - 1;
                         __syncwarp();
-                        attend_row<T, HD>(a, c.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, h, src), lane);
+                        attend_row<T, HD>(a, c.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, h, src), lane, c0, c1);
                     }
                 } else if (in && hf == 0 && (!fold || i == 0)) {
                     *reinterpret_cast<float2*>(part + 4 * row) = make_float2(mt, lt);
