@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (unsigned bad = __ballot_sync(FULL, redo); bad; bad &= bad - 1) {
                         const int src = __ffs(bad) - 1;
                         __syncwarp();
-                        attend_row<T, HD>(a, c.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, h, src), lane, c0, c1);
+                        attend_row<T, HD>(a, c.b, __shfl_sync(FULL, tok, src), __shfl_sync(FULL, h, src), lane, c0 | (c1 << 16));
                     }
                 } else if (in && hf == 0 && (!fold || i == 0)) {
                     *reinterpret_cast<float2*>(part + 4 * row) = make_float2(mt, lt);
