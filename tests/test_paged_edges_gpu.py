@@ -139,3 +139,27 @@ def test_a_column_that_is_not_finite_leaves_the_other_half_alone(dtype, n, ln):
         assert torch.equal(out[..., 64:], clean[..., 64:])
         rows = out.view(seqs, n, 4, 128)
         assert torch.isfinite(rows[:, : n - 3]).all() and torch.isposinf(rows[:, n - 3:, :, 5]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 20])
+@pytest.mark.parametrize("n", [2500, 20000])
+def test_many_small_weights_add_up(dtype, rows, n):
+    """One key with nearly all the weight and n of 2^-25.2 each: the small ones are the whole result.  As many sequences
+    (over the same pages) as SMs, so that a block has the whole of one."""
+    hd, bs = 64, 16
+    seqs = torch.cuda.get_device_properties(0).multi_processor_count
+    table = np.tile(np.arange(-(-n // bs), dtype=np.int32), (seqs, 1))
+    kc = torch.zeros(table.shape[1], 1, bs, hd, device="cuda", dtype=DT[dtype])
+    vc = torch.ones_like(kc)
+    kc[..., 0] = -17.5
+    kc[0, 0, 0], vc[0, 0, 0] = 0, 0
+    q = torch.zeros(rows * seqs, 1, hd, device="cuda", dtype=DT[dtype])
+    q[..., 0] = 1
+    out = f64(attend(q, kc, vc, table, rows * np.arange(seqs + 1), [n] * seqs, 1.0))
+    w = np.tile(n - rows + np.arange(rows), seqs) * math.exp(-17.5)  # the keys of the small weight
+    want = (w / (1 + w))[:, None, None]
+    # the score and its factor log2(e) round to 2^-24 of 25.2 log2 units (ln 2 of that in the weight), the weight and the
+    # result round to the type, and the running sums to 32 bits, one step a key at worst
+    rel = 4 * 25.2 * 2.0 ** -24 + n * 2.0 ** -24 + (3 * u(DT[dtype]) if dtype != "f32" else 0)
+    assert np.all(np.abs(out - want) <= rel * want)

@@ -157,6 +157,9 @@ template <typename T, int HD, int R>
 struct Core {
     static_assert(R == 16, "the instruction's height");
     static constexpr int NO = HD / 8;
+    // fp16 ends at 2^-24, and many weights below that may add up to a result: they are formed, and summed, 2^15 times as
+    // large, which the largest of 1 has room for.  bf16 has fp32's range.
+    static constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
     uint32_t q[HD / 16][4];
     float o[NO][4];
     float m[2], l[2];
@@ -276,7 +279,7 @@ struct Core {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) s[n][2 * i + e] = ex2(s[n][2 * i + e] - base);
+                for (int e = 0; e < 2; e++) s[n][2 * i + e] = ex2(s[n][2 * i + e] - base + kLift);
                 sum += s[n][2 * i] + s[n][2 * i + 1];
             }
             l[i] = l[i] * f[i] + sum;

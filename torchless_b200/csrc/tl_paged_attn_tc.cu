@@ -7,7 +7,7 @@
 // rows of one kv head at a time, as two streams of 128 rows that share every
 // K / V tile:
 //   S_i[128 x 128] = Q_i K^T      tcgen05.mma, tensor memory
-//   P_i            = 2^(S_i scale - m_i)   two threads a row, 16-bit, over S_i
+//   P_i            = 2^(S_i scale - m_i)   two threads a row, 16-bit, over S_i (fp16: 2^11 times as large)
 //   O_i[128 x hd] += P_i V        tcgen05.mma, P_i from tensor memory
 // While the threads of one stream take exponentials, the matrix unit works for
 // the other.  A tile of at most 128 rows (the tail of a chunk, a single token
@@ -17,7 +17,9 @@
 //     lies: nothing is transposed.
 //   - The row maximum moves only when it grows by more than 2^8 (then O is
 //     rescaled in tensor memory); exponents up to 2^8 stay in 16 bits' range and
-//     the final O / l is exact all the same.
+//     the final O / l is exact all the same.  fp16 ends at 2^-24, and many weights
+//     below that may add up to a result: there it moves from 2^4 on, and weights
+//     and sums are 2^11 times as large.
 //   - Persistent blocks with equal shares of the key tiles (tl_paged_attn.cuh);
 //     a row tile that two blocks share is joined by a second kernel.
 // Warps: 0-7 stream 0, 8-15 stream 1 (softmax and epilogue: a row's first 64 keys and first columns by warps 0-3
@@ -47,7 +49,12 @@ using namespace tc;
 
 constexpr int kRows = 256, kHalf = 128, kKB = 128;
 constexpr int kWarps = 20, kThreads = kWarps * 32;
-constexpr float kRescale = 8.f;  // log2 units
+template <typename T>
+struct Range {  // log2 units
+    static constexpr float kRescale = std::is_same<T, __half>::value ? 4.f : 8.f;
+    static constexpr float kLift = std::is_same<T, __half>::value ? 11.f : 0.f;
+    static constexpr float kLeast = std::is_same<T, __half>::value ? 1024.f : 0.5f;  // half of the largest weight's least
+};
 
 // One step: 256 rows x 128 keys, or (tiles of at most 128 rows) 128 rows x 256 keys.  Beginning and ending a
 // tile takes about as long as kTileCost steps, which count as steps before its first key tile (2048 tokens of 4096 / 9
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!good) continue;
                     const float top = fmaxf(own, xl[(2 * i + (hf ^ 1)) * 128 + r]);
                     float f = 1.f;
-                    if (top > m + kRescale || (m == -INFINITY && top > -INFINITY)) {
+                    if (top > m + Range<T>::kRescale || (m == -INFINITY && top > -INFINITY)) {
                         if (m != -INFINITY) f = ex2(m - top);
                         m = top;
                     }
@@ -589,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         asm volatile("bar.sync %0, 64;" ::"r"(3 + 4 * i + (warp & 3)) : "memory");
                     }
                     // masked scores and rows that see nothing: 2^(-inf) = 0
-                    const float base = m == -INFINITY ? 0.f : -m;
+                    const float base = m == -INFINITY ? 0.f : Range<T>::kLift == 0.f ? -m : Range<T>::kLift - m;
                     if (key0 < c.t.lo || key0 > c.t.hi - 64) {
                         // rows of V that no query attends to may hold anything: no 0 x NaN.  (Both streams
                         // write the same zeros; each before its own product.)
@@ -640,9 +647,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             xl[(2 * i + hf) * 128 + r] = l;
             const bool good = stream_sync(i, ok);
             float w0 = 1.f, w1 = 0.f, mt = m, lt = xl[2 * i * 128 + r] + xl[(2 * i + 1) * 128 + r];
-            // The largest weight is 2^-0 to 2^8, but for what m was rounded by, which the exact products in the exponents
-            // bring back: scores beyond 2^24 may lose all their weights by that, and infinite ones do.
-            if ((lt > 0.f && lt < 0.5f) || m == INFINITY) lt = NAN;
+            // The largest weight is 2^kLift at least, but for what m was rounded by, which the exact products in the
+            // exponents bring back: scores beyond 2^24 may lose all their weights by that, and infinite ones do.
+            if ((lt > 0.f && lt < Range<T>::kLeast) || m == INFINITY) lt = NAN;
             if (fold) {
                 stream_sync(i, true);
                 xl[(2 * i + hf) * 128 + r] = !good ? NAN : hf ? lt : m;
