@@ -263,7 +263,7 @@ TL_API tl_status tl_qk_norm_rope(void* q_out, const tl_paged_cache* cache, const
 /* Causal GQA attention of new tokens over the pages (modules.cpp:65-88 for
  * many sequences; q head h reads kv head h / (n_heads / n_kv_heads)).
  * Sequence b has the query rows q_start[b] .. q_start[b + 1) and seq_lens[b]
- * cached tokens, the queries' own among them: its i-th query of n stands at
+ * cached tokens (below 0: none), the queries' own among them: its i-th query of n stands at
  * position p = seq_lens[b] - n + i and attends to the positions
  * max(0, p - window + 1) .. p (window 0: all of 0 .. p) whose table entry
  * names a page of the cache.  What is not attended (other sequences' pages,

@@ -163,3 +163,15 @@ def test_many_small_weights_add_up(dtype, rows, n):
     # result round to the type, and the running sums to 32 bits, one step a key at worst
     rel = 4 * 25.2 * 2.0 ** -24 + n * 2.0 ** -24 + (3 * u(DT[dtype]) if dtype != "f32" else 0)
     assert np.all(np.abs(out - want) <= rel * want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 20, 33, 25]])
+def test_lengths_below_zero(dtype, new):
+    """Queries of a length at or near the smallest whole number stand before position 0: zeros."""
+    q, kc, vc, table, q_start, ln = attend_case([90, 64, 64, 64], new, 8, 2, 64, 16, dtype)
+    ln[1:] = -2 ** 31, -2 ** 31 + 10, -1
+    for window in (0, 20):
+        out = attend(q, kc, vc, table, q_start, ln, window=window)
+        check_attend(out, q, kc, vc, table, q_start, ln, dtype, window=window)
+        assert (out[q_start[1]:] == 0).all()

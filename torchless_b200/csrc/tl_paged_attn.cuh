@@ -46,8 +46,9 @@ __device__ __forceinline__ void rows_of(const AttendArgs& a, int b, int& first, 
     n = max(0, min(a.q_start[b + 1], a.n_tokens) - first);
 }
 
-// Position of the first query row of a sequence with n of them.
-__device__ __forceinline__ int first_pos(const AttendArgs& a, int b, int n) { return min(a.seq_lens[b], kMaxLen) - n; }
+// Position of the first query row of a sequence with n of them.  (A length below 0 leaves all of them before position 0, as
+// 0 does, and less n it could pass the smallest whole number.)
+__device__ __forceinline__ int first_pos(const AttendArgs& a, int b, int n) { return min(max(a.seq_lens[b], 0), kMaxLen) - n; }
 
 // Positions [lo, hi) that the query at position p of a sequence may attend to
 // (pages that do not exist are left out later, key by key).
