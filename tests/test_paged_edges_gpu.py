@@ -175,3 +175,36 @@ def test_lengths_below_zero(dtype, new):
         out = attend(q, kc, vc, table, q_start, ln, window=window)
         check_attend(out, q, kc, vc, table, q_start, ln, dtype, window=window)
         assert (out[q_start[1]:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [1, 30])
+def test_one_kv_head_and_one_page_in_any_layout(dtype, tokens):
+    """A dimension of size 1 has no layout: a cache kept as [n_blocks, block_size, 1, head_dim] is the same pages, and K may
+    come that way beside V in its own."""
+    q, kc, vc, table, q_start, ln = attend_case([60, 40], [tokens, tokens], 4, 1, 64, 16, dtype)
+
+    def turn(c):
+        return torch.empty(c.shape[0], 16, 1, 64, device="cuda", dtype=c.dtype).copy_(c.transpose(1, 2)).transpose(1, 2)
+
+    turned = turn(kc)
+    assert turned.shape == kc.shape and turned.stride(1) == 64
+    want = attend(q, kc, vc, table, q_start, ln)
+    assert torch.equal(attend(q, turned, vc, table, q_start, ln), want)
+    assert torch.equal(attend(q, turned, turn(vc), table, q_start, ln), want)
+    # one page
+    kk, vv = kc[table[1, 0]][None], vc[table[1, 0]].clone()[None]
+    odd = torch.empty(5, *kk.shape[1:], device="cuda", dtype=kk.dtype)[:1].copy_(vv)
+    odd = odd.as_strided(odd.shape, (3, *odd.stride()[1:]))
+    one = [np.zeros((1, 1), np.int32), [0, tokens], [16]]
+    assert torch.equal(attend(q[:tokens], kk, odd, *one), attend(q[:tokens], kk, vv, *one))
+
+
+def test_pages_that_are_not_contiguous_are_refused():
+    kc = torch.zeros(6, 2, 16, 64, device="cuda")
+    q = torch.zeros(1, 4, 64, device="cuda")
+    for bad in (kc.transpose(1, 2).contiguous().transpose(1, 2), kc[:, :, ::2], torch.zeros(6, 2, 16, 128, device="cuda")[..., ::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            attend(q, bad, bad, np.zeros((1, 1), np.int32), [0, 1], [1])
+    with pytest.raises(ValueError, match="layout"):  # unlike strides between the pages
+        attend(q, kc[::2], kc[:3], np.zeros((1, 1), np.int32), [0, 1], [1])

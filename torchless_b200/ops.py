@@ -216,16 +216,19 @@ def _arg(t, dtype, index, n, name):
 
 def _cache(k_cache, v_cache):
     """The pages as the library's structure, and their device."""
-    shape, st, index = k_cache.shape, k_cache.stride(), k_cache.get_device()
-    if len(shape) != 4 or shape != v_cache.shape or st != v_cache.stride():
+    shape, st, sv, index = k_cache.shape, k_cache.stride(), v_cache.stride(), k_cache.get_device()
+    if len(shape) != 4 or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must be [n_blocks, n_kv_heads, block_size, head_dim] of one layout")
     if index < 0 or v_cache.get_device() != index or k_cache.dtype is not v_cache.dtype:
         raise ValueError("k_cache and v_cache must be CUDA tensors of one type and device")
     n, kv, bs, hd = shape
-    if st[1] != bs * hd or st[2] != hd or st[3] != 1:
-        raise ValueError("the pages of a cache must be contiguous")
+    if n > 1 and st[0] != sv[0]:
+        raise ValueError("k_cache and v_cache must be of one layout")
+    inside = (bs * hd, hd, 1)
+    if n and (st[1:] != inside or sv[1:] != inside) and not (k_cache[0].is_contiguous() and v_cache[0].is_contiguous()):
+        raise ValueError("the pages of a cache must be contiguous")  # (a dimension of size 1 may have any stride)
     return tl_paged_cache(k_cache.data_ptr(), v_cache.data_ptr(), n, kv, bs, hd,
-                          st[0] if n > 1 else max(st[0], kv * bs * hd), _dtype(k_cache)), index
+                          st[0] if n > 1 else kv * bs * hd, _dtype(k_cache)), index
 
 
 def paged_plan(block_table, cached, new_tokens, free_blocks, block_size: int, n_tokens: int):
