@@ -208,3 +208,17 @@ def test_pages_that_are_not_contiguous_are_refused():
             attend(q, bad, bad, np.zeros((1, 1), np.int32), [0, 1], [1])
     with pytest.raises(ValueError, match="layout"):  # unlike strides between the pages
         attend(q, kc[::2], kc[:3], np.zeros((1, 1), np.int32), [0, 1], [1])
+
+
+# ---------------------------------------------------------------- waits that run out
+
+def child(kind, polls):
+    env = dict(os.environ, **({} if polls is None else dict(TL_PAGED_WAIT_POLLS=str(polls))))
+    r = subprocess.run([sys.executable, os.path.join(os.path.dirname(__file__), "paged_waits_child.py"), kind], env=env,
+                       capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and f"right {polls}" in r.stdout, r.stdout[-500:] + r.stderr[-3000:]
+
+
+@pytest.mark.parametrize("polls", [None, 0, 1, 20, 100])
+def test_decode_rows_whose_copies_were_not_waited_for_are_done_over(polls):
+    child("decode", polls)

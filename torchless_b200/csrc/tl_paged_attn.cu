@@ -28,6 +28,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "tl_paged_attn.cuh"
@@ -69,14 +70,16 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
-// Waits by polling (the copies are short, and a suspended wait may wake late); false after ~2 s.
-__device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity) {
+// Waits by polling (the copies are short, and a suspended wait may wake late); false after ~2 s, or that many polls.
+__device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity, unsigned polls) {
+    if (polls == 0) return false;
     if (bar_test_now(b, parity)) return true;
     const unsigned long long t0 = gtime();
-    for (unsigned i = 1;; i++) {
+    for (unsigned i = 1; i != polls; i++) {
         if (bar_test_now(b, parity)) return true;
         if ((i & 255) == 0 && gtime() - t0 > kTimeoutNs) return false;
     }
+    return false;
 }
 
 // Keys per step, stages per warp, and the bytes of one side of a stage.
@@ -583,7 +586,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (s >= c.end - P::kTileCost) break;
             if (ahead == 0) continue;  // (a copy never came: no further ones)
-            dead |= !spin(&bars[got_st], (got_parity >> got_st) & 1);
+            // (the outcome is the whole warp's: what follows exchanges values between its lanes)
+            if (!__all_sync(FULL, spin(&bars[got_st], (got_parity >> got_st) & 1, a.polls))) {
+                dead = true;  // and the copies on their way land before anything else happens to their stages
+                for (; ahead > 0; ahead--) {
+                    bar_wait(&bars[got_st], (got_parity >> got_st) & 1);
+                    got_parity ^= 1u << got_st;
+                    got_st = got_st + 1 == NST ? 0 : got_st + 1;
+                }
+                continue;
+            }
             got_parity ^= 1u << got_st;
             StepInfo si;
             si.valid = (valid_bits >> (NT * got_st)) & ((1u << NT) - 1);
@@ -714,6 +726,16 @@ using namespace tl;
 using namespace tl::paged;
 
 namespace {
+// TL_PAGED_WAIT_POLLS: a limit on the polls of the kernels' waits, for tests of what follows when one runs out.
+unsigned wait_polls() {
+    static const unsigned polls = [] {
+        const char* e = std::getenv("TL_PAGED_WAIT_POLLS");
+        const long v = e ? std::atol(e) : -1;
+        return v >= 0 && v < 0x7fffffff ? static_cast<unsigned>(v) : kNoPollLimit;
+    }();
+    return polls;
+}
+
 // Rows per sequence and kv head, on average, from which the kernels for chunks pay: this file's kernel reads all keys
 // once for every 16 rows, theirs for every 256 (fp32: 64).  32 heads, 8 kv heads, hd 128, 64 x 4096 keys, bf16 / fp32:
 // 16 rows 180 / 905 us here and 205 / 1630 us there, 20 rows 343 / 1763 and 212 / 1631; 16 x 1000 keys: 16 rows
@@ -784,6 +806,7 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.cap = static_cast<int>(std::min<size_t>(max_blocks << a.shift, kMaxLen));
     a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
     a.scale = scale == 0.f ? 1e-45f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
+    a.polls = wait_polls();
     if (!many_rows(cache, n_tokens, n_heads, n_seq)) return attend_split(a, cache, workspace, as_stream(stream));
     return cache->dtype == TL_F32 ? attend_chunk_f32(a, cache, workspace, as_stream(stream))
                                   : attend_chunk(a, cache, workspace, as_stream(stream));

@@ -26,7 +26,9 @@ struct AttendArgs {
     int window;   // 0: none
     float scale;
     unsigned long long group_inv;  // ceil(2^64 / group)
+    unsigned polls;  // after so many a role's wait gives up, as it does after about 2 s (kNoPollLimit: only then)
 };
+constexpr unsigned kNoPollLimit = 0xffffffffu;
 
 // r / group, r >= 0 (exact: r < 2^32, and the inverse is off by less than 2^-32 relative)
 __device__ __forceinline__ int div_group(const AttendArgs& a, int r) {
