@@ -1,5 +1,5 @@
-"""Paged attention in a process whose kernels' waits give up after TL_PAGED_WAIT_POLLS polls (read once a process):
-rows whose copies or products were not waited for are done over, and come out right all the same.
+"""Paged attention in a process where about one in TL_PAGED_FAIL_WAITS waits of the kernels gives up (read once a
+process): rows whose copies or products were not waited for are done over, and come out right all the same.
 
     python paged_waits_child.py decode|chunks
 """
@@ -29,7 +29,7 @@ def done_over(new):
 
 
 def main(kind):
-    polls = os.environ.get("TL_PAGED_WAIT_POLLS")
+    one_in = os.environ.get("TL_PAGED_FAIL_WAITS")
     for dtype in TYPES if kind == "decode" else ("f16", "bf16"):
         for again in range(4):
             if kind == "decode":
@@ -41,9 +41,9 @@ def main(kind):
                 run_attend([600] * 6, [20] * 6, 4, 1, 64, 32, dtype, seed=again)  # both streams have each row
                 run_attend([1500], [90], 3, 1, 128, 64, dtype, seed=again, window=1000)  # Q by lanes
     share = done_over([1] * 64 if kind == "decode" else [30, 40])
-    assert share == 1 if polls == "0" else share == 0 if polls is None else True, (polls, share)
+    assert share == 1 if one_in == "1" else share == 0 if one_in is None else True, (one_in, share)
     torch.cuda.synchronize()
-    print("right", polls, share)
+    print("right", one_in, share)
 
 
 if __name__ == "__main__":

@@ -212,13 +212,18 @@ def test_pages_that_are_not_contiguous_are_refused():
 
 # ---------------------------------------------------------------- waits that run out
 
-def child(kind, polls):
-    env = dict(os.environ, **({} if polls is None else dict(TL_PAGED_WAIT_POLLS=str(polls))))
+def child(kind, one_in):
+    env = dict(os.environ, **({} if one_in is None else dict(TL_PAGED_FAIL_WAITS=str(one_in))))
     r = subprocess.run([sys.executable, os.path.join(os.path.dirname(__file__), "paged_waits_child.py"), kind], env=env,
                        capture_output=True, text=True, timeout=240)
-    assert r.returncode == 0 and f"right {polls}" in r.stdout, r.stdout[-500:] + r.stderr[-3000:]
+    assert r.returncode == 0 and f"right {one_in}" in r.stdout, r.stdout[-500:] + r.stderr[-3000:]
 
 
-@pytest.mark.parametrize("polls", [None, 0, 1, 20, 100])
-def test_decode_rows_whose_copies_were_not_waited_for_are_done_over(polls):
-    child("decode", polls)
+@pytest.mark.parametrize("one_in", [None, 1, 100, 1000])
+def test_decode_rows_whose_copies_were_not_waited_for_are_done_over(one_in):
+    child("decode", one_in)
+
+
+@pytest.mark.parametrize("one_in", [None, 1, 100, 1000])
+def test_chunk_rows_whose_products_were_not_waited_for_are_done_over(one_in):
+    child("chunks", one_in)

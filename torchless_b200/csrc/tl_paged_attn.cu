@@ -70,16 +70,15 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
-// Waits by polling (the copies are short, and a suspended wait may wake late); false after ~2 s, or that many polls.
-__device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity, unsigned polls) {
-    if (polls == 0) return false;
+// Waits by polling (the copies are short, and a suspended wait may wake late); false after ~2 s.
+__device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity, unsigned fail_one_in) {
+    if (fail_one_in != 0 && told_to_fail(fail_one_in)) return false;
     if (bar_test_now(b, parity)) return true;
     const unsigned long long t0 = gtime();
-    for (unsigned i = 1; i != polls; i++) {
+    for (unsigned i = 1;; i++) {
         if (bar_test_now(b, parity)) return true;
         if ((i & 255) == 0 && gtime() - t0 > kTimeoutNs) return false;
     }
-    return false;
 }
 
 // Keys per step, stages per warp, and the bytes of one side of a stage.
@@ -587,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (s >= c.end - P::kTileCost) break;
             if (ahead == 0) continue;  // (a copy never came: no further ones)
             // (the outcome is the whole warp's: what follows exchanges values between its lanes)
-            if (!__all_sync(FULL, spin(&bars[got_st], (got_parity >> got_st) & 1, a.polls))) {
+            if (!__all_sync(FULL, spin(&bars[got_st], (got_parity >> got_st) & 1, a.fail_one_in))) {
                 dead = true;  // and the copies on their way land before anything else happens to their stages
                 for (; ahead > 0; ahead--) {
                     bar_wait(&bars[got_st], (got_parity >> got_st) & 1);
@@ -726,14 +725,13 @@ using namespace tl;
 using namespace tl::paged;
 
 namespace {
-// TL_PAGED_WAIT_POLLS: a limit on the polls of the kernels' waits, for tests of what follows when one runs out.
-unsigned wait_polls() {
-    static const unsigned polls = [] {
-        const char* e = std::getenv("TL_PAGED_WAIT_POLLS");
-        const long v = e ? std::atol(e) : -1;
-        return v >= 0 && v < 0x7fffffff ? static_cast<unsigned>(v) : kNoPollLimit;
+// TL_PAGED_FAIL_WAITS=n: about one in n waits of the kernels gives up at once, for tests of what follows.
+unsigned fail_one_in() {
+    static const unsigned n = [] {
+        const char* e = std::getenv("TL_PAGED_FAIL_WAITS");
+        return e ? static_cast<unsigned>(std::max(0, std::atoi(e))) : 0u;
     }();
-    return polls;
+    return n;
 }
 
 // Rows per sequence and kv head, on average, from which the kernels for chunks pay: this file's kernel reads all keys
@@ -806,7 +804,7 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.cap = static_cast<int>(std::min<size_t>(max_blocks << a.shift, kMaxLen));
     a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
     a.scale = scale == 0.f ? 1e-45f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
-    a.polls = wait_polls();
+    a.fail_one_in = fail_one_in();
     if (!many_rows(cache, n_tokens, n_heads, n_seq)) return attend_split(a, cache, workspace, as_stream(stream));
     return cache->dtype == TL_F32 ? attend_chunk_f32(a, cache, workspace, as_stream(stream))
                                   : attend_chunk(a, cache, workspace, as_stream(stream));

@@ -26,9 +26,11 @@ struct AttendArgs {
     int window;   // 0: none
     float scale;
     unsigned long long group_inv;  // ceil(2^64 / group)
-    unsigned polls;  // after so many a role's wait gives up, as it does after about 2 s (kNoPollLimit: only then)
+    unsigned fail_one_in;  // 0; for tests: about one in so many waits gives up at once, as all do after about 2 s
 };
-constexpr unsigned kNoPollLimit = 0xffffffffu;
+__device__ __forceinline__ bool told_to_fail(unsigned one_in) {
+    return ((static_cast<unsigned>(clock()) + 977u * blockIdx.x) * 2654435761u >> 8) % one_in == 0;
+}
 
 // r / group, r >= 0 (exact: r < 2^32, and the inverse is off by less than 2^-32 relative)
 __device__ __forceinline__ int div_group(const AttendArgs& a, int r) {

@@ -143,12 +143,14 @@ __device__ __forceinline__ void mma4_ts(uint32_t b, uint32_t acc) {
         "r"(acc), "r"(D), "r"(ID), "r"(HI), "r"(A), "r"(A + 8), "r"(A + 16), "r"(A + 24));
 }
 
-__device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
-    return bar_spin_ab(b, parity, abort_flag);
+__device__ __noinline__ bool fails(unsigned one_in) { return told_to_fail(one_in); }
+
+__device__ __noinline__ bool wait_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned fail_one_in) {
+    return !(fail_one_in != 0 && fails(fail_one_in)) && bar_spin_ab(b, parity, abort_flag);
 }
 
-__device__ __noinline__ bool doze_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
-    return bar_wait_ab(b, parity, abort_flag);
+__device__ __noinline__ bool doze_slow(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned fail_one_in) {
+    return !(fail_one_in != 0 && fails(fail_one_in)) && bar_wait_ab(b, parity, abort_flag);
 }
 
 // All threads of a stream meet; whether `good` holds for all of them.
@@ -305,8 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     auto fail = [&] { *abort_flag = 1; };
     // waits poll: the hand-offs here are short and frequent
-    auto wait = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || wait_slow(b, parity, abort_flag); };
-    auto doze = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || doze_slow(b, parity, abort_flag); };
+    auto wait = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || wait_slow(b, parity, abort_flag, a.fail_one_in); };
+    auto doze = [&](uint64_t* b, uint32_t parity) { return bar_test_now(b, parity) || doze_slow(b, parity, abort_flag, a.fail_one_in); };
 
     if (warp == 16) {
         // ---- TMA: K_j, V_j of each key tile; lane = one page's rows of one panel ----
@@ -662,6 +664,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 w0 = mt == -INFINITY ? 1.f : ex2(m0 - mt);
                 w1 = mt == -INFINITY ? 1.f : ex2(m1 - mt);
                 lt = xl[128 + r] * w0 + xl[384 + r] * w1;
+                // Warps that gave up do not wait here, and may arrive twice in one phase: what was read need not be this
+                // tile's.  They set the flag before they arrive.
+                __syncwarp();
+                if (*abort_flag) lt = NAN;
                 tc_fence_after();
             }
             const bool whole = c.s == 0 && c.end == c.steps;
@@ -682,9 +688,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (t0) {
                         tmem_ld16_async(ta + col, o);
                         tmem_wait_ld();
-                    } else {
+                    } else {  // (a part of a warp that gave up is not finite in its own columns either)
+                        const uint32_t none = fine ? 0u : 0x7fc00000u;
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = 0u;
+                        for (int e = 0; e < 16; e++) o[e] = none;
                     }
                     if (fold && fine) {
                         uint32_t o1[16];
