@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 import paged_plain as plain
-from test_paged_gpu import DT, TYPES, attend_case, check_attend, f32, f64, i32, ops, rope_case, run_sample, u
+from test_paged_gpu import DT, TYPES, attend_case, check_attend, check_rope, f32, f64, i32, ops, rope_case, run_sample, u
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -208,6 +208,35 @@ def test_pages_that_are_not_contiguous_are_refused():
             attend(q, bad, bad, np.zeros((1, 1), np.int32), [0, 1], [1])
     with pytest.raises(ValueError, match="layout"):  # unlike strides between the pages
         attend(q, kc[::2], kc[:3], np.zeros((1, 1), np.int32), [0, 1], [1])
+
+
+# ---------------------------------------------------------------- cache writes
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_tokens_with_one_slot_leave_every_other_row_right(dtype):
+    q_out, kc, vc, big, qkv, pos, slots, cos, sin, wq, wk = rope_case(30, 4, 2, 64, 16, 64, "f32", dtype, "both", page_pad=16)
+    slots[9] = slots[4]
+    before = [f64(t) for t in (q_out, kc, vc)]
+    ops().qk_norm_rope(q_out, kc, vc, qkv, pos, slots, cos, sin, wq, wk)
+    page, row = divmod(int(slots[4]), 16)
+    kept = kc[page, :, row].clone(), vc[page, :, row].clone()
+    # either token's values may stand in the shared slot: the two are compared with each token in its turn
+    right = []
+    for last in (4, 9):
+        s = slots.clone()
+        s[13 - last] = -1  # the other of 4 and 9
+        c = [torch.from_numpy(b).cuda().to(kc.dtype) for b in before]
+        ops().qk_norm_rope(*c, qkv, pos, s, cos, sin, wq, wk)
+        right.append([x[page, :, row] for x in c[1:]])
+        check_rope(*c, qkv, pos, s, cos, sin, wq, wk, dtype, before)
+        for x, y in zip((q_out, kc, vc), c):
+            y = y.clone()
+            if x is not q_out:
+                y[page, :, row] = x[page, :, row]
+            assert torch.equal(x, y)
+    for got, a, b in zip(kept, *right):
+        assert ((got == a) | (got == b)).all()
+    assert (big[:, :, 2 * 16 * 64:] == 7).all()
 
 
 # ---------------------------------------------------------------- waits that run out

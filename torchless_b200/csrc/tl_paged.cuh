@@ -10,7 +10,7 @@
 namespace tl {
 namespace paged {
 
-// 8 consecutive elements <-> fp32, one 16-byte access (two for fp32).
+// 8 consecutive elements rounded from fp32 (fp32 ones are read too), one 16-byte access (two for fp32).
 template <typename T>
 struct Vec8;
 template <>
@@ -27,16 +27,6 @@ struct Vec8<float> {
 };
 template <>
 struct Vec8<__half> {
-    static __device__ __forceinline__ void load(float (&v)[8], const __half* p) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const __half2* h = reinterpret_cast<const __half2*>(&u);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 f = __half22float2(h[j]);
-            v[2 * j] = f.x;
-            v[2 * j + 1] = f.y;
-        }
-    }
     static __device__ __forceinline__ void store(__half* p, const float (&v)[8]) {
         __half2 h[4];
 #pragma unroll
@@ -46,16 +36,6 @@ struct Vec8<__half> {
 };
 template <>
 struct Vec8<__nv_bfloat16> {
-    static __device__ __forceinline__ void load(float (&v)[8], const __nv_bfloat16* p) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 f = __bfloat1622float2(h[j]);
-            v[2 * j] = f.x;
-            v[2 * j + 1] = f.y;
-        }
-    }
     static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[8]) {
         __nv_bfloat162 h[4];
 #pragma unroll
