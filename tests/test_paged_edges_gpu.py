@@ -178,6 +178,17 @@ def test_lengths_below_zero(dtype, new):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,new", [([3, 90, 2], [8, 1, 1]), ([10, 90], [60, 40])])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 8, 2 ** 31, 2 ** 40])
+def test_the_largest_windows(dtype, lens, new, window):
+    """More than any length is no window, also beside queries that stand before position 0."""
+    q, kc, vc, table, q_start, ln = attend_case(lens, new, 4, 2, 64, 16, dtype)
+    out = attend(q, kc, vc, table, q_start, ln, window=window)
+    check_attend(out, q, kc, vc, table, q_start, ln, dtype)
+    assert torch.equal(out, attend(q, kc, vc, table, q_start, ln))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tokens", [1, 30])
 def test_one_kv_head_and_one_page_in_any_layout(dtype, tokens):
     """A dimension of size 1 has no layout: a cache kept as [n_blocks, block_size, 1, head_dim] is the same pages, and K may

@@ -58,7 +58,7 @@ __device__ __forceinline__ int first_pos(const AttendArgs& a, int b, int n) { re
 // (pages that do not exist are left out later, key by key).
 __device__ __forceinline__ void attended(const AttendArgs& a, int p, int& lo, int& hi) {
     hi = min(p + 1, a.cap);
-    lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
+    lo = a.window > 0 ? max(0, max(p, 0) + 1 - a.window) : 0;  // (p may be far below 0, the window near the largest int)
 }
 
 // The page of position key of sequence b; -1 if there is none.
