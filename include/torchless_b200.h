@@ -263,22 +263,26 @@ TL_API tl_status tl_qk_norm_rope(void* q_out, const tl_paged_cache* cache, const
 /* Causal GQA attention of new tokens over the pages (modules.cpp:65-88 for
  * many sequences; q head h reads kv head h / (n_heads / n_kv_heads)).
  * Sequence b has the query rows q_start[b] .. q_start[b + 1) and seq_lens[b]
- * cached tokens (below 0: none), the queries' own among them: its i-th query of n stands at
- * position p = seq_lens[b] - n + i and attends to the positions
- * max(0, p - window + 1) .. p (window 0: all of 0 .. p) whose table entry
- * names a page of the cache.  What is not attended (other sequences' pages,
- * rows of a page behind the sequence, entries out of range) does not reach the
- * result, not even as NaN or infinity.  A query that attends to nothing gets
- * zeros.  A single query per sequence is a decode step.
+ * cached tokens (below 0: none; above 0x7fff0000: that many), the queries' own
+ * among them: its i-th query of n stands at position p = seq_lens[b] - n + i
+ * and attends to the positions max(0, p - window + 1) .. p (window 0, or 2^30
+ * and more: all of 0 .. p) whose table entry names a page of the cache.  What
+ * is not attended (other sequences' pages, rows of a page behind the sequence,
+ * entries out of range) does not reach the result, not even as NaN or infinity.
+ * A query that attends to nothing gets zeros.  A single query per sequence is a
+ * decode step.
  *   q    rows of n_heads x head_dim, q_stride elements apart; out [n_tokens]
  *        [n_heads][head_dim], both in the cache's dtype, not overlapping
  *   block_table [n_seq][max_blocks]; q_start [n_seq + 1], not decreasing
  * Rows outside q_start[0] .. q_start[n_seq] stay as they were.  Scores and sums
- * are fp32 (fp64, key by key, for rows whose scores pass it); with fp16 / bf16 caches the weights of the values are rounded to
- * that type for the tensor cores.  `workspace` holds the partial results
- * of split sequences: tl_paged_attention_workspace bytes, 16-byte aligned, its
- * contents need no preparation; calls that may overlap in time need one each.
- * A captured call keeps using the workspace it was captured with. */
+ * are fp32 (fp64, key by key, for rows whose scores or sums pass it); with fp16
+ * and bf16 caches, from 17 rows a sequence and kv head on average, the weights
+ * of the values are rounded to that type for the tensor cores.  A call of more
+ * than 2^40 (tiles of 16 rows of one kv head) x (keys they attend to) is not
+ * done.  `workspace` holds the partial results of split sequences:
+ * tl_paged_attention_workspace bytes, 16-byte aligned, its contents need no
+ * preparation; calls that may overlap in time need one each.  A captured call
+ * keeps using the workspace it was captured with. */
 TL_API tl_status tl_paged_attention_workspace(const tl_paged_cache* cache, size_t n_tokens, size_t n_heads,
                                               size_t n_seq, size_t max_blocks, size_t* bytes);
 TL_API tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl_paged_cache* cache,

@@ -71,13 +71,24 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
 }
 
 // Waits by polling (the copies are short, and a suspended wait may wake late); false after ~2 s.
-__device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity, unsigned fail_one_in) {
+__device__ __noinline__ bool spin_slow(uint64_t* b, uint32_t parity, unsigned fail_one_in) {
     if (fail_one_in != 0 && told_to_fail(fail_one_in)) return false;
-    if (bar_test_now(b, parity)) return true;
     const unsigned long long t0 = gtime();
     for (unsigned i = 1;; i++) {
         if (bar_test_now(b, parity)) return true;
         if ((i & 255) == 0 && gtime() - t0 > kTimeoutNs) return false;
+    }
+}
+__device__ __forceinline__ bool spin(uint64_t* b, uint32_t parity, unsigned fail_one_in) {
+    return (bar_test_now(b, parity) && fail_one_in == 0) || spin_slow(b, parity, fail_one_in);
+}
+
+// Waits for the copies of `n` stages from st on.
+template <int NST>
+__device__ __noinline__ void drain(uint64_t* bars, int st, uint32_t parity, int n) {
+    for (; n > 0; n--) {
+        bar_wait(&bars[st], (parity >> st) & 1);
+        st = st + 1 == NST ? 0 : st + 1;
     }
 }
 
@@ -160,7 +171,8 @@ struct Core {
     static_assert(R == 16, "the instruction's height");
     static constexpr int NO = HD / 8;
     // fp16 ends at 2^-24, and many weights below that may add up to a result: they are formed, and summed, 2^15 times as
-    // large, which the largest of 1 has room for.  bf16 has fp32's range.
+    // large, which the largest of 1 has room for.  (Where scores beyond 2^24 round that to 2^16, an infinity, the rows are
+    // done over.)  bf16 has fp32's range.
     static constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
     uint32_t q[HD / 16][4];
     float o[NO][4];
@@ -274,14 +286,15 @@ struct Core {
             mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
             const float mn = fmaxf(m[i], mx);
-            const float base = mn == -INFINITY ? 0.f : mn;
+            float base = mn == -INFINITY ? 0.f : mn;
             f[i] = ex2(m[i] - base);
             m[i] = mn;
+            if (kLift != 0.f) base -= kLift;
             float sum = 0.f;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) s[n][2 * i + e] = ex2(s[n][2 * i + e] - base + kLift);
+                for (int e = 0; e < 2; e++) s[n][2 * i + e] = ex2(s[n][2 * i + e] - base);
                 sum += s[n][2 * i] + s[n][2 * i + 1];
             }
             l[i] = l[i] * f[i] + sum;
@@ -587,12 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ahead == 0) continue;  // (a copy never came: no further ones)
             // (the outcome is the whole warp's: what follows exchanges values between its lanes)
             if (!__all_sync(FULL, spin(&bars[got_st], (got_parity >> got_st) & 1, a.fail_one_in))) {
-                dead = true;  // and the copies on their way land before anything else happens to their stages
-                for (; ahead > 0; ahead--) {
-                    bar_wait(&bars[got_st], (got_parity >> got_st) & 1);
-                    got_parity ^= 1u << got_st;
-                    got_st = got_st + 1 == NST ? 0 : got_st + 1;
-                }
+                dead = true;  // and the copies on their way land before the block ends
+                drain<NST>(bars, got_st, got_parity, ahead);
+                ahead = 0;
                 continue;
             }
             got_parity ^= 1u << got_st;
@@ -802,7 +812,7 @@ tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, const tl
     a.n_blocks = static_cast<int>(cache->n_blocks);
     a.shift = __builtin_ctzll(cache->block_size);
     a.cap = static_cast<int>(std::min<size_t>(max_blocks << a.shift, kMaxLen));
-    a.window = window == 0 || window > 0x7fffffffull ? 0 : static_cast<int>(window);
+    a.window = window >= 1ull << 30 ? 0 : static_cast<int>(window);
     a.scale = scale == 0.f ? 1e-45f : scale;  // (a masked score is -inf, which no factor may turn into NaN)
     a.fail_one_in = fail_one_in();
     if (!many_rows(cache, n_tokens, n_heads, n_seq)) return attend_split(a, cache, workspace, as_stream(stream));

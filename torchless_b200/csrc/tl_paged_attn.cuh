@@ -23,7 +23,7 @@ struct AttendArgs {
     size_t q_stride, block_stride;
     int n_seq, n_tokens, H, KV, group, max_blocks, n_blocks, shift;  // block size 1 << shift
     int cap;      // positions that a table can name, at most kMaxLen
-    int window;   // 0: none
+    int window;   // 0: none; below 2^30, so that no difference of it and a position passes 32 bits
     float scale;
     unsigned long long group_inv;  // ceil(2^64 / group)
     unsigned fail_one_in;  // 0; for tests: about one in so many waits gives up at once, as all do after about 2 s
@@ -58,7 +58,7 @@ __device__ __forceinline__ int first_pos(const AttendArgs& a, int b, int n) { re
 // (pages that do not exist are left out later, key by key).
 __device__ __forceinline__ void attended(const AttendArgs& a, int p, int& lo, int& hi) {
     hi = min(p + 1, a.cap);
-    lo = a.window > 0 ? max(0, max(p, 0) + 1 - a.window) : 0;  // (p may be far below 0, the window near the largest int)
+    lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
 }
 
 // The page of position key of sequence b; -1 if there is none.
