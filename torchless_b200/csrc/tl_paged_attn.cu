@@ -21,10 +21,11 @@
 //   - At a tile's end the warps join (max, sum, accumulator) in shared memory;
 //     a tile that continues in another block leaves its part in the workspace,
 //     and a second small kernel joins the parts in order.
-// 32 heads, 8 kv heads, hd 128, one token a sequence: 64 x 4096 keys bf16 178 us (6.0 TB/s of 6.55 that a copy reaches),
-// fp32 329 us (6.5 TB/s), 64 ragged lengths of at most 4096 fp16 70 us (5.3 TB/s); 1 x 8192 bf16 15.4 us, where finding
-// the shares (2.7 us), the first copies, the join and the launches count more than the 5.1 us of reading.  A tile
-// costs about 3 us beside its keys: 200 x 300 keys 73 us (3.4 TB/s).
+// 32 heads, 8 kv heads, hd 128, one token a sequence: 64 x 4096 keys bf16 177 us (6.1 TB/s of 6.55 that a copy reaches),
+// hd 64 94 us, fp32 333 us (6.45 TB/s; 24 us more where 512 MB were written before it, whose last part leaves L2
+// meanwhile), 64 ragged lengths of at most 4096 fp16 69 us (5.4 TB/s); 1 x 8192 bf16 15.1 us, where finding the shares
+// (2.7 us), the first copies, the join and the launches count more than the 5.1 us of reading.  A tile costs about 3 us
+// beside its keys: 200 x 300 keys 73 us (3.4 TB/s).
 #include <math.h>
 
 #include <algorithm>
@@ -103,9 +104,10 @@ struct Shape {
 };
 
 // Steps of KS keys, tiles of R rows.  Beginning and ending a tile takes about as long as kTileCost steps, which count
-// as steps before its first key, so that a batch of short sequences is shared as evenly as one of long ones (64 ragged
-// lengths of at most 4096: 12 steps 78.8 us, 16 73.7, 24 69.9, 32 69.9, 48 74.4 us; where all are alike it makes no
-// difference).  A tile without keys counts one step more, so that its zeros get written.
+// as steps before its first key, so that a batch of short sequences is shared as evenly as one of long ones.  64 ragged
+// lengths of at most 4096, 12 / 16 / 24 / 32 steps: fp16 (steps of 16 keys) 78 / 73 / 68 / 69 us, bf16 hd 64 (32 keys)
+// 54.1 / 51.1 / 49.5 / 52.2, fp32 (8 keys) 125.8 / 122.5 / 120.6 / 122; where all are alike (200 x 300) it makes no
+// difference.  A tile without keys counts one step more, so that its zeros get written.
 template <int R_, int KS>
 struct SplitPlan {
     static constexpr int R = R_;

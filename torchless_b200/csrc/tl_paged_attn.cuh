@@ -94,9 +94,9 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs& a, int b, int rt, int 
 // The steps of all tiles lie in one line: sequence by sequence, row tile by row
 // tile, kv head by kv head.  Block i takes the steps [i * per, (i + 1) * per).
 // `Plan` says how many rows a tile has (R) and how many steps, and (kLookAgain) whether a tile's lengths are looked up
-// again for the next kv head.  That only costs time (8192 tokens bf16: 604 us against 594, many short sequences 3 %), but
-// some kernels' registers come out better with it (fp32: 2048 tokens of 4096 2.46 ms against 2.60, decode 64 x 4096 329 us
-// against 337; decode 64 x 4096 bf16 hd 64 92.6 us against 95.8).
+// again for the next kv head.  That only costs time (8192 tokens bf16: 614 us against 602, 130 short sequences 42.4 against
+// 41.3), but some kernels' registers come out better with it (2048 tokens of 4096 fp32 2.47 ms against 2.61, decode 64 x
+// 4096 bf16 hd 64 94.2 us against 96.2; decode fp32 333 us both ways).
 
 // What a block leaves behind of a tile that it begins and others end.
 struct Head {

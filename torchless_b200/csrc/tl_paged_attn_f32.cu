@@ -17,7 +17,7 @@
 //   - Two blocks an SM: one takes exponentials while the other multiplies.
 // Blocks have equal shares of the key tiles (tl_paged_attn.cuh).
 // Bound by the FMA pipes and by what two warps a scheduler can hide: 2048 tokens of 4096, 32 heads, 8 kv heads, hd 128:
-// 2.46 ms, 41.9 TFLOP/s of 72 that the pipes have (plain FMAs: 2.99 ms); 512 of 1024: 191 us (in 16-row tiles of the
+// 2.47 ms, 41.7 TFLOP/s of 72 that the pipes have (plain FMAs: 2.99 ms); 512 of 1024: 192 us (in 16-row tiles of the
 // decode kernel 395 us).  128 rows in one block of 256 threads: the same where rows abound, and 229 instead of 130 us
 // for 16 sequences of 20 rows.
 #include <math.h>

@@ -31,8 +31,8 @@
 // What bounds it: a step of 256 rows x 128 keys is 2048 cycles of the matrix unit and as many of the special function
 // units (one exponential a score at 8 cycles a warp); it takes about 4100, since a stream's scores wait for its last
 // product and its exponentials for the scores, and two streams cover that only in part.  32 heads, 8 kv heads, hd 128,
-// bf16: 2048 tokens of 4096 122 us (845 TFLOP/s, of 1675 that a large product reaches), 2048 of 2048 70 us, a prompt of
-// 8192 594 us (925 TFLOP/s), 256 of 4096 35.5 us; hd 64, 2048 of 4096 111 us.  Some 20 us of a call are its
+// bf16: 2048 tokens of 4096 123 us (840 TFLOP/s, of 1675 that a large product reaches), 2048 of 2048 71 us, a prompt of
+// 8192 602 us (913 TFLOP/s), 256 of 4096 36 us; hd 64, 2048 of 4096 111 us.  Some 20 us of a call are its
 // beginning (finding the shares 3.3 us, first copies 2 us), the tiles' epilogues and the join.
 #include <math.h>
 
@@ -57,8 +57,9 @@ struct Range {  // log2 units
 };
 
 // One step: 256 rows x 128 keys, or (tiles of at most 128 rows) 128 rows x 256 keys.  Beginning and ending a
-// tile takes about as long as kTileCost steps, which count as steps before its first key tile (2048 tokens of 4096 / 9
-// ragged chunks: 0 steps 136 / 51 us, 2 130 / 49, 4 129 / 51).
+// tile takes about as long as kTileCost steps, which count as steps before its first key tile.  0 / 2 / 4 steps: 2048
+// tokens of 4096 bf16 128 / 124 / 127 us, 2048 of 2048 138 / 71 / 66, 9 ragged chunks of at most 389 tokens fp16 146 / 108 /
+// 110, 9 x 200 tokens of 2000 117 / 109 / 105.
 struct ChunkPlan {
     static constexpr int R = kRows;
     static constexpr int kTileCost = 2;
