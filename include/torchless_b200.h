@@ -307,10 +307,10 @@ TL_API tl_status tl_paged_attention(void* out, const void* q, size_t q_stride, c
  * logit, or with -inf alone, gives n - 1 at a temperature > 0, as
  * tl_sample_multinomial does.
  * Weights are fp64 rounded to multiples of 2^-40 and summed exactly, so the
- * result does not depend on the order of the sums.  logits: n values per row
- * in `dtype`, row_stride elements apart; n < 2^22.  Rows of more than 262141
- * values take a way that reads them many times and is 4 to 15 times as long.
- * No allocation. */
+ * result does not depend on the order of the sums; what rounds to 0 is never
+ * drawn, not at r = 0 either.  logits: n values per row in `dtype`, row_stride
+ * elements apart; n < 2^22.  Rows of more than 262141 values take a way that
+ * reads them many times and is 4 to 15 times as long.  No allocation. */
 TL_API tl_status tl_sample_rows(uint32_t* out, const void* logits, tl_dtype dtype, size_t row_stride, size_t n_rows,
                                 size_t n, const float* r, const float* temperature, const int32_t* top_k,
                                 const float* top_p, const float* min_p, void* stream);

@@ -620,10 +620,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             ahead--;
             __syncwarp();  // every lane has read the stage
         }
-        // A result that is not finite: a value that one row must not see may have met it as 0 x infinity,
-        // or an infinite value the split weights, or values near the type's largest add up to more.  Such a tile is done over row by row, which gives the
-        // formula's result to each.  The same where a score passed fp32's range or a copy never came, and for a row whose
-        // weights are all 0: it attends to nothing, or all its scores lie below that range.
+        // A result that is not finite: a value that one row must not see may have met it as 0 x infinity, or an infinite
+        // value the split weights, or values near the type's largest add up to more.  Such a tile is done over row by
+        // row, which gives the formula's result to each.  The same where a score passed fp32's range or a copy never
+        // came, and for a row whose weights are all 0: it attends to nothing, or all its scores lie below that range.
         const bool redo = core.finish(c.t.nrows, lane) || dead;
         const bool whole = c.s == 0 && c.end == c.steps;
         float* part = parts + (static_cast<size_t>(blockIdx.x) * 2 + (first_tile ? 0 : 1)) * R * (HD + 4);
